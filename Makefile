@@ -8,9 +8,11 @@ ARCH ?= gfx950
 BUILD := build
 SRC := embedding.cpp_amd/csrc
 INC := -Iinclude -I$(SRC)
-HOST_SRCS := gguf_io.cpp quantize.cpp quantize_model.cpp synth.cpp tokenizer.cpp runtime.cpp
+HOST_SRCS := gguf_io.cpp quantize.cpp quantize_model.cpp synth.cpp tokenizer.cpp runtime.cpp ops_api.cpp
 HOST_OBJS := $(addprefix $(BUILD)/obj/,$(HOST_SRCS:.cpp=.o))
 HIP_OBJS := $(BUILD)/obj/kernels.o $(BUILD)/obj/gemm_i8.o
+# the operators around the encoder
+OPS_OBJS := $(BUILD)/obj/ops_linear.o $(BUILD)/obj/ops_rows.o $(BUILD)/obj/ops_adamw.o
 # the library's sources, in the order bench.py's src_hash() reads them
 SRC_HASH_FILES := $(sort $(wildcard $(SRC)/*.hip $(SRC)/*.cpp $(SRC)/*.h $(SRC)/*.inc include/*.h include/ggml/*.h)) Makefile
 CXXFLAGS := -O2 -std=c++17 -fPIC -fvisibility=hidden -ffp-contract=off -Wall -Wno-unused-function -Wno-unused-result \
@@ -29,7 +31,12 @@ $(BUILD)/obj/%.o: $(SRC)/%.hip $(SRC)/kernels.h $(SRC)/kernels_common.h $(SRC)/i
 	@mkdir -p $(dir $@)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
-$(BUILD)/libbert.so: $(HOST_OBJS) $(HIP_OBJS)
+# the operators are built without the packed f32 instructions
+$(BUILD)/obj/ops_%.o: $(SRC)/ops_%.hip $(SRC)/ops.h $(SRC)/ops_common.h include/bert_amd.h
+	@mkdir -p $(dir $@)
+	$(HIPCC) $(HIPFLAGS) -Xclang -target-feature -Xclang -packed-fp32-ops -c $< -o $@
+
+$(BUILD)/libbert.so: $(HOST_OBJS) $(HIP_OBJS) $(OPS_OBJS)
 	$(HIPCC) -shared -fPIC --offload-arch=$(ARCH) -o $@ $^ -lpthread
 	@# the commit this library was built from (bench.py / tools/pmc_traffic.py record it), and a
 	@# hash of the sources it was built from (bench.py compares it with the tree it runs in, so a

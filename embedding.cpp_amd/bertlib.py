@@ -37,6 +37,9 @@ EXT_SYMBOLS = [
     "bert_amd_profile_enable", "bert_amd_profile_read", "bert_amd_synth_model", "bert_amd_tokenize_json",
     "bert_amd_debug_embed", "bert_amd_workspace_rows", "bert_amd_last_error", "bert_amd_load_opts",
     "bert_amd_debug_layers", "bert_amd_set_option", "bert_amd_get_option", "bert_amd_shard_cuts",
+    "bert_amd_linear", "bert_amd_linear_workspace", "bert_amd_linear_backward", "bert_amd_linear_backward_workspace",
+    "bert_amd_lookup", "bert_amd_lookup_grad", "bert_amd_lookup_grad_workspace", "bert_amd_word_table",
+    "bert_amd_adamw", "bert_amd_adamw_moments",
 ]
 
 # model shapes of BASELINE.json's configs
@@ -109,6 +112,23 @@ def lib() -> ctypes.CDLL:
     L.bert_amd_workspace_rows.restype = ctypes.c_int64
     L.bert_amd_workspace_rows.argtypes = [ctypes.c_void_p, ctypes.c_int32]
     L.bert_amd_last_error.restype = ctypes.c_char_p
+    # the operators around the encoder (bertops.py)
+    i32, i64, p, f64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_double
+    for name, res, args in (
+        ("bert_amd_linear_workspace", i64, [i32, i64, i32, i32]),
+        ("bert_amd_linear", i32, [i32, i32, i32, i64, i32, i32, p, i64, p, i64, p, p, i64, p, i64, p, i64, p, i64, p]),
+        ("bert_amd_linear_backward_workspace", i64, [i32, i32, i64, i32, i32]),
+        ("bert_amd_linear_backward", i32, [i32, i32, i32, i64, i32, i32, p, i64, p, i64, p, i64, p, i64, p, i64, p, i64,
+                                           p, p, i64, p]),
+        ("bert_amd_lookup", i32, [i32, i32, i32, i64, i32, i32, p, i64, p, ctypes.c_float, p, i64, p]),
+        ("bert_amd_lookup_grad_workspace", i64, [i64, i32, i32]),
+        ("bert_amd_lookup_grad", i32, [i32, i32, i64, i32, i32, p, i64, p, ctypes.c_float, i32, i32, p, i64, p, i64, p]),
+        ("bert_amd_word_table", i32, [p, i32, ctypes.POINTER(p), I_P, I_P, I_P, I_P]),
+        ("bert_amd_adamw", i32, [i32, i32, p, i32, i32, i32, f64, f64, f64, f64, i64, ctypes.c_uint32, p, p]),
+        ("bert_amd_adamw_moments", i32, [i32, i64, p, p, p, p, p, p, p]),
+    ):
+        getattr(L, name).restype = res
+        getattr(L, name).argtypes = args
     _lib = L
     return L
 
@@ -310,6 +330,16 @@ class BertModel:
         if self.lib.bert_amd_get_option(self.ctx, key.encode(), ctypes.byref(v)) != 0:
             raise ValueError(f"bert_amd_get_option({key}) failed: {last_error()}")
         return int(v.value)
+
+    def word_table(self, slot: int = 0):
+        """bert_amd_word_table: (device pointer, row type, n_rows, width, device) of a replica's word-embedding table."""
+        t = ctypes.c_void_p()
+        typ, rows, width, dev = (ctypes.c_int32() for _ in range(4))
+        rc = self.lib.bert_amd_word_table(self.ctx, slot, ctypes.byref(t), ctypes.byref(typ), ctypes.byref(rows),
+                                          ctypes.byref(width), ctypes.byref(dev))
+        if rc != 0:
+            raise RuntimeError(f"bert_amd_word_table failed ({rc}): {last_error()}")
+        return t.value, typ.value, rows.value, width.value, dev.value
 
     def workspace_rows(self, slot: int = 0) -> int:
         return int(self.lib.bert_amd_workspace_rows(self.ctx, slot))

@@ -1,0 +1,70 @@
+// ops_common.h — device helpers shared by the operator kernels (ops_*.hip).
+#pragma once
+#include "ops.h"
+
+namespace bertamd {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+// what each element type of bert_amd.h is on the device; 16 bytes hold CH of them
+template <int TYPE> struct Elem;
+template <> struct Elem<BERT_AMD_F32> { typedef float T; static constexpr int CH = 4; };
+template <> struct Elem<BERT_AMD_F16> { typedef _Float16 T; static constexpr int CH = 8; };
+template <> struct Elem<BERT_AMD_BF16> { typedef __bf16 T; static constexpr int CH = 8; };
+
+inline int elem_size(int type) { return type == BERT_AMD_F32 ? 4 : 2; }
+inline bool aligned16(const void *p, int64_t stride_bytes) {
+    return ((uintptr_t)p & 15) == 0 && (stride_bytes & 15) == 0;
+}
+template <typename T>
+constexpr T ceil_div(T a, T b) { return (a + b - 1) / b; }
+
+// Activations and their slopes in f32.  gelu is the tanh form that the
+// encoder's feed-forward layer uses, written z * sigmoid(2u): no cancellation
+// in its lower tail.
+// the exponential never overflows: a far tail fades out through the subnormals
+__device__ __forceinline__ float sigmoid_f(float v) {
+    const float t = expf(-fabsf(v));
+    return (v < 0.f ? t : 1.f) / (1.f + t);
+}
+constexpr float GELU_C = 0.7978845608028654f, GELU_K = 0.044715f;
+
+__device__ __forceinline__ float act_f(float z, int act) {
+    switch (act) {
+        case BERT_AMD_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
+        case BERT_AMD_ACT_GELU: return z * sigmoid_f(2.f * GELU_C * (z + GELU_K * z * z * z));
+        case BERT_AMD_ACT_GELU_ERF: return 0.5f * z * erfcf(-z * 0.70710678118654752f);
+        case BERT_AMD_ACT_SILU: return z * sigmoid_f(z);
+        case BERT_AMD_ACT_TANH: return tanhf(z);
+    }
+    return z;
+}
+// Past |z| = 90 every slope is 0 or 1 in f32: z is held there, so that no
+// product of an infinite factor and a vanished one makes a NaN (a NaN stays).
+__device__ __forceinline__ float act_slope_f(float z, int act) {
+    z = z > 90.f ? 90.f : z < -90.f ? -90.f : z;
+    switch (act) {
+        case BERT_AMD_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
+        case BERT_AMD_ACT_GELU: {
+            const float s = sigmoid_f(2.f * GELU_C * (z + GELU_K * z * z * z));
+            return s + z * s * (1.f - s) * 2.f * GELU_C * (1.f + 3.f * GELU_K * z * z);
+        }
+        case BERT_AMD_ACT_GELU_ERF:
+            return 0.5f * erfcf(-z * 0.70710678118654752f) + z * 0.3989422804014327f * expf(-0.5f * z * z);
+        case BERT_AMD_ACT_SILU: {
+            const float s = sigmoid_f(z);
+            return s + z * s * (1.f - s);
+        }
+        case BERT_AMD_ACT_TANH: {
+            const float t = tanhf(z);
+            return (1.f - t) * (1.f + t);
+        }
+    }
+    return 1.f;
+}
+
+}  // namespace bertamd

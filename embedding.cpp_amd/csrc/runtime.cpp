@@ -35,6 +35,7 @@
 #include "ggml_formats.h"
 #include "gguf_io.h"
 #include "kernels.h"
+#include "ops.h"
 #include "tokenizer.h"
 
 using namespace bertamd;
@@ -51,6 +52,12 @@ void set_err(const char *fmt, ...) {
     va_end(ap);
     g_err = buf;
 }
+
+}  // namespace
+
+void bertamd::set_last_error(const char *msg) { g_err = msg; }
+
+namespace {
 
 #define HIP_OK_RC(expr, rc)                                                           \
     do {                                                                              \
@@ -2409,6 +2416,20 @@ int64_t bert_amd_workspace_rows(bert_ctx *ctx, int32_t slot) {
     int64_t rows = 0;  // the largest lane (bert_encode_batch may have added lanes)
     for (auto &ln : ctx->reps[slot]->lanes) rows = std::max(rows, ln->ws.cap_rows);
     return rows;
+}
+
+int32_t bert_amd_word_table(bert_ctx *ctx, int32_t slot, const void **table, int32_t *type, int32_t *n_rows,
+                            int32_t *width, int32_t *device) {
+    if (!ctx || slot < 0 || slot >= (int32_t)ctx->reps.size() || !table || !type || !n_rows || !width || !device) {
+        set_err("bert_amd_word_table: invalid arguments");
+        return -1;
+    }
+    *table = ctx->reps[slot]->word;
+    *type = ctx->emb_raw ? (int32_t)ctx->word_t : (int32_t)BERT_AMD_F32;
+    *n_rows = ctx->hp.n_vocab;
+    *width = ctx->hp.n_embd;
+    *device = ctx->reps[slot]->device;
+    return 0;
 }
 
 const char *bert_amd_last_error(void) { return g_err.c_str(); }

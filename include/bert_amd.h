@@ -177,6 +177,136 @@ BERT_API int32_t bert_amd_get_option(struct bert_ctx *ctx, const char *key, int3
    coverage.  Returns 0, or -1 on invalid arguments. */
 BERT_API int32_t bert_amd_shard_cuts(int32_t n_seqs, const int32_t *n_tokens, int32_t n_replicas, int32_t *cut);
 
+/* ---------------------------------------------------------------------------
+   Operators around the encoder, on device tensors of the caller: a dense layer
+   and its gradients (a trained head or adapter on the embeddings), the lookup
+   of token rows and its gradient, and the AdamW step that trains them.
+
+   All of them run asynchronously on `hip_stream` (a hipStream_t; NULL = the
+   null stream of `device`), allocate nothing, copy nothing to or from the host
+   and may be captured into a HIP graph.  `device` is the HIP device that the
+   tensors and the stream belong to; the caller's current device is left as it
+   was.  Where a call takes a workspace, the caller gives device memory of at
+   least the bytes its *_workspace function names, 16-byte aligned; the call may
+   write all of it and keeps nothing in it for the next, so calls that may run
+   at the same time (two streams, two graphs) need one each.  Rows of a matrix
+   are `ld*` elements apart (at least its width; 0 for an input: the one row
+   again for every row); nothing is written between them.  Results do not
+   depend on the launch: the same inputs give the same bits.  Outputs must not
+   overlap inputs or each other unless a call says so.  Each returns 0, or
+   negative without having launched anything: -1 an invalid argument, -3 a HIP
+   error (message via bert_amd_last_error). */
+
+/* element types of the operators' tensors (ggml's numbers, as in the model files) */
+enum bert_amd_type {
+    BERT_AMD_F32 = 0,
+    BERT_AMD_F16 = 1,
+    BERT_AMD_Q4_0 = 2,
+    BERT_AMD_Q4_1 = 3,
+    BERT_AMD_BF16 = 30
+};
+
+/* activations; GELU is the tanh form the encoder's feed-forward layer uses,
+   GELU_ERF z/2 (1 + erf(z / sqrt 2)), SILU z / (1 + exp(-z)) */
+enum bert_amd_act {
+    BERT_AMD_ACT_NONE = 0,
+    BERT_AMD_ACT_RELU = 1,
+    BERT_AMD_ACT_GELU = 2,
+    BERT_AMD_ACT_GELU_ERF = 3,
+    BERT_AMD_ACT_SILU = 4,
+    BERT_AMD_ACT_TANH = 5
+};
+
+/* Dense layer: z = x W^T + bias, y = act(z) + residual.
+     type     : F32, F16 or BF16, of x, w, residual, y and z; sums are f32, each
+                output is rounded once
+     x, w     : [M][K], [N][K]; bias: f32 [N] or NULL; residual: [M][N] or NULL
+                (may be y itself, with ldr = ldy)
+     y        : [M][N]; z: [M][N] or NULL: the pre-activation, kept for
+                bert_amd_linear_backward
+   M = 0 does nothing; M < 2^31, 1 <= N, K < 2^22, and none of M N, M K and N K
+   over 2^34. */
+BERT_API int64_t bert_amd_linear_workspace(int32_t type, int64_t M, int32_t N, int32_t K);
+BERT_API int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int64_t M, int32_t N, int32_t K,
+                                 const void *x, int64_t ldx, const void *w, int64_t ldw, const float *bias,
+                                 const void *residual, int64_t ldr, void *y, int64_t ldy, void *z, int64_t ldz,
+                                 void *workspace, int64_t workspace_bytes, void *hip_stream);
+
+/* Its gradients from dy [M][N] (the residual's gradient is dy itself):
+   dz = dy act'(z), dx = dz W [M][K], dw = dz^T x [N][K], dbias = the sum of dz
+   over the rows, f32 [N].  z is not read (and may be NULL) for act NONE; it may
+   be any [M][N] values.  Any of dx, dw, dbias may be NULL: not computed.  F16
+   and BF16 round dz to the type before the two products.  M = 0 gives zero dw
+   and dbias. */
+BERT_API int64_t bert_amd_linear_backward_workspace(int32_t type, int32_t act, int64_t M, int32_t N, int32_t K);
+BERT_API int32_t bert_amd_linear_backward(int32_t device, int32_t type, int32_t act, int64_t M, int32_t N, int32_t K,
+                                          const void *dy, int64_t lddy, const void *z, int64_t ldz, const void *x,
+                                          int64_t ldx, const void *w, int64_t ldw, void *dx, int64_t lddx, void *dw,
+                                          int64_t lddw, float *dbias, void *workspace, int64_t workspace_bytes,
+                                          void *hip_stream);
+
+/* Token rows: out[i] = scale * table[ids[i]], in f32, rounded once to out_type
+   (F32, F16 or BF16).  An id outside [0, n_rows) gives a row of zeros (unlike
+   the encoder's own gather, whose ids are tokens of a checked batch).
+     table    : [n_rows][width] of table_type, F32, F16, BF16 or a GGUF's Q4_0 or
+                Q4_1 rows (width a multiple of 32; a block's values as ggml's
+                get_rows gives them), ld_table_bytes between rows
+     out      : [n][width] */
+BERT_API int32_t bert_amd_lookup(int32_t device, int32_t table_type, int32_t out_type, int64_t n, int32_t n_rows,
+                                 int32_t width, const void *table, int64_t ld_table_bytes, const int32_t *ids,
+                                 float scale, void *out, int64_t ldo, void *hip_stream);
+
+/* The table's gradient: dtable[v] = scale * (sum of dout[i] over the i with
+   ids[i] = v), f32, in one fixed order of i; every row is written, unused ones
+   as zero.  accumulate != 0 adds it to dtable instead and leaves unused rows
+   untouched.  Ids outside [0, n_rows) and pad_id (-1: none) have no gradient.
+     dout     : [n][width] of type F32, F16 or BF16; dtable: f32 [n_rows][width]
+   n <= 2^30, n_rows <= 2^30. */
+BERT_API int64_t bert_amd_lookup_grad_workspace(int64_t n, int32_t n_rows, int32_t width);
+BERT_API int32_t bert_amd_lookup_grad(int32_t device, int32_t type, int64_t n, int32_t n_rows, int32_t width,
+                                      const void *dout, int64_t ldd, const int32_t *ids, float scale, int32_t pad_id,
+                                      int32_t accumulate, float *dtable, int64_t ldt, void *workspace,
+                                      int64_t workspace_bytes, void *hip_stream);
+
+/* The word-embedding table of replica `slot` as bert_amd_lookup takes it (rows
+   contiguous); it belongs to the context and is read-only.  `type` is the
+   file's row type, or F32 where the context keeps an f32 copy ("emb_raw" 0). */
+BERT_API int32_t bert_amd_word_table(struct bert_ctx *ctx, int32_t slot, const void **table, int32_t *type,
+                                     int32_t *n_rows, int32_t *width, int32_t *device);
+
+/* One tensor of an AdamW step: n f32 weights p (updated), their gradient, and
+   the moments (updated; all zero before step 1).  state_bits 32: m and v are
+   f32 [n].  state_bits 8: codes, one byte each, [n], and the f32 scales
+   m_scale, v_scale [(n + 255) / 256] of each 256 elements.  copy: n updated
+   weights rounded to copy_type, or NULL. */
+struct bert_amd_adamw_tensor {
+    float *p;
+    const void *grad;
+    void *m, *v;
+    float *m_scale, *v_scale;
+    void *copy;
+    int64_t n;
+    double weight_decay;
+};
+
+/* One step over n_tensors tensors (a host array, not kept):
+     m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+     p = p (1 - lr weight_decay)
+         - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+   in f32.  g is grad (grad_type F32, F16 or BF16) times *grad_scale (one f32 in
+   device memory; NULL: 1).  8-bit states store m and sqrt(v) as small floats,
+   rounded up or down at random by `seed`, another one each step (unused with 32
+   bits).  An infinity or NaN in g makes its weight and moments NaN, with 8-bit
+   states the moments of its whole block of 256.  n <= 2^34; tensors must not overlap. */
+BERT_API int32_t bert_amd_adamw(int32_t device, int32_t n_tensors, const struct bert_amd_adamw_tensor *tensors,
+                                int32_t state_bits, int32_t grad_type, int32_t copy_type, double lr, double beta1,
+                                double beta2, double eps, int64_t step, uint32_t seed, const float *grad_scale,
+                                void *hip_stream);
+
+/* 8-bit moments as f32 values: m_out, v_out [n] (either may be NULL). */
+BERT_API int32_t bert_amd_adamw_moments(int32_t device, int64_t n, const void *m, const float *m_scale, const void *v,
+                                        const float *v_scale, float *m_out, float *v_out, void *hip_stream);
+
 BERT_API const char *bert_amd_last_error(void);
 
 #ifdef __cplusplus

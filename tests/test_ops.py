@@ -1,0 +1,751 @@
+"""The operators around the encoder (include/bert_amd.h, bertops.py) against plain implementations in
+64 bits, and what they refuse.
+
+Tolerances: a result rounded to type t is off by at most u(t) = finfo(t).eps / 2 of its value; a sum of n
+terms held in f32, in any order, by at most n 2^-24 of the sum of the terms' magnitudes; f32 operands may be
+taken as two 16-bit halves, 22 bits or more of them, which three products leave at most 3 * 2^-22 = 12 * 2^-24
+off; f32 evaluations of the activations by a few 2^-24 of the largest term in them (SLACK of them).
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+import bertlib
+
+torch = pytest.importorskip("torch")
+import bertops  # noqa: E402
+
+gpu = pytest.mark.gpu
+F64 = torch.float64
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U32 = 2.0**-24
+SLACK = 32
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    """Half the spacing of the smallest values: what rounding is off by next to zero."""
+    return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(g, *shape, std=1.0):
+    return torch.randn(*shape, generator=g, dtype=F64) * std
+
+
+def act64(z, act):
+    if act == "relu":
+        return torch.relu(z)
+    if act == "gelu":
+        return z * torch.sigmoid(2 * (2 / np.pi) ** 0.5 * (z + 0.044715 * z**3))
+    if act == "gelu_erf":
+        return 0.5 * z * torch.special.erfc(-z * 0.5**0.5)  # its lower tail has no cancellation
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    return torch.tanh(z) if act == "tanh" else z
+
+
+def strided(t, pad):
+    """The same values with rows `pad` elements further apart, the space between filled with NaN."""
+    wide = torch.full((t.shape[0], t.shape[1] + pad), float("nan"), dtype=t.dtype, device=t.device)
+    wide[:, : t.shape[1]] = t
+    return wide[:, : t.shape[1]]
+
+
+def close(got, want, tol, what):
+    got = got.detach().to("cpu", F64)
+    off = (got - want).abs() - tol
+    assert torch.isfinite(got).all(), what
+    assert (off <= 0).all(), f"{what}: {int((off > 0).sum())} of {off.numel()} too far, worst {float(off.max()):.3g} over its bound"
+
+
+# ---- the dense layer
+
+ODD = [(1, 1, 1), (1, 384, 384), (3, 5, 7), (17, 33, 65), (64, 64, 64), (130, 200, 72), (257, 128, 96), (5, 4100, 31), (300, 31, 1030)]
+
+
+def make_layer(M, K, N, dtype, seed=0):
+    g = gen(seed)
+    return [t.to(dtype) for t in (normal(g, M, K), normal(g, N, K, std=K**-0.5), normal(g, M, N))] + [normal(g, N).float()]
+
+
+def check_linear(x, w, b, r, act, y, z=None):
+    """y and z against 64 bits; the arguments on the CPU."""
+    dt, K = x.dtype, x.shape[1]
+    terms = x.to(F64).abs() @ w.to(F64).abs().t() + (0 if b is None else b.to(F64).abs())
+    zz = x.to(F64) @ w.to(F64).t() + (0 if b is None else b.to(F64))
+    off = (K + 2 + 12) * U32 * terms
+    if z is not None:
+        close(z, zz, off + u(dt) * (zz.abs() + off) + tiny(dt), "z")
+    want = act64(zz, act)
+    off = 1.13 * off + SLACK * U32 * zz.abs()  # no activation is steeper than 1.13
+    if r is not None:
+        want = want + r.to(F64)
+        off = off + U32 * (want.abs() + off)
+    close(y, want, off + u(dt) * (want.abs() + off) + tiny(dt), "y")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", ODD)
+def test_linear(M, K, N, dtype):
+    x, w, r, b = make_layer(M, K, N, DTYPES[dtype])
+    X, W, R, B = (t.cuda() for t in (x, w, r, b))
+    for i, act in enumerate(bertops.ACTS):
+        res, bias = (i & 1) == 0, i != 3
+        y, z = bertops.linear(X, W, B if bias else None, residual=R if res else None, act=act, save_z=True)
+        check_linear(x, w, b if bias else None, r if res else None, act, y, z)
+    again = bertops.linear(X, W, B, residual=R, act=act)
+    assert torch.equal(again, bertops.linear(X, W, B, residual=R, act=act))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(1, 768, 384), (2, 1024, 1024), (16, 384, 1536), (100, 1024, 768), (1024, 384, 384), (2050, 768, 520), (1100, 1000, 1100)])
+def test_linear_wide(M, K, N, dtype):
+    """Sizes of whole layers: every tile form, ends of rows and columns inside a tile."""
+    x, w, r, b = make_layer(M, K, N, DTYPES[dtype], seed=1)
+    y, z = bertops.linear(x.cuda(), w.cuda(), b.cuda(), residual=r.cuda(), act="gelu", save_z=True)
+    check_linear(x, w, b, r, "gelu", y, z)
+    check_linear(x, w, None, None, "none", bertops.linear(x.cuda(), w.cuda()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pad", [1, 3, 8])
+def test_linear_strides(pad, dtype):
+    """Rows further apart than their width, at every alignment; nothing is read or written between them."""
+    M, K, N = 70, 96, 130
+    x, w, r, b = make_layer(M, K, N, DTYPES[dtype], seed=2)
+    out = strided(torch.zeros(M, N, dtype=DTYPES[dtype], device="cuda"), pad)
+    y = bertops.linear(strided(x.cuda(), pad), strided(w.cuda(), pad), b.cuda(), residual=strided(r.cuda(), pad), act="silu", out=out)
+    assert y.data_ptr() == out.data_ptr()
+    check_linear(x, w, b, r, "silu", y)
+    assert torch.isnan(out._base[:, N:]).all()
+    y = bertops.linear(x.cuda()[:1].expand(M, K), w.cuda(), b.cuda())  # one row for all
+    check_linear(x[:1].expand(M, K), w, b, None, "none", y)
+    got = r.cuda()
+    bertops.linear(x.cuda(), w.cuda(), b.cuda(), residual=got, out=got)  # in place on the residual
+    check_linear(x, w, b, r, "none", got)
+
+
+@gpu
+def test_linear_large_values_and_nonfinite():
+    """f32 rows of any size keep their precision; an infinity or NaN stays in its row."""
+    x, w, _, b = make_layer(40, 256, 64, torch.float32, seed=3)
+    size = torch.logspace(-30, 30, 40, dtype=F64)[:, None].float()
+    y = bertops.linear((x * size).cuda(), w.cuda())
+    check_linear(x * size, w, None, None, "none", y)
+    mixed = x.clone()
+    mixed[:, ::3] *= 1e-6
+    check_linear(mixed, w, None, None, "none", bertops.linear(mixed.cuda(), w.cuda()))
+    for bad in (float("inf"), float("nan")):
+        for rows in (40, 1):
+            xb = x[:rows].clone()
+            xb[0, 5] = bad
+            y = bertops.linear(xb.cuda(), w.cuda(), b.cuda()).cpu()
+            assert not torch.isfinite(y[0]).any()
+            assert torch.isfinite(y[1:]).all()
+
+
+@gpu
+@pytest.mark.parametrize("act", bertops.ACTS)
+def test_activations_far_out(act):
+    """One column, weight 1: every activation and slope over the whole range, tails and extremes."""
+    z = torch.cat([torch.linspace(-30, 30, 4001, dtype=F64), torch.tensor([-1e4, -88.8, -1e-8, 0.0, 1e-30, 1e-8, 89.5, 1e4, 3e18, -3e18, 1e30, -1e30], dtype=F64)]).float()
+    one = torch.ones(1, 1, device="cuda")
+    y = bertops.linear(z[:, None].cuda(), one, act=act)
+    want = act64(z.to(F64), act)
+    # the tanh form's argument u, cubic in z, is rounded to a few 2^-24 of itself and enters an exponential
+    steep = 1 + (2 * z.to(F64).abs() ** 3).clamp(max=200) if act == "gelu" else 1 + z.to(F64).abs().clamp(max=200) ** (2 if act == "gelu_erf" else 1)
+    close(y[:, 0], want, SLACK * U32 * steep * want.abs() + 2.0**-126, "y")
+    dx, dw, db = bertops.linear_backward(torch.ones(len(z), 1, device="cuda"), z[:, None].cuda(), one, z=z[:, None].cuda(), act=act)
+    at = z.to(F64).clone().requires_grad_(True)
+    (slope,) = torch.autograd.grad(act64(at, act).sum(), at)
+    slope = torch.nan_to_num(slope, nan=0.0)
+    far = z.abs() > 100  # the reference's own products of 0 and infinity
+    slope[far] = 0.0 if act == "tanh" else 1.0
+    slope[far & (z < 0)] = 1.0 if act == "none" else 0.0
+    close(dx[:, 0], slope, SLACK * U32 * (1 + z.to(F64).abs().clamp(max=30)), "slope")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N,pad", [(1, 1, 1, 0), (1, 384, 384, 0), (3, 5, 7, 0), (65, 130, 33, 3), (200, 64, 96, 8), (1000, 72, 40, 0), (1030, 384, 256, 0), (513, 520, 768, 0), (0, 48, 24, 0)])
+def test_linear_backward(M, K, N, pad, dtype):
+    dt = DTYPES[dtype]
+    x, w, dy, _ = make_layer(M, K, N, dt, seed=4)
+    z = normal(gen(5), M, N).to(dt)
+    dev = (lambda t: strided(t.cuda(), pad)) if pad else (lambda t: t.cuda())
+    for act in bertops.ACTS:
+        dx, dw, db = bertops.linear_backward(dev(dy), dev(x), dev(w), z=dev(z), act=act)
+        at = z.to(F64).clone().requires_grad_(True)
+        (dz,) = torch.autograd.grad(act64(at, act), at, dy.to(F64))
+        # the slope's own error, and in 16 bits the rounding of dz
+        off = SLACK * U32 * (1 + z.to(F64).abs()) * dy.to(F64).abs() * (act != "none")
+        offr = off + (u(dt) * dz.abs() + tiny(dt) if dt != torch.float32 else 0)
+        terms = dz.abs() + offr
+        for got, a, b, n, what in ((dx, terms, w.to(F64).abs(), N, "dx"), (dw, terms.t(), x.to(F64).abs(), M, "dw")):
+            want = dz @ w.to(F64) if what == "dx" else dz.t() @ x.to(F64)
+            o = (offr if what == "dx" else offr.t()) @ b + (n + 12) * U32 * (a @ b)
+            close(got, want, o + u(dt) * (want.abs() + o) + tiny(dt), f"{what} {act}")
+        o = off.sum(0) + (M + 1) * U32 * (dz.abs() + off).sum(0)
+        close(db, dz.sum(0), o, f"db {act}")
+        for need in ((True, False, False), (False, True, False), (False, False, True)):
+            part = bertops.linear_backward(dev(dy), dev(x), dev(w), z=dev(z), act=act, need=need)
+            for a, b, n in zip(part, (dx, dw, db), need):
+                assert (a is None) if not n else torch.equal(a, b)
+
+
+@gpu
+def test_linear_backward_by_differences():
+    """The loss sum(c y) changes along each input as its gradient says."""
+    M, K, N = 6, 11, 9
+    g = gen(6)
+    x, w, r, c = (normal(g, *s).float() for s in ((M, K), (N, K), (M, N), (M, N)))
+    b = normal(g, N).float()
+    for act in ("gelu", "gelu_erf", "silu", "tanh"):
+        y, z = bertops.linear(x.cuda(), w.cuda(), b.cuda(), residual=r.cuda(), act=act, save_z=True)
+        grads = dict(zip("xwb", bertops.linear_backward(c.cuda(), x.cuda(), w.cuda(), z=z, act=act)))
+        for name, t in (("x", x), ("w", w), ("b", b)):
+            d = normal(gen(7), *t.shape)
+            h = 1e-6
+            loss = lambda s: float((c.to(F64) * act64((x.to(F64) + (s * d if name == "x" else 0)) @ (w.to(F64) + (s * d if name == "w" else 0)).t() + b.to(F64) + (s * d if name == "b" else 0), act)).sum())  # noqa: E731, B023
+            want = (loss(h) - loss(-h)) / (2 * h)
+            got = float((grads[name].cpu().to(F64) * d).sum())
+            size = float((grads[name].cpu().to(F64) * d).abs().sum())
+            # the difference is off by h^2 times third derivatives and by 64-bit rounding over h; the gradient by f32 sums
+            assert abs(got - want) <= 1e-8 * (1 + size) * 10 + (max(M, K, N) + SLACK + 12) * U32 * size * 4, (name, act, got, want)
+
+
+# ---- token rows
+
+
+def make_table(t, V, E, seed=0):
+    g = gen(seed)
+    if t in DTYPES:
+        v = normal(g, V, E).to(DTYPES[t])
+        return v, v.to(F64)
+    nb = E // 32
+    qs = torch.randint(0, 256, (V, nb, 16), generator=g, dtype=torch.uint8)
+    head = (normal(g, V, nb, 1 if t == "q4_0" else 2) * 0.1).half()
+    raw = torch.cat([head.view(torch.uint8), qs], 2).reshape(V, -1).contiguous()
+    q = torch.cat([qs & 15, qs >> 4], 2).to(F64)
+    d = head[..., :1].to(F64)
+    return raw, ((q - 8) * d if t == "q4_0" else q * d + head[..., 1:].to(F64)).reshape(V, E)
+
+
+@gpu
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("kind,E,pad", [("f32", 1, 0), ("f32", 384, 0), ("f16", 7, 0), ("f16", 768, 8), ("bf16", 129, 3), ("bf16", 1024, 0), ("q4_0", 32, 0), ("q4_0", 384, 2), ("q4_1", 96, 0), ("q4_1", 1024, 4), ("f16", 100, 4), ("f32", 2050, 2)])
+def test_lookup(kind, E, pad, out):
+    V = 50
+    table, values = make_table(kind, V, E)
+    dev = strided(table.cuda(), pad) if pad and kind in DTYPES else table.cuda()
+    if pad and kind not in DTYPES:
+        wide = torch.full((V, table.shape[1] + pad), 255, dtype=torch.uint8, device="cuda")
+        wide[:, : table.shape[1]] = table.cuda()
+        dev = wide[:, : table.shape[1]]
+    for ids in ([0], [V - 1, -1, 3, 3, V, 2**31 - 1, -(2**31), 0], list(range(V)) * 41):
+        ids = torch.tensor(ids, dtype=torch.int32)
+        for scale in (1.0, E**0.5):
+            got = bertops.lookup(dev, ids.cuda(), scale=scale, table_type=kind, out_dtype=DTYPES[out])
+            there = (ids >= 0) & (ids < V)
+            want = torch.where(there[:, None], values[ids.clamp(0, V - 1).long()], torch.zeros((), dtype=F64)) * scale
+            off = 3 * U32 * (want.abs() + (values.abs().max() * scale if kind == "q4_1" else 0))  # the scale's rounding, the product's, q4_1's sum
+            close(got, want, off + u(DTYPES[out]) * (want.abs() + off) + tiny(DTYPES[out]), f"{kind} {out}")
+            assert (got[~there.cuda()] == 0).all()
+    assert bertops.lookup(dev, torch.zeros(0, dtype=torch.int32, device="cuda"), table_type=kind).shape[0] == 0
+    grid = torch.tensor([[1, 2, 3], [4, 5, 6]], dtype=torch.int32)
+    assert torch.equal(bertops.lookup(dev, grid.cuda(), table_type=kind).reshape(6, E), bertops.lookup(dev, grid.flatten().cuda(), table_type=kind))
+
+
+@gpu
+def test_lookup_past_32_bits():
+    """Rows that begin over 2^32 bytes into the table, and an output over 2^31 elements."""
+    V, E = 1_500_000, 1024
+    table = torch.empty(V, E, dtype=torch.float32, device="cuda")
+    at = torch.tensor([0, 1_048_575, 1_048_576, 1_048_577, V - 1], dtype=torch.int32, device="cuda")
+    for i in at.tolist():
+        table[i] = torch.arange(E, device="cuda") + i
+    assert torch.equal(bertops.lookup(table, at), table[at.long()])
+    del table
+    small = normal(gen(8), 3, E).half().cuda()
+    ids = torch.zeros((1 << 21) + 5, dtype=torch.int32, device="cuda")
+    ids[-3:] = torch.tensor([1, -1, 2])
+    out = bertops.lookup(small, ids)
+    assert torch.equal(out[-3], small[1]) and (out[-2] == 0).all() and torch.equal(out[-1], small[2]) and torch.equal(out[1 << 20], small[0])
+
+
+def check_grad(got, dout, ids, V, scale, pad, base=None):
+    there = (ids >= 0) & (ids < V) & (ids != pad)
+    at, rows = ids[there].long(), dout[there].to(F64)
+    E = dout.shape[1]
+    want = torch.zeros(V, E, dtype=F64).index_add_(0, at, rows)
+    size = torch.zeros(V, E, dtype=F64).index_add_(0, at, rows.abs())
+    count = torch.bincount(at, minlength=V).to(F64)[:, None]
+    off = (count + 2) * U32 * size * abs(scale)
+    want = want * scale
+    if base is not None:
+        want = want + base.to(F64)
+        off = off + U32 * want.abs()
+        assert torch.equal(got.cpu()[count[:, 0] == 0], base[count[:, 0] == 0])
+    close(got, want, off + 2.0**-149, "dtable")
+    if base is None:
+        assert (got.cpu()[count[:, 0] == 0] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,E,pad_ld", [(0, 5, 8, 0), (1, 1, 1, 0), (1, 30522, 384, 0), (7, 3, 33, 3), (64, 10, 384, 0), (1000, 100, 130, 8), (2048, 30522, 64, 0), (2049, 517, 96, 0), (5000, 2, 40, 0), (40000, 70000, 32, 0), (9000, 1, 300, 1), (30000, 900, 768, 0)])
+def test_lookup_grad(n, V, E, pad_ld, dtype):
+    g = gen(9)
+    dout = normal(g, n, E).to(DTYPES[dtype])
+    ids = (V * torch.rand(n, generator=g, dtype=F64) ** 4).to(torch.int32)
+    if n > 4:
+        ids[1], ids[3] = -1, V
+    dev = strided(dout.cuda(), pad_ld) if pad_ld and n else dout.cuda()
+    for scale, pad in ((1.0, -1), (-2.5, 0)):
+        out = strided(torch.zeros(V, E, device="cuda"), pad_ld) if pad_ld else torch.full((V, E), float("nan"), device="cuda")
+        got = bertops.lookup_grad(dev, ids.cuda(), V, scale=scale, pad_id=pad, out=out)
+        check_grad(got, dout, ids, V, scale, pad)
+        if pad_ld:
+            assert torch.isnan(out._base[:, E:]).all()
+        assert torch.equal(got, bertops.lookup_grad(dev, ids.cuda(), V, scale=scale, pad_id=pad))  # the same bits
+        base = normal(g, V, E).float()
+        got = bertops.lookup_grad(dev, ids.cuda(), V, scale=scale, pad_id=pad, out=base.cuda(), accumulate=True)
+        check_grad(got, dout, ids, V, scale, pad, base)
+
+
+@gpu
+def test_lookup_grad_one_token():
+    """Every place the same token, and one gradient row broadcast to all places."""
+    n, E = 70000, 48
+    dout = normal(gen(10), 1, E).half()
+    ids = torch.full((n,), 2, dtype=torch.int32)
+    got = bertops.lookup_grad(dout.cuda().expand(n, E), ids.cuda(), 4)
+    check_grad(got, dout.expand(n, E), ids, 4, 1.0, -1)
+    got = bertops.lookup_grad(dout.cuda().expand(n, E), torch.full_like(ids, -1).cuda(), 4)
+    assert (got == 0).all()
+
+
+@gpu
+def test_lookup_grad_by_differences():
+    """The loss sum(c out) is linear in the table: its change along any direction is the gradient's product with it."""
+    V, E, n = 20, 24, 60
+    g = gen(11)
+    d, c = normal(g, V, E), normal(g, n, E)
+    ids = torch.randint(-1, V, (n,), generator=g, dtype=torch.int32)
+    grad = bertops.lookup_grad(c.float().cuda(), ids.cuda(), V, scale=3.0)
+    moved = bertops.lookup(d.float().cuda(), ids.cuda(), scale=3.0).cpu().to(F64)
+    size = float((moved * c).abs().sum())
+    assert abs(float((grad.cpu().to(F64) * d.float().to(F64)).sum()) - float((moved * c.float().to(F64)).sum())) <= (n + 4) * 2 * U32 * size
+
+
+# ---- AdamW
+
+
+def mix(h):
+    h = np.asarray(h, np.uint32)
+    h = (h ^ (h >> np.uint32(16))) * np.uint32(0x9E3779B9)
+    h = (h ^ (h >> np.uint32(15))) * np.uint32(0xBB67AE85)
+    return h ^ (h >> np.uint32(16))
+
+
+def code_values(mant):
+    n = 1 << mant
+    c = np.arange(16 * n)
+    e, f = c >> mant, c & (n - 1)
+    return np.where(e == 0, f * (2.0 / n), (1 + f / n) * 2.0**e).astype(np.float32)
+
+
+def encode(a, mant, h):
+    """Codes and scales of f32 magnitudes, block by block, rounded at random by the bits h."""
+    n, codes, scales = 1 << mant, np.zeros(len(a), np.int64), []
+    drop = 23 - mant
+    top = np.float32((2 - 2.0**-mant) * 2.0**15)
+    for s in range(0, len(a), 256):
+        x, bits = a[s : s + 256], h[s : s + 256]
+        peak = x.max() if not np.isnan(x).any() else np.float32(np.nan)
+        scale = np.float32(0) if peak < 2.0**-100 else np.float32(peak / top)
+        scales.append(scale)
+        if not (scale > 0 and np.isfinite(scale)):
+            continue
+        y = x * (np.float32(1) / scale)
+        far = ((y.view(np.uint32).astype(np.int64) + (bits >> np.uint32(32 - drop))) >> drop) - 127 * n
+        near = np.floor(y * np.float32(n / 2) + (bits >> np.uint32(8)).astype(np.float32) * np.float32(2.0**-24)).astype(np.int64)
+        codes[s : s + 256] = np.minimum(np.where(y >= 2, far, near), 16 * n - 1)
+    return codes, np.asarray(scales, np.float32)
+
+
+class PlainAdamW:
+    """The step on numpy f32 arrays in the order the header gives, every operation rounded by itself."""
+
+    def __init__(self, ps, bits, lr, betas, eps, decay, seed):
+        self.ps = [p.copy() for p in ps]
+        self.m, self.v = [np.zeros_like(p) for p in ps], [np.zeros_like(p) for p in ps]
+        self.bits, self.lr, self.betas, self.eps, self.decay, self.seed, self.t = bits, lr, betas, eps, decay, seed, 0
+
+    def step(self, gs, scale=None):
+        f = np.float32
+        self.t += 1
+        (b1, b2), t = self.betas, self.t
+        k, root = f(self.lr / (1 - b1**t)), f(1 / (1 - b2**t) ** 0.5)
+        with np.errstate(over="ignore", invalid="ignore", under="ignore"):
+            for i, g in enumerate(gs):
+                g = g.astype(f) * (f(scale) if scale is not None else f(1))
+                m = self.m[i] * f(b1) + g * f(1 - b1)
+                v = self.v[i] * f(b2) + (g * f(1 - b2)) * g
+                r = np.sqrt(v)
+                self.ps[i] = self.ps[i] * f(1 - self.lr * self.decay[i]) - (m * k) / (r * root + f(self.eps))
+                if self.bits == 8:
+                    seed = np.uint32((self.seed + t) & 0xFFFFFFFF)
+                    with np.errstate(over="ignore"):
+                        h = mix(np.arange(len(g), dtype=np.uint32) ^ mix(np.uint32(i) * np.uint32(0x9E3779B9) ^ seed))
+                    c, s = encode(np.abs(m), 3, h)
+                    each = np.repeat(s, 256)[: len(g)]
+                    m = code_values(3)[c] * each * np.where(m < 0, f(-1), f(1))
+                    c, s = encode(r, 4, mix(h ^ np.uint32(0x9E3779B9)))
+                    each = np.repeat(s, 256)[: len(g)]
+                    c = np.where((r > 0) & (c == 0) & (each > 0) & np.isfinite(each), 1, c)
+                    r = code_values(4)[c] * each
+                    v = r * r
+                self.m[i], self.v[i] = m, v
+
+
+@gpu
+@pytest.mark.parametrize("grad", DTYPES)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw(bits, grad):
+    """Four steps over tensors of every odd size: the same bits as the plain step, which rounds in the same order."""
+    sizes = [1, 3, 255, 256, 257, 1000, 4096, 4097, 70001] + [5, 600] * 30  # more than one launch's table
+    g = gen(12)
+    ps = [normal(g, n, std=0.1).float() for n in sizes]
+    decay = [0.1 * (i % 3) for i in range(len(sizes))]
+    dev = [p.cuda() for p in ps]
+    copies = [torch.zeros_like(p, dtype=torch.float16) for p in dev]
+    opt = bertops.AdamW(dev, lr=3e-3, betas=(0.8, 0.99), eps=1e-7, weight_decay=decay, bits=bits, copies=copies, seed=0xFFFFFFFE)
+    plain = PlainAdamW([p.numpy() for p in ps], bits, 3e-3, (0.8, 0.99), 1e-7, decay, 0xFFFFFFFE)
+    for step in range(4):
+        gs = [(normal(g, n, std=0.01) * torch.logspace(-6, 0, n, dtype=F64)).to(DTYPES[grad]) for n in sizes]
+        for x in gs:
+            x[::7] = 0
+        scale = None if step < 2 else 0.37
+        opt.step([x.cuda() for x in gs], None if scale is None else torch.tensor([scale], device="cuda"))
+        plain.step([x.float().numpy() for x in gs], scale)
+        m, v = opt.moments()
+        for i, n in enumerate(sizes):
+            a = opt.where[i]
+            for got, want, what in ((dev[i], plain.ps[i], "p"), (m[a : a + n], plain.m[i], "m"), (v[a : a + n], plain.v[i], "v")):
+                assert np.array_equal(got.cpu().numpy(), want), (what, i, n, step)
+            assert torch.equal(copies[i], dev[i].half())
+
+
+@gpu
+def test_adamw_against_64_bits():
+    """f32 states stay within the f32 error of each operation of the same step in 64 bits."""
+    n = 5000
+    g = gen(13)
+    p = normal(g, n).float()
+    dev = p.cuda()
+    opt = bertops.AdamW([dev], lr=1e-2, weight_decay=0.1)
+    q, m, v = p.to(F64), torch.zeros(n, dtype=F64), torch.zeros(n, dtype=F64)
+    moved = torch.zeros(n, dtype=F64)
+    for t in range(1, 6):
+        gr = normal(g, n).float()
+        opt.step([gr.cuda()])
+        m, v = 0.9 * m + 0.1 * gr.to(F64), 0.999 * v + 0.001 * gr.to(F64) ** 2
+        d = 1e-2 / (1 - 0.9**t) * m / (v.sqrt() / (1 - 0.999**t) ** 0.5 + 1e-8)
+        q = q * (1 - 1e-2 * 0.1) - d
+        moved += 1e-2 / (1 - 0.9**t) * (0.1 * 5 * 4) / (v.sqrt() / (1 - 0.999**t) ** 0.5 + 1e-8)  # |m| of gradients of at most 4 sigma
+    got_m, got_v = opt.moments()
+    close(got_v[:n], v, 5 * 6 * U32 * v, "v")
+    close(got_m[:n], m, 5 * 4 * U32 * 6.0, "m")
+    close(dev, q, 5 * 4 * U32 * (q.abs() + 1) + 40 * U32 * moved, "p")
+
+
+@gpu
+def test_adamw_8_bit_states_follow_the_32_bit_ones():
+    """Rounding up or down at random has no drift: over blocks of equal values the stored moments average to the exact ones."""
+    n, steps = 256 * 64, 40
+    g = torch.logspace(-3, 0, 64, dtype=F64).repeat_interleave(256).float()  # one size a block
+    a = bertops.AdamW([torch.zeros(n, device="cuda")], bits=8, seed=1)
+    for _ in range(steps):
+        a.step([g.cuda()])
+    m, v = a.moments()
+    want_m, want_r = g.to(F64) * (1 - 0.9**steps), g.to(F64) * (1 - 0.999**steps) ** 0.5
+    got_m, got_r = (x.cpu().to(F64).reshape(64, 256).mean(1) for x in (m, v.sqrt()))
+    # each step's rounding is within one code's step (2^-3 of m, 2^-4 of r) of the value, and the scale follows the
+    # block's largest: a mean over 256 elements of a sum of such roundings, forgotten at rate 1 - beta, stays within one step
+    assert ((got_m / want_m[::256] - 1).abs() < 2.0**-3).all()
+    assert ((got_r / want_r[::256] - 1).abs() < 2.0**-2).all()
+
+
+@gpu
+def test_adamw_nonfinite_and_tiny():
+    n = 700
+    p = normal(gen(14), n).float().cuda()
+    g = torch.zeros(n)
+    g[300] = float("inf")
+    for bits in (32, 8):
+        w = p.clone()
+        opt = bertops.AdamW([w], bits=bits, weight_decay=0.0)
+        opt.step([g.cuda()])
+        m, v = opt.moments()
+        assert not torch.isfinite(w[300]) and torch.isfinite(w[:300]).all() and torch.isfinite(w[301:]).all()
+        hurt = slice(300, 301) if bits == 32 else slice(256, 512)
+        assert not torch.isfinite(m[hurt]).any() and not torch.isfinite(v[hurt]).any()
+        assert torch.isfinite(m[:256]).all() and torch.isfinite(v[512:n]).all()
+    w = p.clone()
+    opt = bertops.AdamW([w], bits=8, weight_decay=0.0)
+    opt.step([torch.full((n,), 1e-44).cuda()])  # moments under any scale: stored as zero, and the weights are sound
+    assert (opt.moments()[0] == 0).all() and torch.isfinite(w).all()
+    opt.step([torch.zeros(n, device="cuda")])
+    assert torch.isfinite(w).all()
+
+
+# ---- together: streams, graphs, other shapes of use
+
+
+def train_once(table, w, b, ids, target, opts, copies=None):
+    """Rows, a layer on their mean over each sentence, and one step of both: every operator, as they are used together."""
+    rows = bertops.lookup(table, ids, scale=2.0)
+    e = rows.mean(1)
+    y, z = bertops.linear(e, w, b, residual=e, act="tanh", save_z=True)
+    dy = (y - target) / len(y)
+    de, dw, db = bertops.linear_backward(dy, e, w, z=z, act="tanh")
+    de = de + dy
+    dt = bertops.lookup_grad((de / ids.shape[1])[:, None, :].expand(rows.shape).contiguous(), ids, table.shape[0], scale=2.0, pad_id=0)
+    return y, [dt, dw, db]
+
+
+def training_inputs(V=300, E=64, n=40, L=12):
+    g = gen(15)
+    table, w, b = normal(g, V, E, std=0.5).float().cuda(), normal(g, E, E, std=0.1).float().cuda(), torch.zeros(E, device="cuda")
+    ids = torch.randint(0, V, (n, L), generator=g, dtype=torch.int32).cuda()
+    return table, w, b, ids, normal(g, n, E).float().cuda()
+
+
+@gpu
+def test_together_against_autograd():
+    """One pass through lookup, layer and both gradients against torch's own gradients in 64 bits."""
+    table, w, b, ids, target = training_inputs()
+    y, (dt, dw, db) = train_once(table, w, b, ids, target, None)
+    T, W, B = (t.cpu().to(F64).requires_grad_(True) for t in (table, w, b))
+    rows = torch.where((ids.cpu() != 0)[..., None], T[ids.cpu().long()], T[ids.cpu().long()].detach()) * 2.0
+    e = rows.mean(1)
+    yy = torch.tanh(e @ W.t() + B) + e
+    loss = (0.5 * (yy - target.cpu().to(F64)) ** 2).sum() / len(yy)
+    loss.backward()
+    # f32 through about ten sums of at most 64 terms: every value within 2^-24 times 1000 of the largest one around it
+    for got, want in ((y, yy.detach()), (dt, T.grad), (dw, W.grad), (db, B.grad)):
+        close(got, want, 1000 * U32 * want.abs().max() * torch.ones_like(want), "gradient")
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_together_in_a_graph(bits):
+    """A whole training step captured once and replayed, with eager work and synchronisation between the replays."""
+    table, w, b, ids, target = training_inputs()
+    opts = [bertops.AdamW([t.clone() for t in (table, w, b)], bits=bits, seed=3) for _ in range(2)]
+    static = [t.clone() for t in (ids, target)]
+
+    def grads(opt):
+        y, g = train_once(*opt.params, *static, None)
+        return y, g
+
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        grads(opts[1])
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, g = grads(opts[1])
+    for k in range(4):
+        static[0].copy_((ids + k) % table.shape[0])
+        static[1].copy_(target * (k + 1))
+        graph.replay()
+        want_y, want_g = grads(opts[0])
+        torch.cuda.synchronize()
+        assert torch.equal(y, want_y) and all(torch.equal(a, c) for a, c in zip(g, want_g)), k
+        for o, gr in ((opts[0], want_g), (opts[1], g)):
+            o.step(gr)
+        assert all(torch.equal(a, c) for a, c in zip(opts[0].params, opts[1].params))
+
+
+@gpu
+def test_two_streams_at_once():
+    """The same calls on two streams at a time give what each gives alone."""
+    x, w, r, b = (t.cuda() for t in make_layer(700, 384, 384, torch.bfloat16, seed=16))
+    g = gen(17)
+    ids = [torch.randint(0, 5000, (20000,), generator=g, dtype=torch.int32).cuda() for _ in range(2)]
+    dout = [normal(g, 20000, 96).half().cuda() for _ in range(2)]
+    alone = [(bertops.lookup_grad(d, i, 5000), bertops.linear_backward(r, x, w, z=r, act="gelu")) for d, i in zip(dout, ids)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for s, d, i in zip(streams, dout, ids):
+            with torch.cuda.stream(s):
+                got.append((bertops.lookup_grad(d, i, 5000), bertops.linear_backward(r, x, w, z=r, act="gelu")))
+        torch.cuda.synchronize()
+        for (a, b1), (c, d1) in zip(got, alone):
+            assert torch.equal(a, c) and all(torch.equal(p, q) for p, q in zip(b1, d1))
+
+
+@gpu
+def test_adapter_and_token_table(model_dir):
+    """An adapter on a model's embeddings and its word rows made trainable: the framework's own users of the operators."""
+    import os
+
+    path = os.path.join(model_dir, "ops_minilm_q4_0.gguf")
+    if not os.path.exists(path):
+        bertlib.synth_model(path, "minilm", "q4_0", n_layer=1)
+    for options, kind in ((None, "q4_0"), ({"emb_raw": 0}, "f32")):
+        model = bertlib.BertModel(path, devices=[0], options=options)
+        rows = bertops.word_rows(model)
+        assert rows.shape == (30522, 384) and model.word_table()[1] == bertops.TABLE_TYPES[kind]
+        from gguf_reader import GGUF
+
+        want = torch.from_numpy(GGUF(path).f32("embeddings.word_embeddings.weight").reshape(30522, 384).copy())
+        assert torch.equal(rows.cpu(), want)
+        ids = torch.tensor([[101, 7, 102], [-1, 30522, 30521]], dtype=torch.int32)
+        some = bertops.word_rows(model, ids.cuda(), scale=2.0).cpu()
+        assert torch.equal(some[0], want[ids[0].long()] * 2) and (some[1, :2] == 0).all()
+        sentences = ["hello world", "a second sentence", "x"]
+        e = model.encode(sentences)
+        adapter = bertops.Adapter(384, lr=1e-2)
+        assert np.allclose(adapter.encode(model, sentences), e, atol=4 * 2.0**-23)  # zero weights: the embeddings themselves
+        E = torch.from_numpy(e).cuda()
+        y = adapter.forward(E)
+        assert torch.equal(y, E)
+        de = adapter.backward(y - 1.0, need_input=True)
+        assert torch.equal(de, y - 1.0)  # through zero weights only the residual passes
+        before = adapter.b.clone()
+        adapter.step()
+        assert (adapter.b > before).all()  # each bias's gradient is a sum of negative values
+        table = bertops.TokenTable(model, lr=1e-2)
+        out = table.forward(torch.tensor([5, 5, 9], dtype=torch.int32, device="cuda"))
+        table.backward(torch.ones_like(out))
+        table.backward(torch.ones_like(out))
+        table.step()
+        moved = (table.rows.cpu() != want * (1 - 1e-2 * 0.01)).any(1).nonzero()[:, 0].tolist()
+        assert 5 in moved and 9 in moved and (table.rows.cpu()[5] < want[5]).all()
+        model.close()
+
+
+# ---- refusals: no GPU is needed, none is launched
+
+
+def test_refusals_of_the_library():
+    """Every bad argument of the C entry points is refused with a message before any device call."""
+    L = bertlib.lib()
+    P, NULL = 1 << 20, None  # an aligned address that nothing dereferences
+    big = 1 << 40
+
+    def refused(rc, word):
+        assert rc == -1 and word in bertlib.last_error(), (rc, bertlib.last_error())
+
+    ok = dict(device=0, type=0, act=0, M=4, N=8, K=8, x=P, ldx=8, w=P, ldw=8, bias=P, r=P, ldr=8, y=P + 4096, ldy=8, z=NULL, ldz=8, ws=P, nws=big, s=NULL)
+    for change, word in ((dict(type=2), "type"), (dict(type=7), "type"), (dict(act=6), "activation"), (dict(act=-1), "activation"), (dict(M=-1), "size"), (dict(M=1 << 31), "size"), (dict(N=0), "size"), (dict(K=0), "size"), (dict(N=1 << 22), "size"), (dict(M=1 << 30, N=1 << 10), "size"), (dict(x=NULL), "x"), (dict(x=P + 2), "x"), (dict(ldx=7), "x"), (dict(ldx=-8), "x"), (dict(w=NULL), "w"), (dict(y=NULL), "y"), (dict(ldy=0), "y"), (dict(ldy=7), "y"), (dict(r=P + 1), "residual"), (dict(z=P, ldz=0), "z"), (dict(bias=P + 1), "bias"), (dict(r=P + 4096, ldr=9), "residual")):
+        refused(L.bert_amd_linear(*{**ok, **change}.values()), word)
+    need = L.bert_amd_linear_workspace(0, 4, 8, 100000)
+    assert need >= 0 and L.bert_amd_linear_workspace(5, 4, 8, 8) == -1
+    if need:
+        for change in (dict(ws=NULL), dict(nws=need - 1), dict(ws=P + 8)):
+            refused(L.bert_amd_linear(*{**ok, "K": 100000, "ldx": 100000, "ldw": 100000, **change}.values()), "workspace")
+    assert L.bert_amd_linear(*{**ok, "M": 0, "x": NULL}.values()) == 0
+
+    ok = dict(device=0, type=1, act=2, M=4, N=8, K=8, dy=P, lddy=8, z=P, ldz=8, x=P, ldx=8, w=P, ldw=8, dx=P, lddx=8, dw=P, lddw=8, db=P, ws=P, nws=big, s=NULL)
+    for change, word in ((dict(type=3), "type"), (dict(act=9), "activation"), (dict(M=-1), "size"), (dict(dy=NULL), "dy"), (dict(dy=P + 1), "dy"), (dict(z=NULL), "z"), (dict(ldz=4), "z"), (dict(x=NULL), "x"), (dict(w=NULL), "w"), (dict(lddx=0), "dx"), (dict(lddw=7), "dw"), (dict(db=P + 2), "dbias"), (dict(ws=NULL), "workspace"), (dict(nws=1), "workspace")):
+        refused(L.bert_amd_linear_backward(*{**ok, **change}.values()), word)
+    assert L.bert_amd_linear_backward(*{**ok, "dx": NULL, "dw": NULL, "db": NULL}.values()) == 0
+    assert L.bert_amd_linear_backward_workspace(1, 2, -1, 8, 8) == -1
+
+    ok = dict(device=0, type=2, out=0, n=4, V=10, E=64, table=P, ld=36, ids=P, scale=1.0, o=P, ldo=64, s=NULL)
+    for change, word in ((dict(type=8), "types"), (dict(out=2), "types"), (dict(n=-1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(E=40), "size"), (dict(table=NULL), "table"), (dict(table=P + 1), "table"), (dict(ld=35), "table"), (dict(ld=37), "table"), (dict(ids=NULL), "ids"), (dict(ids=P + 2), "ids"), (dict(o=NULL), "out"), (dict(ldo=63), "out"), (dict(ldo=0), "out")):
+        refused(L.bert_amd_lookup(*{**ok, **change}.values()), word)
+    assert L.bert_amd_lookup(*{**ok, "n": 0, "ids": NULL}.values()) == 0
+
+    ok = dict(device=0, type=0, n=4, V=10, E=8, dout=P, ldd=8, ids=P, scale=1.0, pad=-1, acc=0, dt=P, ldt=8, ws=P, nws=big, s=NULL)
+    for change, word in ((dict(type=2), "type"), (dict(n=-1), "size"), (dict(n=(1 << 30) + 1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(dout=NULL), "dout"), (dict(ldd=7), "dout"), (dict(ids=NULL), "ids"), (dict(dt=NULL), "dtable"), (dict(ldt=7), "dtable"), (dict(ws=NULL), "workspace"), (dict(nws=16), "workspace")):
+        refused(L.bert_amd_lookup_grad(*{**ok, **change}.values()), word)
+    assert L.bert_amd_lookup_grad_workspace(-1, 10, 8) == -1
+
+    row = np.zeros(2, bertops.AdamW._ROW)
+    for k in ("p", "g", "m", "v", "ms", "vs"):
+        row[k] = [P, P + (1 << 16)]
+    row["n"] = 100
+
+    def adamw(rows=row, n=2, bits=32, grad=0, copy=30, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, step=1, scale=NULL):
+        return L.bert_amd_adamw(0, n, rows.ctypes.data if rows is not None else NULL, bits, grad, copy, lr, b1, b2, eps, step, 0, scale, NULL)
+
+    nan = float("nan")
+    for change, word in ((dict(rows=None), "tensors"), (dict(n=-1), "tensors"), (dict(bits=16), "bits"), (dict(grad=2), "type"), (dict(lr=-1.0), "lr"), (dict(lr=nan), "lr"), (dict(b1=1.0), "beta"), (dict(b2=-0.1), "beta"), (dict(b2=nan), "beta"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"), (dict(step=0), "step"), (dict(scale=P + 1), "grad_scale")):
+        refused(adamw(**change), word)
+
+    def with_(**kw):
+        r = row.copy()
+        for k, v in kw.items():
+            r[k][1] = v
+        return r
+
+    for kw, word in ((dict(n=-1), "size"), (dict(n=(1 << 34) + 1), "size"), (dict(decay=nan), "decay"), (dict(decay=-1.0), "decay"), (dict(p=0), "pointer"), (dict(g=0), "pointer"), (dict(m=P + 2), "pointer"), (dict(copy=P + 1), "copy"), (dict(p=P + 396), "share")):
+        refused(adamw(with_(**kw)), word)
+    refused(adamw(with_(copy=P), copy=0), "copies")
+    refused(adamw(with_(ms=0), bits=8), "pointer")
+    assert adamw(n=0) == 0
+    refused(L.bert_amd_adamw_moments(0, -1, P, P, P, P, P, P, NULL), "size")
+    refused(L.bert_amd_adamw_moments(0, 4, NULL, P, P, P, P, P, NULL), "pointer")
+    out = [ctypes.c_void_p()] + [ctypes.c_int32() for _ in range(4)]
+    refused(L.bert_amd_word_table(None, 0, *(ctypes.byref(t) for t in out)), "invalid")
+
+
+def test_workspace_sizes():
+    """Bytes for every size, zero rows among them."""
+    L = bertlib.lib()
+    for t in (0, 1, 30):
+        for N, K in ((1, 1), (384, 384), (31, 4097), ((1 << 22) - 1, 4)):
+            for M in (0, 1, 63, 64, 1000, 4096):
+                assert L.bert_amd_linear_workspace(t, M, N, K) >= 0
+                for act in (0, 2):
+                    assert L.bert_amd_linear_backward_workspace(t, act, M, N, K) >= (M * N * (4 if t == 0 else 2) if act else 0)
+    for n in (0, 1, 2048, 2049, 1 << 30):
+        for V in (1, 511, 512, 1 << 30):
+            assert L.bert_amd_lookup_grad_workspace(n, V, 8) >= 0
+
+
+def test_refusals_on_tensors():
+    """bertops refuses tensors of the wrong kind before it calls the library."""
+    x = torch.zeros(4, 8)
+    for call in (lambda: bertops.linear(x, x), lambda: bertops.linear_backward(x, x, x), lambda: bertops.lookup(x, torch.zeros(3, dtype=torch.int32)),
+                 lambda: bertops.lookup_grad(x, torch.zeros(4, dtype=torch.int32), 5), lambda: bertops.AdamW([x]), lambda: bertops.AdamW([]),
+                 lambda: bertops._act("swish"), lambda: bertops._matrix("m", x.t(), torch.float32, x.device, 8, 4),
+                 lambda: bertops._matrix("m", x, torch.float16, x.device, 4, 8), lambda: bertops._matrix("m", x, torch.float32, x.device, 4, 7),
+                 lambda: bertops._ids(torch.zeros(3, dtype=torch.int64), x.device), lambda: bertops._ids(torch.zeros(6, dtype=torch.int32)[::2], x.device)):
+        with pytest.raises(ValueError):
+            call()
+
+
+@gpu
+def test_refusals_on_the_gpu():
+    x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
+    z = torch.zeros(4, 6, device="cuda")
+    for call in (lambda: bertops.linear(x, w[:, :7]), lambda: bertops.linear(x, w.half()), lambda: bertops.linear(x.int(), w), lambda: bertops.linear(x, w, torch.zeros(6)),
+                 lambda: bertops.linear(x, w, torch.zeros(6, device="cuda").half()), lambda: bertops.linear(x, w, residual=x), lambda: bertops.linear(x, w, out=torch.zeros(1, 6, device="cuda").expand(4, 6)),
+                 lambda: bertops.linear(x, w, act="swish"), lambda: bertops.linear(x.t(), w[:, :4]), lambda: bertops.linear_backward(z, x, w, act="gelu"),
+                 lambda: bertops.lookup(w, torch.zeros(2, dtype=torch.int64, device="cuda")), lambda: bertops.lookup(w, torch.zeros(2, dtype=torch.int32)),
+                 lambda: bertops.lookup(w, torch.zeros(2, dtype=torch.int32, device="cuda"), table_type="q4_0"), lambda: bertops.lookup(w, torch.zeros(2, dtype=torch.int32, device="cuda"), table_type="f16"),
+                 lambda: bertops.lookup_grad(x, torch.zeros(3, dtype=torch.int32, device="cuda"), 5), lambda: bertops.lookup_grad(x, torch.zeros(4, dtype=torch.int32, device="cuda"), 5, accumulate=True),
+                 lambda: bertops.lookup_grad(x, torch.zeros(4, dtype=torch.int32, device="cuda"), 0), lambda: bertops.AdamW([x.half()]), lambda: bertops.AdamW([x.t()]), lambda: bertops.AdamW([x], bits=16),
+                 lambda: bertops.AdamW([x], copies=[x]), lambda: bertops.AdamW([x], weight_decay=[0.1, 0.1]), lambda: bertops.AdamW([x, x[1:]]).step([x, x[1:]]), lambda: bertops.AdamW([x]).step([w]),
+                 lambda: bertops.AdamW([x]).step([x], torch.ones(2, device="cuda")), lambda: bertops.Adapter(4).step(), lambda: bertops.Adapter(4).backward(x)):
+        with pytest.raises(ValueError):
+            call()
