@@ -8,6 +8,7 @@
 #include "ops_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace bertamd {
 
@@ -130,6 +131,274 @@ __global__ __launch_bounds__(256) void tile_gemm_kernel(Operand A, Operand B, in
     }
 }
 
+// ---- the tile kernel for 16-bit operands in whole chunks ---------------------
+//
+// The same products from operands whose rows are 16-byte aligned and whose
+// contiguous axis is a multiple of 8 long.  BM x BN tiles, k in stages of 64,
+// two stages of both operands in LDS: while a stage is multiplied the next one
+// is on its way from memory straight into LDS (16 bytes a lane, no registers).
+// One barrier a stage: behind it all of this stage has landed (each wave has
+// waited for its own loads) and all waves are done with the other buffer.
+//
+// Loads go through a buffer descriptor at the stage's start; a lane whose chunk
+// lies outside its matrix gives an offset past the descriptor's range, for
+// which the hardware writes zeros, so k and both tile edges need no branch.
+//
+// An operand stored along k has 64 k of a row in 128 bytes of LDS, 8 chunks
+// permuted by the row so that the rows of an operand read lie in different
+// banks.  An operand stored along m (the gradients' W, dz and x) stays so in
+// LDS, and ds_read_b64_tr_b16 transposes 4 k x 16 m as it is read: no
+// transposed copy is made in memory.
+//
+// The second matrix is the matrix instruction's row operand, so that a lane
+// holds 4 consecutive columns of one row of C at a time.  The finished sums go
+// through LDS, 64 rows of each wave's tile at a time, for whole 128-byte row
+// pieces on the way out and one copy of the epilogue's code.
+constexpr int SK = 64;                          // k of a stage
+constexpr uint32_t OUTSIDE = 0x80000000u;       // an offset past every descriptor's range (2^31 bytes)
+
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+// 16 bytes a lane from `base` + off to LDS bytes lds .. lds + 1023
+__device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ u32x4 descriptor(const char *base) {
+    const uint64_t b = (uint64_t)base;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(b >> 32) & 0xffffu)), OUTSIDE, 0x00020000u};
+}
+
+// one operand's tile of R rows (of the product; its contiguous axis if TRANS)
+template <bool TRANS, int R, int NT>
+struct Tile {
+    static constexpr int LOADS = R * SK * 2 / 16 / NT;  // 16-byte chunks a thread loads per stage
+    static constexpr int BYTES = R * SK * 2;
+    const char *base;     // of the stage to load next
+    int64_t step;         // bytes from a stage to the next
+    uint32_t off[LOADS];  // from base
+    int at[LOADS];        // the chunk's k within the stage
+
+    // the place of k chunk c (of 8) in row r's 128 bytes
+    static __device__ __forceinline__ int spread(int r, int c) { return c ^ (r & 7); }
+    // the place of column chunk c in k row k
+    static __device__ __forceinline__ int spread_t(int k, int c) { return c ^ ((4 * (k & 3)) & (R / 8 - 1)); }
+
+    __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t rows, int64_t k0) {
+        const int t = threadIdx.x;
+        if constexpr (!TRANS) {
+            base = (const char *)o.p + (row0 * o.ld + k0) * 2;
+            step = SK * 2;
+        } else {
+            base = (const char *)o.p + (k0 * o.ld + row0) * 2;
+            step = SK * o.ld * 2;
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int q = i * NT + t;
+            if constexpr (!TRANS) {
+                const int r = q >> 3, c = spread(r, q & 7);
+                at[i] = 8 * c;
+                off[i] = row0 + r < rows ? (uint32_t)(r * o.ld * 2) + 16 * c : OUTSIDE;
+            } else {
+                const int k = q / (R / 8), c = spread_t(k, q % (R / 8));
+                at[i] = k;
+                off[i] = row0 + 8 * c < rows ? (uint32_t)(k * o.ld * 2) + 16 * c : OUTSIDE;
+            }
+        }
+    }
+    __device__ __forceinline__ void load(uint32_t lds, int64_t k_left) {
+        const u32x4 d = descriptor(base);
+        const uint32_t w = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x >> 6) * 1024);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) load_to_lds(d, at[i] < k_left ? off[i] : OUTSIDE, w + i * NT * 16);
+        base += step;
+    }
+    // operand registers of rows r0 .. r0 + 31, k 16 ks .. 16 ks + 15 of the stage at `lds`
+    static __device__ __forceinline__ u32x4 read(const char *lds, int r0, int ks) {
+        const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
+        if constexpr (!TRANS) {
+            return *(const u32x4 *)(lds + (r0 + c) * 128 + spread(c, 2 * ks + h) * 16);
+        } else {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
+            // lane i of each 16 gives the address of k row i / 4's columns 4 (i % 4) .. + 3 and gets column i of the 4 rows
+            const int col = r0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const int k = 16 * ks + 8 * h + ((lane & 15) >> 2);
+            const char *p0 = lds + k * (R * 2) + spread_t(k, col >> 3) * 16 + (col & 7) * 2;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p0);
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p0 + 4 * R * 2));
+            struct { s16x4 a, b; } both = {a, b};
+            return __builtin_bit_cast(u32x4, both);
+        }
+    }
+};
+
+template <int TYPE>
+__device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (TYPE == BERT_AMD_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ void act8(float *v, int act) {
+    constexpr bool WIDE = sizeof(T) == 4;
+    const auto each = [&](auto a) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_t<decltype(a)::value, WIDE>(v[i]);
+    };
+    switch (act) {
+        case BERT_AMD_ACT_RELU: each(std::integral_constant<int, BERT_AMD_ACT_RELU>()); break;
+        case BERT_AMD_ACT_GELU: each(std::integral_constant<int, BERT_AMD_ACT_GELU>()); break;
+        case BERT_AMD_ACT_GELU_ERF: each(std::integral_constant<int, BERT_AMD_ACT_GELU_ERF>()); break;
+        case BERT_AMD_ACT_SILU: each(std::integral_constant<int, BERT_AMD_ACT_SILU>()); break;
+        case BERT_AMD_ACT_TANH: each(std::integral_constant<int, BERT_AMD_ACT_TANH>()); break;
+    }
+}
+
+// 8 elements in the type to or from an aligned row piece
+template <typename T>
+__device__ __forceinline__ void put8(T *p, const float *v) {
+    constexpr int CH = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += CH) {
+        Chunk<T, CH> o;
+#pragma unroll
+        for (int j = 0; j < CH; j++) o.v[j] = (T)v[i + j];
+        *(u32x4 *)(p + i) = __builtin_bit_cast(u32x4, o);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void add8(const T *p, float *v) {
+    constexpr int CH = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += CH) {
+        const auto o = __builtin_bit_cast(Chunk<T, CH>, *(const u32x4 *)(p + i));
+#pragma unroll
+        for (int j = 0; j < CH; j++) v[i + j] += (float)o.v[j];
+    }
+}
+
+// 8 consecutive columns of row m: bias, z, activation, residual, y
+template <typename T>
+__device__ __forceinline__ void store8(const Epilogue &e, int64_t m, int64_t n, int64_t N, bool vec, float *v) {
+    const bool whole = vec && n + 8 <= N;
+    if (e.bias) {
+        if (whole) add8(e.bias + n, v);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] += n + i < N ? e.bias[n + i] : 0.f;
+    }
+    if (e.z) {
+        T *z = (T *)e.z + m * e.ldz + n;
+        if (whole) put8(z, v);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (n + i < N) z[i] = (T)v[i];
+    }
+    act8<T>(v, e.act);
+    const T *r = (const T *)e.r + m * e.ldr + n;
+    T *y = (T *)e.y + m * e.ldy + n;
+    if (whole) {
+        if (e.r) add8(r, v);
+        put8(y, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (n + i < N) y[i] = (T)(v[i] + (e.r ? (float)r[i] : 0.f));
+    }
+}
+
+// LDS row of the epilogue: a wave's 64 columns and 16 bytes more, so that the rows of a write start in different banks
+constexpr int OUT_LD = 68;
+
+template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Operand A, Operand B, int64_t M, int64_t N, int64_t K,
+                                                                  int64_t k_per_split, float *part, Epilogue e, bool vec) {
+    typedef typename Elem<TYPE>::T T;
+    constexpr int NT = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
+    static_assert(BN / WN == 64 && BM / WM % 64 == 0, "the epilogue takes 64 x 64 of a wave's tile at a time");
+    typedef Tile<TA, BM, NT> TileA;
+    typedef Tile<TBT, BN, NT> TileB;
+    constexpr int STAGE = TileA::BYTES + TileB::BYTES;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    // workgroups of one XCD take neighbouring tiles, 8 tile rows at a time: they share operand rows in its L2
+    const int tm = (int)ceil_div<int64_t>(M, BM), tn = (int)ceil_div<int64_t>(N, BN), all = tm * tn;
+    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const int tile = xcd * (all >> 3) + min(xcd, all & 7) + slot;
+    const int group = tile / (8 * tn), in_group = tile - group * 8 * tn, high = min(8, tm - 8 * group);
+    const int64_t m0 = (int64_t)(8 * group + in_group % high) * BM, n0 = (int64_t)(in_group / high) * BN;
+    const int64_t ka = (int64_t)blockIdx.z * k_per_split, kb = min(K, ka + k_per_split);
+    TileA ta;
+    TileB tb;
+    ta.init(A, m0, M, ka);
+    tb.init(B, n0, N, ka);
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+    const int wave = threadIdx.x >> 6, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    f32x16 acc[TM][TN] = {};
+    ta.load(lds, kb - ka);
+    tb.load(lds + TileA::BYTES, kb - ka);
+    int buf = 0;
+    for (int64_t k0 = ka; k0 < kb; k0 += SK) {
+        wait_loads();
+        barrier();
+        const int64_t left = kb - k0 - SK;
+        if (left > 0) {
+            ta.load(lds + (buf ^ 1) * STAGE, left);
+            tb.load(lds + (buf ^ 1) * STAGE + TileA::BYTES, left);
+        }
+        const char *sa = smem + buf * STAGE, *sb = sa + TileA::BYTES;
+#pragma unroll
+        for (int ks = 0; ks < SK / 16; ks++) {
+            u32x4 a[TM], b[TN];
+#pragma unroll
+            for (int i = 0; i < TN; i++) b[i] = TileB::read(sb, wn + 32 * i, ks);
+#pragma unroll
+            for (int i = 0; i < TM; i++) a[i] = TileA::read(sa, wm + 32 * i, ks);
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++) acc[i][j] = mfma16<TYPE>(b[j], a[i], acc[i][j]);
+        }
+        buf ^= 1;
+    }
+    barrier();  // the stages' last reads are done: the LDS is the epilogue's
+    const int lane = threadIdx.x & 63;
+    float *out = (float *)smem + wave * 64 * OUT_LD;
+#pragma unroll 1
+    for (int part64 = 0; part64 < TM / 2; part64++) {
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+            if (i / 2 == part64)
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+#pragma unroll
+                    for (int a = 0; a < 4; a++)
+                        *(f32x4 *)(out + (32 * (i & 1) + (lane & 31)) * OUT_LD + 32 * j + 8 * a + 4 * (lane >> 5)) =
+                            f32x4{acc[i][j][4 * a], acc[i][j][4 * a + 1], acc[i][j][4 * a + 2], acc[i][j][4 * a + 3]};
+#pragma unroll 2
+        for (int row = lane >> 3; row < 64; row += 8) {
+            const int64_t m = m0 + wm + 64 * part64 + row, n = n0 + wn + 8 * (lane & 7);
+            if (m >= M || n >= N) continue;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = out[row * OUT_LD + 8 * (lane & 7) + i];
+            if (part) {
+                float *q = part + ((int64_t)blockIdx.z * M + m) * N + n;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (n + i < N) q[i] = v[i];
+            } else {
+                store8<T>(e, m, n, N, vec, v);
+            }
+        }
+    }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void split_join_kernel(const float *part, int splits, int64_t M, int64_t N, Epilogue e) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * N; i += (int64_t)gridDim.x * 256) {
@@ -167,28 +436,68 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const float *part, int6
     out[n] = v;
 }
 
-// k is split where the tiles alone leave most of the 256 CUs idle
-int splits_for(int64_t M, int64_t N, int64_t K) {
-    const int64_t tiles = ceil_div<int64_t>(M, TB) * ceil_div<int64_t>(N, TB);
-    if (tiles >= 256 || tiles == 0) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, K / 256));
-}
-int64_t split_bytes(int64_t M, int64_t N, int64_t K) {
-    const int s = splits_for(M, N, K);
-    return s > 1 ? s * M * N * 4 : 0;
-}
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
+// How a product runs: its tile kernel and in how many parts k is split, where
+// the tiles alone leave most of the 256 CUs idle.  `fits`: both operands suit
+// the stage kernel.
+struct Plan {
+    int bm, bn;  // 64 x 64: tile_gemm_kernel
+    int splits;
+    int64_t per;  // k of a split
+};
+Plan plan_for(bool fits, int64_t M, int64_t N, int64_t K) {
+    Plan p = {TB, TB, 1, 0};
+    if (fits) {
+        p.bm = p.bn = 256;
+        if (ceil_div<int64_t>(M, 256) * ceil_div<int64_t>(N, 256) < 192) p.bm = p.bn = 128;
+    }
+    const int64_t tiles = ceil_div<int64_t>(M, p.bm) * ceil_div<int64_t>(N, p.bn);
+    if (tiles > 0 && tiles < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, K / 256));
+    p.per = ceil_div(ceil_div<int64_t>(K, p.splits), (int64_t)SK) * SK;
+    return p;
+}
+int64_t split_bytes(bool fits, int64_t M, int64_t N, int64_t K) {
+    const Plan p = plan_for(fits, M, N, K);
+    return p.splits > 1 ? round256(p.splits * M * N * 4) : 0;
+}
+
+// whether the stage kernel takes an operand: whole aligned chunks, and offsets within a tile under 2^31
+template <int TYPE>
+bool stage_operand(const Operand &o, bool trans, int64_t rows, int64_t k) {
+    return TYPE != BERT_AMD_F32 && o.vec && (trans ? rows : k) % 8 == 0 && o.ld < (1 << 22);
+}
+
+template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
+void launch_stage(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, const Plan &p, float *part, const Epilogue &e,
+                  bool vec, hipStream_t s) {
+    constexpr int lds = std::max(2 * (BM + BN) * SK * 2, WM * WN * 64 * OUT_LD * 4);
+    const auto k = stage_gemm_kernel<TYPE, TA, TBT, BM, BN, WM, WN>;
+    (void)hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    const int64_t tiles = ceil_div<int64_t>(M, BM) * ceil_div<int64_t>(N, BN);
+    hipLaunchKernelGGL(k, dim3(tiles, 1, p.splits), dim3(WM * WN * 64), lds, s, A, B, M, N, K, p.per, part, e, vec);
+}
+
 template <int TYPE, bool TA, bool TBT>
-hipError_t tile_gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, void *ws, const Epilogue &e, hipStream_t s) {
+hipError_t gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, void *ws, const Epilogue &e, hipStream_t s) {
     typedef typename Elem<TYPE>::T T;
-    const int splits = splits_for(M, N, K);
-    const int64_t per = ceil_div(ceil_div<int64_t>(K, splits), (int64_t)tile_k<TYPE>()) * tile_k<TYPE>();
-    const int64_t tiles = ceil_div<int64_t>(M, TB) * ceil_div<int64_t>(N, TB);
-    float *part = splits > 1 ? (float *)ws : nullptr;
-    hipLaunchKernelGGL((tile_gemm_kernel<TYPE, TA, TBT>), dim3(tiles, 1, splits), dim3(256), 0, s, A, B, M, N, K, per, part, e);
+    const bool fits = stage_operand<TYPE>(A, TA, M, K) && stage_operand<TYPE>(B, TBT, N, K);
+    const Plan p = plan_for(fits, M, N, K);
+    float *part = p.splits > 1 ? (float *)ws : nullptr;
+    if constexpr (TYPE != BERT_AMD_F32) {
+        const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(T)); };
+        const bool vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr) && ok(e.bias, 4);
+        if (p.bm == 256)
+            launch_stage<TYPE, TA, TBT, 256, 256, 2, 4>(A, B, M, N, K, p, part, e, vec, s);
+        else if (p.bm == 128)
+            launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
+    }
+    if (p.bm == TB) {
+        const int64_t tiles = ceil_div<int64_t>(M, TB) * ceil_div<int64_t>(N, TB);
+        hipLaunchKernelGGL((tile_gemm_kernel<TYPE, TA, TBT>), dim3(tiles, 1, p.splits), dim3(256), 0, s, A, B, M, N, K, p.per, part, e);
+    }
     if (part)
-        hipLaunchKernelGGL((split_join_kernel<T>), dim3(std::min<int64_t>(1024, ceil_div<int64_t>(M * N, 256))), dim3(256), 0, s, part, splits, M, N, e);
+        hipLaunchKernelGGL((split_join_kernel<T>), dim3(std::min<int64_t>(1024, ceil_div<int64_t>(M * N, 256))), dim3(256), 0, s, part, p.splits, M, N, e);
     return hipGetLastError();
 }
 
@@ -196,7 +505,7 @@ Operand operand(const void *p, int64_t ld, int type) { return {p, ld, aligned16(
 
 template <int TYPE>
 hipError_t linear_t(const LinearArgs &a, hipStream_t s) {
-    return tile_gemm<TYPE, false, false>(operand(a.x, a.ldx, TYPE), operand(a.w, a.ldw, TYPE), a.M, a.N, a.K, a.ws,
+    return gemm<TYPE, false, false>(operand(a.x, a.ldx, TYPE), operand(a.w, a.ldw, TYPE), a.M, a.N, a.K, a.ws,
                                          {a.act, a.bias, a.r, a.y, a.z, a.ldr, a.ldy, a.ldz}, s);
 }
 
@@ -227,20 +536,20 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         Epilogue e;
         e.y = a.dx;
         e.ldy = a.lddx;
-        if (hipError_t r = tile_gemm<TYPE, false, true>(dz, operand(a.w, a.ldw, TYPE), a.M, a.K, a.N, ws, e, s); r != hipSuccess) return r;
+        if (hipError_t r = gemm<TYPE, false, true>(dz, operand(a.w, a.ldw, TYPE), a.M, a.K, a.N, ws, e, s); r != hipSuccess) return r;
     }
     if (a.dw) {
         Epilogue e;
         e.y = a.dw;
         e.ldy = a.lddw;
-        if (hipError_t r = tile_gemm<TYPE, true, true>(dz, operand(a.x, a.ldx, TYPE), a.N, a.K, a.M, ws, e, s); r != hipSuccess) return r;
+        if (hipError_t r = gemm<TYPE, true, true>(dz, operand(a.x, a.ldx, TYPE), a.N, a.K, a.M, ws, e, s); r != hipSuccess) return r;
     }
     return hipSuccess;
 }
 
 }  // namespace
 
-int64_t linear_ws_bytes(int, int64_t M, int N, int K) { return split_bytes(M, N, K); }
+int64_t linear_ws_bytes(int, int64_t M, int N, int K) { return std::max(split_bytes(false, M, N, K), split_bytes(true, M, N, K)); }
 
 hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
     switch (a.type) {
@@ -252,7 +561,8 @@ hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
 
 int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K) {
     return (act ? round256(M * N * elem_size(type)) : 0) + round256(ceil_div<int64_t>(M, DB_ROWS) * N * 4) +
-           std::max(split_bytes(M, K, N), split_bytes(N, K, M));
+           std::max(std::max(split_bytes(false, M, K, N), split_bytes(true, M, K, N)),
+                    std::max(split_bytes(false, N, K, M), split_bytes(true, N, K, M)));
 }
 
 hipError_t launch_linear_grad(const LinearGradArgs &a, hipStream_t s) {
