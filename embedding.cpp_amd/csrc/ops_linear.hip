@@ -14,6 +14,21 @@ namespace bertamd {
 
 namespace {
 
+// v *= act'(z), 8 at a time: one choice of the activation
+__device__ __forceinline__ void slope8(float *v, const float *z, int act) {
+    const auto each = [&](auto a) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= act_slope_f(z[i], decltype(a)::value);
+    };
+    switch (act) {
+        case BERT_AMD_ACT_RELU: each(std::integral_constant<int, BERT_AMD_ACT_RELU>()); break;
+        case BERT_AMD_ACT_GELU: each(std::integral_constant<int, BERT_AMD_ACT_GELU>()); break;
+        case BERT_AMD_ACT_GELU_ERF: each(std::integral_constant<int, BERT_AMD_ACT_GELU_ERF>()); break;
+        case BERT_AMD_ACT_SILU: each(std::integral_constant<int, BERT_AMD_ACT_SILU>()); break;
+        case BERT_AMD_ACT_TANH: each(std::integral_constant<int, BERT_AMD_ACT_TANH>()); break;
+    }
+}
+
 // ---- the tile kernel for any size, stride and alignment --------------------
 //
 // C[m][n] = sum over k of A(m, k) B(n, k) in 64 x 64 tiles, four waves of
@@ -134,17 +149,19 @@ __global__ __launch_bounds__(256) void tile_gemm_kernel(Operand A, Operand B, in
 // ---- the tile kernel for 16-bit operands in whole chunks ---------------------
 //
 // The same products from operands whose rows are 16-byte aligned and whose
-// contiguous axis is a multiple of 8 long.  BM x BN tiles, k in stages of 64,
-// two stages of both operands in LDS: while a stage is multiplied the next one
-// is on its way from memory straight into LDS (16 bytes a lane, no registers).
-// One barrier a stage: behind it all of this stage has landed (each wave has
-// waited for its own loads) and all waves are done with the other buffer.
+// contiguous axis is a multiple of 8 long.  BM x BN tiles, k in stages of 32,
+// three stages of both operands in LDS: while one is multiplied the next two
+// are on their way from memory straight into LDS (16 bytes a lane, no
+// registers).  One barrier a stage: behind it all of this stage has landed
+// (each wave has waited for its own loads, all but the last stage's) and all
+// waves are done with the buffer that is loaded next.  Two workgroups share a
+// CU, so that one's way out overlaps the other's products.
 //
 // Loads go through a buffer descriptor at the stage's start; a lane whose chunk
 // lies outside its matrix gives an offset past the descriptor's range, for
 // which the hardware writes zeros, so k and both tile edges need no branch.
 //
-// An operand stored along k has 64 k of a row in 128 bytes of LDS, 8 chunks
+// An operand stored along k has 32 k of a row in 64 bytes of LDS, 4 chunks
 // permuted by the row so that the rows of an operand read lie in different
 // banks.  An operand stored along m (the gradients' W, dz and x) stays so in
 // LDS, and ds_read_b64_tr_b16 transposes 4 k x 16 m as it is read: no
@@ -152,12 +169,14 @@ __global__ __launch_bounds__(256) void tile_gemm_kernel(Operand A, Operand B, in
 //
 // The second matrix is the matrix instruction's row operand, so that a lane
 // holds 4 consecutive columns of one row of C at a time.  The finished sums go
-// through LDS, 64 rows of each wave's tile at a time, for whole 128-byte row
+// through LDS, 32 rows of each wave's tile at a time, for whole 128-byte row
 // pieces on the way out and one copy of the epilogue's code.
-constexpr int SK = 64;                          // k of a stage
+constexpr int SK = 32, STAGES = 3;              // k of a stage, stages in LDS
 constexpr uint32_t OUTSIDE = 0x80000000u;       // an offset past every descriptor's range (2^31 bytes)
 
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// until at most LEFT of this wave's loads are on their way
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // 16 bytes a lane from `base` + off to LDS bytes lds .. lds + 1023
@@ -180,8 +199,8 @@ struct Tile {
     uint32_t off[LOADS];  // from base
     int at[LOADS];        // the chunk's k within the stage
 
-    // the place of k chunk c (of 8) in row r's 128 bytes
-    static __device__ __forceinline__ int spread(int r, int c) { return c ^ (r & 7); }
+    // the place of k chunk c (of 4) in row r's 64 bytes
+    static __device__ __forceinline__ int spread(int r, int c) { return c ^ ((r >> 2) & 3); }
     // the place of column chunk c in k row k
     static __device__ __forceinline__ int spread_t(int k, int c) { return c ^ ((4 * (k & 3)) & (R / 8 - 1)); }
 
@@ -198,7 +217,7 @@ struct Tile {
         for (int i = 0; i < LOADS; i++) {
             const int q = i * NT + t;
             if constexpr (!TRANS) {
-                const int r = q >> 3, c = spread(r, q & 7);
+                const int r = q >> 2, c = spread(r, q & 3);
                 at[i] = 8 * c;
                 off[i] = row0 + r < rows ? (uint32_t)(r * o.ld * 2) + 16 * c : OUTSIDE;
             } else {
@@ -219,7 +238,7 @@ struct Tile {
     static __device__ __forceinline__ u32x4 read(const char *lds, int r0, int ks) {
         const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
         if constexpr (!TRANS) {
-            return *(const u32x4 *)(lds + (r0 + c) * 128 + spread(c, 2 * ks + h) * 16);
+            return *(const u32x4 *)(lds + (r0 + c) * 64 + spread(c, 2 * ks + h) * 16);
         } else {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
@@ -282,31 +301,22 @@ __device__ __forceinline__ void add8(const T *p, float *v) {
     }
 }
 
-// 8 consecutive columns of row m: bias, z, activation, residual, y
+// 8 consecutive columns of row m, the bias added: z, activation, residual, y
 template <typename T>
-__device__ __forceinline__ void store8(const Epilogue &e, int64_t m, int64_t n, int64_t N, bool vec, float *v) {
-    const bool whole = vec && n + 8 <= N;
-    if (e.bias) {
-        if (whole) add8(e.bias + n, v);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] += n + i < N ? e.bias[n + i] : 0.f;
-    }
-    if (e.z) {
-        T *z = (T *)e.z + m * e.ldz + n;
-        if (whole) put8(z, v);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (n + i < N) z[i] = (T)v[i];
-    }
-    act8<T>(v, e.act);
+__device__ __forceinline__ void store8(const Epilogue &e, int64_t m, int64_t n, int64_t N, bool whole, float *v) {
+    T *z = (T *)e.z + m * e.ldz + n, *y = (T *)e.y + m * e.ldy + n;
     const T *r = (const T *)e.r + m * e.ldr + n;
-    T *y = (T *)e.y + m * e.ldy + n;
     if (whole) {
+        if (e.z) put8(z, v);
+        act8<T>(v, e.act);
         if (e.r) add8(r, v);
         put8(y, v);
     } else {
+        if (e.z)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (n + i < N) z[i] = (T)v[i];
+        act8<T>(v, e.act);
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (n + i < N) y[i] = (T)(v[i] + (e.r ? (float)r[i] : 0.f));
@@ -321,7 +331,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Operand A, O
                                                                   int64_t k_per_split, float *part, Epilogue e, bool vec) {
     typedef typename Elem<TYPE>::T T;
     constexpr int NT = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
-    static_assert(BN / WN == 64 && BM / WM % 64 == 0, "the epilogue takes 64 x 64 of a wave's tile at a time");
+    static_assert(BN / WN == 64, "the epilogue takes 32 x 64 of a wave's tile at a time");
     typedef Tile<TA, BM, NT> TileA;
     typedef Tile<TBT, BN, NT> TileB;
     constexpr int STAGE = TileA::BYTES + TileB::BYTES;
@@ -340,16 +350,21 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Operand A, O
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
     const int wave = threadIdx.x >> 6, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
     f32x16 acc[TM][TN] = {};
-    ta.load(lds, kb - ka);
-    tb.load(lds + TileA::BYTES, kb - ka);
+    constexpr int LOADS = TileA::LOADS + TileB::LOADS;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) {
+        ta.load(lds + i * STAGE, kb - ka - i * SK);
+        tb.load(lds + i * STAGE + TileA::BYTES, kb - ka - i * SK);
+    }
     int buf = 0;
     for (int64_t k0 = ka; k0 < kb; k0 += SK) {
-        wait_loads();
+        wait_loads<LOADS>();
         barrier();
-        const int64_t left = kb - k0 - SK;
-        if (left > 0) {
-            ta.load(lds + (buf ^ 1) * STAGE, left);
-            tb.load(lds + (buf ^ 1) * STAGE + TileA::BYTES, left);
+        {   // past the end these write zeros that nothing reads: every turn waits for the same count
+            const int64_t left = kb - k0 - (STAGES - 1) * SK;
+            const int to = buf == 0 ? STAGES - 1 : buf - 1;
+            ta.load(lds + to * STAGE, left);
+            tb.load(lds + to * STAGE + TileA::BYTES, left);
         }
         const char *sa = smem + buf * STAGE, *sb = sa + TileA::BYTES;
 #pragma unroll
@@ -364,36 +379,43 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Operand A, O
 #pragma unroll
                 for (int j = 0; j < TN; j++) acc[i][j] = mfma16<TYPE>(b[j], a[i], acc[i][j]);
         }
-        buf ^= 1;
+        buf = buf == STAGES - 1 ? 0 : buf + 1;
     }
-    barrier();  // the stages' last reads are done: the LDS is the epilogue's
+    wait_loads<0>();
+    barrier();  // the stages' last loads and reads are done: the LDS is the epilogue's
     const int lane = threadIdx.x & 63;
-    float *out = (float *)smem + wave * 64 * OUT_LD;
+    float *out = (float *)smem + wave * 32 * OUT_LD;
+    const int64_t n = n0 + wn + 8 * (lane & 7);
+    const bool whole = vec && n + 8 <= N;
+    float bias[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) bias[i] = e.bias && !part && n + i < N ? e.bias[n + i] : 0.f;
 #pragma unroll 1
-    for (int part64 = 0; part64 < TM / 2; part64++) {
+    for (int part32 = 0; part32 < TM; part32++) {
 #pragma unroll
         for (int i = 0; i < TM; i++)
-            if (i / 2 == part64)
+            if (i == part32)
 #pragma unroll
                 for (int j = 0; j < TN; j++)
 #pragma unroll
                     for (int a = 0; a < 4; a++)
-                        *(f32x4 *)(out + (32 * (i & 1) + (lane & 31)) * OUT_LD + 32 * j + 8 * a + 4 * (lane >> 5)) =
+                        *(f32x4 *)(out + (lane & 31) * OUT_LD + 32 * j + 8 * a + 4 * (lane >> 5)) =
                             f32x4{acc[i][j][4 * a], acc[i][j][4 * a + 1], acc[i][j][4 * a + 2], acc[i][j][4 * a + 3]};
-#pragma unroll 2
-        for (int row = lane >> 3; row < 64; row += 8) {
-            const int64_t m = m0 + wm + 64 * part64 + row, n = n0 + wn + 8 * (lane & 7);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = 8 * i + (lane >> 3);
+            const int64_t m = m0 + wm + 32 * part32 + row;
             if (m >= M || n >= N) continue;
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = out[row * OUT_LD + 8 * (lane & 7) + i];
+            for (int j = 0; j < 8; j++) v[j] = out[row * OUT_LD + 8 * (lane & 7) + j] + bias[j];
             if (part) {
                 float *q = part + ((int64_t)blockIdx.z * M + m) * N + n;
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (n + i < N) q[i] = v[i];
+                for (int j = 0; j < 8; j++)
+                    if (n + j < N) q[j] = v[j];
             } else {
-                store8<T>(e, m, n, N, vec, v);
+                store8<T>(e, m, n, N, whole, v);
             }
         }
     }
@@ -408,32 +430,75 @@ __global__ __launch_bounds__(256) void split_join_kernel(const float *part, int 
     }
 }
 
-// dz = dy act'(z) in the layer's type, and its sums over 64 rows at a time
-constexpr int DB_ROWS = 64;
+// dz = dy act'(z) in the layer's type, and the unrounded dz's column sums over
+// `rows` rows at a time: 32 threads of 8 columns each, 8 rows side by side,
+// their sums joined in LDS in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, const T *z, int64_t ldz, int act, int64_t M, int64_t N,
-                                                 T *dz, float *part) {
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
-    for (int64_t b = blockIdx.y; b * DB_ROWS < M; b += gridDim.y) {
-        const int64_t m1 = min(M, (b + 1) * DB_ROWS);
-        float sum = 0.f;
-        for (int64_t m = b * DB_ROWS; m < m1; m++) {
-            float v = (float)dy[m * lddy + n];
-            if (act) v *= act_slope_f((float)z[m * ldz + n], act);
-            if (dz) dz[m * N + n] = (T)v;
-            sum += v;
+                                                 int rows, T *dz, float *part, bool vec) {
+    __shared__ float sums[8][32][9];
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 256 + 8 * c, m1 = min(M, (int64_t)(blockIdx.y + 1) * rows);
+    const bool whole = vec && n + 8 <= N;
+    float sum[8] = {};
+    for (int64_t m = (int64_t)blockIdx.y * rows + r; m < m1; m += 8) {
+        float v[8] = {}, s[8] = {};
+        if (whole) {
+            add8(dy + m * lddy + n, v);
+            if (act) add8(z + m * ldz + n, s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (n + i < N) {
+                    v[i] = (float)dy[m * lddy + n + i];
+                    if (act) s[i] = (float)z[m * ldz + n + i];
+                }
         }
-        if (part) part[b * N + n] = sum;
+        slope8(v, s, act);
+        if (dz) {
+            if (whole && N % 8 == 0) put8(dz + m * N + n, v);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (n + i < N) dz[m * N + n + i] = (T)v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum[i] += v[i];
     }
+    if (!part) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++) sums[r][c][i] = sum[i];
+    __syncthreads();
+    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (col >= N) return;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v += sums[i][threadIdx.x >> 3][threadIdx.x & 7];
+    part[blockIdx.y * N + col] = v;
 }
 
+// the column sums of `part`: 32 columns, 8 rows side by side
 __global__ __launch_bounds__(256) void column_sum_kernel(const float *part, int64_t rows, int64_t N, float *out) {
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
+    __shared__ float sums[8][33];
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 32 + c;
     float v = 0.f;
-    for (int64_t b = 0; b < rows; b++) v += part[b * N + n];
+    if (n < N)
+        for (int64_t b = r; b < rows; b += 8) v += part[b * N + n];
+    sums[r][c] = v;
+    __syncthreads();
+    if (r || n >= N) return;
+#pragma unroll
+    for (int i = 1; i < 8; i++) v += sums[i][c];
     out[n] = v;
+}
+
+// rows of a dz_kernel workgroup: about 2048 workgroups, and no more partial sums than that
+int dz_rows(int64_t M, int64_t N) {
+    int64_t rows = 8;
+    while (rows < M && ceil_div(M, rows) * ceil_div<int64_t>(N, 256) > 2048) rows *= 2;
+    while (ceil_div(M, rows) > 2048) rows *= 2;
+    return (int)std::min<int64_t>(rows, 1 << 30);
 }
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -449,8 +514,8 @@ struct Plan {
 Plan plan_for(bool fits, int64_t M, int64_t N, int64_t K) {
     Plan p = {TB, TB, 1, 0};
     if (fits) {
-        p.bm = p.bn = 256;
-        if (ceil_div<int64_t>(M, 256) * ceil_div<int64_t>(N, 256) < 192) p.bm = p.bn = 128;
+        p.bm = 128, p.bn = 256;
+        if (ceil_div<int64_t>(M, 128) * ceil_div<int64_t>(N, 256) < 384) p.bn = 128;
     }
     const int64_t tiles = ceil_div<int64_t>(M, p.bm) * ceil_div<int64_t>(N, p.bn);
     if (tiles > 0 && tiles < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, K / 256));
@@ -471,7 +536,7 @@ bool stage_operand(const Operand &o, bool trans, int64_t rows, int64_t k) {
 template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
 void launch_stage(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, const Plan &p, float *part, const Epilogue &e,
                   bool vec, hipStream_t s) {
-    constexpr int lds = std::max(2 * (BM + BN) * SK * 2, WM * WN * 64 * OUT_LD * 4);
+    constexpr int lds = std::max(STAGES * (BM + BN) * SK * 2, WM * WN * 32 * OUT_LD * 4);
     const auto k = stage_gemm_kernel<TYPE, TA, TBT, BM, BN, WM, WN>;
     (void)hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     const int64_t tiles = ceil_div<int64_t>(M, BM) * ceil_div<int64_t>(N, BN);
@@ -487,12 +552,12 @@ hipError_t gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_
     if constexpr (TYPE != BERT_AMD_F32) {
         const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(T)); };
         const bool vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr) && ok(e.bias, 4);
-        if (p.bm == 256)
-            launch_stage<TYPE, TA, TBT, 256, 256, 2, 4>(A, B, M, N, K, p, part, e, vec, s);
-        else if (p.bm == 128)
+        if (p.bn == 256)
+            launch_stage<TYPE, TA, TBT, 128, 256, 1, 4>(A, B, M, N, K, p, part, e, vec, s);
+        else if (p.bn == 128)
             launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
     }
-    if (p.bm == TB) {
+    if (p.bn == TB) {
         const int64_t tiles = ceil_div<int64_t>(M, TB) * ceil_div<int64_t>(N, TB);
         hipLaunchKernelGGL((tile_gemm_kernel<TYPE, TA, TBT>), dim3(tiles, 1, p.splits), dim3(256), 0, s, A, B, M, N, K, p.per, part, e);
     }
@@ -521,13 +586,15 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         dz = operand(kept, a.N, TYPE);
     }
     if (kept || a.db) {
-        const int64_t blocks = ceil_div<int64_t>(a.M, DB_ROWS);
+        const int rows = dz_rows(a.M, a.N);
+        const int64_t blocks = ceil_div<int64_t>(a.M, rows);
         float *part = a.db ? (float *)ws : nullptr;
+        const bool vec = aligned16(a.dy, a.lddy * (int64_t)sizeof(T)) && (!a.act || aligned16(a.z, a.ldz * (int64_t)sizeof(T)));
         if (blocks)
-            hipLaunchKernelGGL((dz_kernel<T>), dim3(ceil_div(a.N, 256), std::min<int64_t>(blocks, 65535)), dim3(256), 0, s, (const T *)a.dy,
-                           a.lddy, (const T *)a.z, a.ldz, a.act, a.M, (int64_t)a.N, kept, part);
+            hipLaunchKernelGGL((dz_kernel<T>), dim3(ceil_div(a.N, 256), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z,
+                               a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, part, vec);
         if (a.db) {
-            hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 256)), dim3(256), 0, s, part, blocks, (int64_t)a.N, a.db);
+            hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 32)), dim3(256), 0, s, part, blocks, (int64_t)a.N, a.db);
             ws += round256(blocks * a.N * 4);
         }
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
@@ -560,7 +627,7 @@ hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
 }
 
 int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K) {
-    return (act ? round256(M * N * elem_size(type)) : 0) + round256(ceil_div<int64_t>(M, DB_ROWS) * N * 4) +
+    return (act ? round256(M * N * elem_size(type)) : 0) + round256(ceil_div<int64_t>(M, dz_rows(M, N)) * N * 4) +
            std::max(std::max(split_bytes(false, M, K, N), split_bytes(true, M, K, N)),
                     std::max(split_bytes(false, N, K, M), split_bytes(true, N, K, M)));
 }
