@@ -31,10 +31,12 @@ $(BUILD)/obj/%.o: $(SRC)/%.hip $(SRC)/kernels.h $(SRC)/kernels_common.h $(SRC)/i
 	@mkdir -p $(dir $@)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
-# the operators are built without the packed f32 instructions
+# the operators are built without the packed f32 instructions, and with the matrix units'
+# sums where the compiler puts them (256 of them beside 113 other registers a lane)
+OPSFLAGS := $(filter-out -mllvm -amdgpu-mfma-vgpr-form,$(HIPFLAGS)) -Xclang -target-feature -Xclang -packed-fp32-ops
 $(BUILD)/obj/ops_%.o: $(SRC)/ops_%.hip $(SRC)/ops.h $(SRC)/ops_common.h include/bert_amd.h
 	@mkdir -p $(dir $@)
-	$(HIPCC) $(HIPFLAGS) -Xclang -target-feature -Xclang -packed-fp32-ops -c $< -o $@
+	$(HIPCC) $(OPSFLAGS) -c $< -o $@
 
 $(BUILD)/libbert.so: $(HOST_OBJS) $(HIP_OBJS) $(OPS_OBJS)
 	$(HIPCC) -shared -fPIC --offload-arch=$(ARCH) -o $@ $^ -lpthread

@@ -77,8 +77,9 @@ __device__ __forceinline__ float act_t(float z) {
     if constexpr (!WIDE && ACT == BERT_AMD_ACT_GELU) return z * sigmoid_16(2.f * GELU_C * (z + GELU_K * z * z * z));
     else if constexpr (!WIDE && ACT == BERT_AMD_ACT_SILU) return z * sigmoid_16(z);
     else if constexpr (!WIDE && ACT == BERT_AMD_ACT_TANH) {
-        const float q = z * z;  // next to zero the quotient would cancel: the odd series up to z^7
-        return q < 0.0625f ? z * (1.f + q * (-1.f / 3 + q * (2.f / 15 - q * (17.f / 315)))) : 1.f - 2.f * sigmoid_16(-2.f * z);
+        const float q = z * z, far = 1.f - 2.f * sigmoid_16(-2.f * z);
+        const float near = z * (1.f + q * (-1.f / 3 + q * (2.f / 15 - q * (17.f / 315))));  // next to zero, where `far` cancels
+        return q < 0.0625f ? near : far;
     } else return act_f(z, ACT);
 }
 

@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 namespace bertamd {
 
@@ -169,14 +170,17 @@ __global__ __launch_bounds__(256) void tile_gemm_kernel(Operand A, Operand B, in
 //
 // The second matrix is the matrix instruction's row operand, so that a lane
 // holds 4 consecutive columns of one row of C at a time.  The finished sums go
-// through LDS, 32 rows of each wave's tile at a time, for whole 128-byte row
-// pieces on the way out and one copy of the epilogue's code.
-constexpr int SK = 32, STAGES = 3;              // k of a stage, stages in LDS
+// through LDS, 64 columns of each wave's tile at a time, for whole 128-byte
+// row pieces on the way out.  One wave a SIMD has nothing to hide latencies
+// behind there, so inside the matrix four rows' reads, loads and stores go
+// together without a branch between them.
+constexpr int SK = 64;                          // k of a stage
 constexpr uint32_t OUTSIDE = 0x80000000u;       // an offset past every descriptor's range (2^31 bytes)
 
 // until at most LEFT of this wave's loads are on their way
 template <int LEFT>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // 16 bytes a lane from `base` + off to LDS bytes lds .. lds + 1023
@@ -199,8 +203,8 @@ struct Tile {
     uint32_t off[LOADS];  // from base
     int at[LOADS];        // the chunk's k within the stage
 
-    // the place of k chunk c (of 4) in row r's 64 bytes
-    static __device__ __forceinline__ int spread(int r, int c) { return c ^ ((r >> 2) & 3); }
+    // the place of k chunk c (of 8) in row r's 128 bytes
+    static __device__ __forceinline__ int spread(int r, int c) { return c ^ (r & 7); }
     // the place of column chunk c in k row k
     static __device__ __forceinline__ int spread_t(int k, int c) { return c ^ ((4 * (k & 3)) & (R / 8 - 1)); }
 
@@ -217,7 +221,7 @@ struct Tile {
         for (int i = 0; i < LOADS; i++) {
             const int q = i * NT + t;
             if constexpr (!TRANS) {
-                const int r = q >> 2, c = spread(r, q & 3);
+                const int r = q >> 3, c = spread(r, q & 7);
                 at[i] = 8 * c;
                 off[i] = row0 + r < rows ? (uint32_t)(r * o.ld * 2) + 16 * c : OUTSIDE;
             } else {
@@ -227,18 +231,20 @@ struct Tile {
             }
         }
     }
-    __device__ __forceinline__ void load(uint32_t lds, int64_t k_left) {
+    // loads FROM .. TO - 1 of a stage to `lds`; `left`: k from the stage's start to the end
+    template <int FROM, int TO>
+    __device__ __forceinline__ void load(uint32_t lds, int left) {
         const u32x4 d = descriptor(base);
         const uint32_t w = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x >> 6) * 1024);
 #pragma unroll
-        for (int i = 0; i < LOADS; i++) load_to_lds(d, at[i] < k_left ? off[i] : OUTSIDE, w + i * NT * 16);
-        base += step;
+        for (int i = FROM; i < TO; i++) load_to_lds(d, at[i] < left ? off[i] : OUTSIDE, w + i * NT * 16);
+        if (TO == LOADS) base += step;
     }
     // operand registers of rows r0 .. r0 + 31, k 16 ks .. 16 ks + 15 of the stage at `lds`
     static __device__ __forceinline__ u32x4 read(const char *lds, int r0, int ks) {
         const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
         if constexpr (!TRANS) {
-            return *(const u32x4 *)(lds + (r0 + c) * 64 + spread(c, 2 * ks + h) * 16);
+            return *(const u32x4 *)(lds + (r0 + c) * 128 + spread(c, 2 * ks + h) * 16);
         } else {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
@@ -254,6 +260,12 @@ struct Tile {
     }
 };
 
+template <int... I, typename F>
+__device__ __forceinline__ void for_const_(std::integer_sequence<int, I...>, const F &f) { (f(std::integral_constant<int, I>()), ...); }
+// f(0), .. f(N - 1), each number a constant
+template <int N, typename F>
+__device__ __forceinline__ void for_const(const F &f) { for_const_(std::make_integer_sequence<int, N>(), f); }
+
 template <int TYPE>
 __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c) {
     if constexpr (TYPE == BERT_AMD_F16)
@@ -262,12 +274,13 @@ __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <typename T>
-__device__ __forceinline__ void act8(float *v, int act) {
+// v = act(v), N at a time: one choice of the activation
+template <typename T, int N>
+__device__ __forceinline__ void act_n(float *v, int act) {
     constexpr bool WIDE = sizeof(T) == 4;
     const auto each = [&](auto a) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = act_t<decltype(a)::value, WIDE>(v[i]);
+        for (int i = 0; i < N; i++) v[i] = act_t<decltype(a)::value, WIDE>(v[i]);
     };
     switch (act) {
         case BERT_AMD_ACT_RELU: each(std::integral_constant<int, BERT_AMD_ACT_RELU>()); break;
@@ -301,37 +314,30 @@ __device__ __forceinline__ void add8(const T *p, float *v) {
     }
 }
 
-// 8 consecutive columns of row m, the bias added: z, activation, residual, y
+// 8 consecutive columns of row m, the bias added, some of them past the end or not aligned: z, activation, residual, y
 template <typename T>
-__device__ __forceinline__ void store8(const Epilogue &e, int64_t m, int64_t n, int64_t N, bool whole, float *v) {
+__device__ __forceinline__ void store_edge(const Epilogue &e, int64_t m, int64_t n, int64_t N, float *v) {
     T *z = (T *)e.z + m * e.ldz + n, *y = (T *)e.y + m * e.ldy + n;
     const T *r = (const T *)e.r + m * e.ldr + n;
-    if (whole) {
-        if (e.z) put8(z, v);
-        act8<T>(v, e.act);
-        if (e.r) add8(r, v);
-        put8(y, v);
-    } else {
-        if (e.z)
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (n + i < N) z[i] = (T)v[i];
-        act8<T>(v, e.act);
+    if (e.z)
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (n + i < N) y[i] = (T)(v[i] + (e.r ? (float)r[i] : 0.f));
-    }
+            if (n + i < N) z[i] = (T)v[i];
+    act_n<T, 8>(v, e.act);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (n + i < N) y[i] = (T)(v[i] + (e.r ? (float)r[i] : 0.f));
 }
 
 // LDS row of the epilogue: a wave's 64 columns and 16 bytes more, so that the rows of a write start in different banks
 constexpr int OUT_LD = 68;
 
 template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Operand A, Operand B, int64_t M, int64_t N, int64_t K,
+__global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_kernel(Operand A, Operand B, int64_t M, int64_t N, int64_t K,
                                                                   int64_t k_per_split, float *part, Epilogue e, bool vec) {
     typedef typename Elem<TYPE>::T T;
     constexpr int NT = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
-    static_assert(BN / WN == 64, "the epilogue takes 32 x 64 of a wave's tile at a time");
+    static_assert(BN / WN % 64 == 0, "the epilogue takes 64 columns of a wave's tile at a time");
     typedef Tile<TA, BM, NT> TileA;
     typedef Tile<TBT, BN, NT> TileB;
     constexpr int STAGE = TileA::BYTES + TileB::BYTES;
@@ -349,73 +355,115 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Operand A, O
     tb.init(B, n0, N, ka);
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
     const int wave = threadIdx.x >> 6, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    // this lane's columns' bias, on its way from here (none: zeros; past the end: the last one, not used)
+    const int lane = threadIdx.x & 63;
+    float biases[TN / 2][8] = {};
+    if (e.bias && !part)
+#pragma unroll
+        for (int h = 0; h < TN / 2; h++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) biases[h][i] = e.bias[min(n0 + wn + 64 * h + 8 * (lane & 7) + i, N - 1)];
     f32x16 acc[TM][TN] = {};
-    constexpr int LOADS = TileA::LOADS + TileB::LOADS;
+    constexpr int KS = SK / 16;
+    u32x4 a[2][TM], b[2][TN];
+    const auto read_a = [&](int set, int i, int from, int ks) { a[set][i] = TileA::read(smem + from * STAGE, wm + 32 * i, ks); };
+    const auto read_b = [&](int set, int i, int from, int ks) { b[set][i] = TileB::read(smem + from * STAGE + TileA::BYTES, wn + 32 * i, ks); };
+    const auto left_at = [&](int64_t k0) { return (int)max((int64_t)0, min((int64_t)SK, kb - k0)); };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) {
-        ta.load(lds + i * STAGE, kb - ka - i * SK);
-        tb.load(lds + i * STAGE + TileA::BYTES, kb - ka - i * SK);
+    for (int i = 0; i < 2; i++) {
+        ta.template load<0, TileA::LOADS>(lds + i * STAGE, left_at(ka + i * SK));
+        tb.template load<0, TileB::LOADS>(lds + i * STAGE + TileA::BYTES, left_at(ka + i * SK));
     }
+    wait_loads<TileA::LOADS + TileB::LOADS>();
+    barrier();
+#pragma unroll
+    for (int i = 0; i < TN; i++) read_b(0, i, 0, 0);
+#pragma unroll
+    for (int i = 0; i < TM; i++) read_a(0, i, 0, 0);
     int buf = 0;
-    for (int64_t k0 = ka; k0 < kb; k0 += SK) {
-        wait_loads<LOADS>();
-        barrier();
-        {   // past the end these write zeros that nothing reads: every turn waits for the same count
-            const int64_t left = kb - k0 - (STAGES - 1) * SK;
-            const int to = buf == 0 ? STAGES - 1 : buf - 1;
-            ta.load(lds + to * STAGE, left);
-            tb.load(lds + to * STAGE + TileA::BYTES, left);
+    for (int64_t k0 = ka; k0 < kb; k0 += SK, buf ^= 1) {
+        // The loads of the stage after the next go out between the products of
+        // this stage's last 16 k (its second matrix, once the barrier has freed
+        // the buffer) and the next stage's first (its first matrix): a burst of them would hold up
+        // the products behind it, and they have half a stage left to arrive in.
+        // Past the end they write zeros, and the last reads take what nothing multiplies.
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int set = ks & 1, next = set ^ 1, from = ks < KS - 1 ? buf : buf ^ 1, kn = (ks + 1) % KS;
+            if (ks == KS - 1) {
+                wait_reads();
+                wait_loads<0>();
+                barrier();
+            }
+            for_const<TM>([&](auto ic) {
+                constexpr int i = ic.value;
+                if (ks == KS - 1) tb.template load<i * TileB::LOADS / TM, (i + 1) * TileB::LOADS / TM>(lds + buf * STAGE + TileA::BYTES, left_at(k0 + 2 * SK));
+                if (ks == 0) if (k0 > ka) ta.template load<i * TileA::LOADS / TM, (i + 1) * TileA::LOADS / TM>(lds + (buf ^ 1) * STAGE, left_at(k0 + SK));
+                if (i < TN) read_b(next, i, from, kn);
+                read_a(next, i, from, kn);
+#pragma unroll
+                for (int j = 0; j < TN; j++) acc[i][j] = mfma16<TYPE>(b[set][j], a[set][i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
         }
-        const char *sa = smem + buf * STAGE, *sb = sa + TileA::BYTES;
-#pragma unroll
-        for (int ks = 0; ks < SK / 16; ks++) {
-            u32x4 a[TM], b[TN];
-#pragma unroll
-            for (int i = 0; i < TN; i++) b[i] = TileB::read(sb, wn + 32 * i, ks);
-#pragma unroll
-            for (int i = 0; i < TM; i++) a[i] = TileA::read(sa, wm + 32 * i, ks);
-#pragma unroll
-            for (int i = 0; i < TM; i++)
-#pragma unroll
-                for (int j = 0; j < TN; j++) acc[i][j] = mfma16<TYPE>(b[j], a[i], acc[i][j]);
-        }
-        buf = buf == STAGES - 1 ? 0 : buf + 1;
     }
+    wait_reads();
     wait_loads<0>();
     barrier();  // the stages' last loads and reads are done: the LDS is the epilogue's
-    const int lane = threadIdx.x & 63;
-    float *out = (float *)smem + wave * 32 * OUT_LD;
-    const int64_t n = n0 + wn + 8 * (lane & 7);
-    const bool whole = vec && n + 8 <= N;
-    float bias[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) bias[i] = e.bias && !part && n + i < N ? e.bias[n + i] : 0.f;
+    constexpr int WR = BM / WM, G = 4;
+    float *out = (float *)smem + wave * WR * OUT_LD;
+    const int row0 = lane >> 3, col = 8 * (lane & 7);
 #pragma unroll 1
-    for (int part32 = 0; part32 < TM; part32++) {
+    for (int half = 0; half < TN / 2; half++) {
+        const int64_t n = n0 + wn + 64 * half + col, m = m0 + wm + row0;
+        float bias[8];
 #pragma unroll
-        for (int i = 0; i < TM; i++)
-            if (i == part32)
+        for (int i = 0; i < 8; i++) bias[i] = half ? biases[1 % (TN / 2)][i] : biases[0][i];
 #pragma unroll
-                for (int j = 0; j < TN; j++)
+        for (int j = 0; j < TN; j++)
+            if (j / 2 == half)
 #pragma unroll
-                    for (int a = 0; a < 4; a++)
-                        *(f32x4 *)(out + (lane & 31) * OUT_LD + 32 * j + 8 * a + 4 * (lane >> 5)) =
-                            f32x4{acc[i][j][4 * a], acc[i][j][4 * a + 1], acc[i][j][4 * a + 2], acc[i][j][4 * a + 3]};
+                for (int i = 0; i < TM; i++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int row = 8 * i + (lane >> 3);
-            const int64_t m = m0 + wm + 32 * part32 + row;
-            if (m >= M || n >= N) continue;
-            float v[8];
+                    for (int c = 0; c < 4; c++)
+                        *(f32x4 *)(out + (32 * i + (lane & 31)) * OUT_LD + 32 * (j & 1) + 8 * c + 4 * (lane >> 5)) =
+                            f32x4{acc[i][j][4 * c], acc[i][j][4 * c + 1], acc[i][j][4 * c + 2], acc[i][j][4 * c + 3]};
+        if (vec && !part && m0 + BM <= M && n0 + BN <= N) {
+            const T *r = (const T *)e.r + m * e.ldr + n;
+            T *y = (T *)e.y + m * e.ldy + n, *z = (T *)e.z + m * e.ldz + n;
+#pragma unroll 1
+            for (int g = 0; g < WR; g += 8 * G) {
+                float v[8 * G];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = out[row * OUT_LD + 8 * (lane & 7) + j] + bias[j];
-            if (part) {
-                float *q = part + ((int64_t)blockIdx.z * M + m) * N + n;
+                for (int i = 0; i < G; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (n + j < N) q[j] = v[j];
-            } else {
-                store8<T>(e, m, n, N, whole, v);
+                    for (int c = 0; c < 8; c++) v[8 * i + c] = out[(g + 8 * i + row0) * OUT_LD + col + c] + bias[c];
+                if (e.z)
+#pragma unroll
+                    for (int i = 0; i < G; i++) put8(z + (g + 8 * i) * e.ldz, v + 8 * i);
+                act_n<T, 8 * G>(v, e.act);
+                if (e.r)
+#pragma unroll
+                    for (int i = 0; i < G; i++) add8(r + (g + 8 * i) * e.ldr, v + 8 * i);
+#pragma unroll
+                for (int i = 0; i < G; i++) put8(y + (g + 8 * i) * e.ldy, v + 8 * i);
+            }
+        } else if (n < N) {
+#pragma unroll 1
+            for (int g = 0; g < WR && m + g < M; g += 8) {
+                float v[8];
+#pragma unroll
+                for (int c = 0; c < 8; c++) v[c] = out[(g + row0) * OUT_LD + col + c] + bias[c];
+                if (part) {
+                    float *q = part + ((int64_t)blockIdx.z * M + m + g) * N + n;
+                    if (N % 4 == 0 && n + 8 <= N) put8(q, v);
+                    else
+#pragma unroll
+                        for (int c = 0; c < 8; c++)
+                            if (n + c < N) q[c] = v[c];
+                } else {
+                    store_edge<T>(e, m + g, n, N, v);
+                }
             }
         }
     }
@@ -514,8 +562,8 @@ struct Plan {
 Plan plan_for(bool fits, int64_t M, int64_t N, int64_t K) {
     Plan p = {TB, TB, 1, 0};
     if (fits) {
-        p.bm = 128, p.bn = 256;
-        if (ceil_div<int64_t>(M, 128) * ceil_div<int64_t>(N, 256) < 384) p.bn = 128;
+        p.bm = p.bn = 256;
+        if (ceil_div<int64_t>(M, 256) * ceil_div<int64_t>(N, 256) < 192) p.bm = p.bn = 128;
     }
     const int64_t tiles = ceil_div<int64_t>(M, p.bm) * ceil_div<int64_t>(N, p.bn);
     if (tiles > 0 && tiles < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, K / 256));
@@ -536,7 +584,7 @@ bool stage_operand(const Operand &o, bool trans, int64_t rows, int64_t k) {
 template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
 void launch_stage(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, const Plan &p, float *part, const Epilogue &e,
                   bool vec, hipStream_t s) {
-    constexpr int lds = std::max(STAGES * (BM + BN) * SK * 2, WM * WN * 32 * OUT_LD * 4);
+    constexpr int lds = std::max(2 * (BM + BN) * SK * 2, BM * WN * OUT_LD * 4);
     const auto k = stage_gemm_kernel<TYPE, TA, TBT, BM, BN, WM, WN>;
     (void)hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     const int64_t tiles = ceil_div<int64_t>(M, BM) * ceil_div<int64_t>(N, BN);
@@ -551,9 +599,9 @@ hipError_t gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_
     float *part = p.splits > 1 ? (float *)ws : nullptr;
     if constexpr (TYPE != BERT_AMD_F32) {
         const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(T)); };
-        const bool vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr) && ok(e.bias, 4);
+        const bool vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr);
         if (p.bn == 256)
-            launch_stage<TYPE, TA, TBT, 128, 256, 1, 4>(A, B, M, N, K, p, part, e, vec, s);
+            launch_stage<TYPE, TA, TBT, 256, 256, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
         else if (p.bn == 128)
             launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
     }
