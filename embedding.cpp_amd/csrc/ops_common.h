@@ -83,4 +83,19 @@ __device__ __forceinline__ float act_t(float z) {
     } else return act_f(z, ACT);
 }
 
+template <int ACT, bool WIDE>
+__device__ __forceinline__ float act_slope_t(float z) {
+    if constexpr (!WIDE && (ACT == BERT_AMD_ACT_GELU || ACT == BERT_AMD_ACT_SILU)) {
+        z = z > 90.f ? 90.f : z < -90.f ? -90.f : z;
+        constexpr bool G = ACT == BERT_AMD_ACT_GELU;
+        const float q = z * z, s = sigmoid_16(G ? 2.f * GELU_C * z * (1.f + GELU_K * q) : z);
+        return s + z * s * (1.f - s) * (G ? 2.f * GELU_C * (1.f + 3.f * GELU_K * q) : 1.f);
+    } else if constexpr (!WIDE && ACT == BERT_AMD_ACT_TANH) {
+        const float t = act_t<ACT, false>(z);
+        return (1.f - t) * (1.f + t);
+    } else {
+        return act_slope_f(z, ACT);
+    }
+}
+
 }  // namespace bertamd

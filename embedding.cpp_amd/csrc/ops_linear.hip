@@ -16,10 +16,11 @@ namespace bertamd {
 namespace {
 
 // v *= act'(z), 8 at a time: one choice of the activation
+template <typename T>
 __device__ __forceinline__ void slope8(float *v, const float *z, int act) {
     const auto each = [&](auto a) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= act_slope_f(z[i], decltype(a)::value);
+        for (int i = 0; i < 8; i++) v[i] *= act_slope_t<decltype(a)::value, sizeof(T) == 4>(z[i]);
     };
     switch (act) {
         case BERT_AMD_ACT_RELU: each(std::integral_constant<int, BERT_AMD_ACT_RELU>()); break;
@@ -147,34 +148,32 @@ __global__ __launch_bounds__(256) void tile_gemm_kernel(Operand A, Operand B, in
     }
 }
 
-// ---- the tile kernel for 16-bit operands in whole chunks ---------------------
+// ---- the tile kernel for operands in whole chunks ---------------------------
 //
 // The same products from operands whose rows are 16-byte aligned and whose
-// contiguous axis is a multiple of 8 long.  BM x BN tiles, k in stages of 32,
-// three stages of both operands in LDS: while one is multiplied the next two
-// are on their way from memory straight into LDS (16 bytes a lane, no
-// registers).  One barrier a stage: behind it all of this stage has landed
-// (each wave has waited for its own loads, all but the last stage's) and all
-// waves are done with the buffer that is loaded next.  Two workgroups share a
-// CU, so that one's way out overlaps the other's products.
+// contiguous axis is a multiple of 16 bytes long.  BM x BN tiles, k in stages
+// of 128 bytes (64 k, in f32 32), two stages of both operands in LDS, loaded
+// from memory straight into it (16 bytes a lane, no registers).  One barrier a
+// stage: behind it all of the next stage has landed (each wave has waited for
+// its own loads) and all waves have taken this stage's last operands, so that
+// its buffer is free.
 //
 // Loads go through a buffer descriptor at the stage's start; a lane whose chunk
 // lies outside its matrix gives an offset past the descriptor's range, for
 // which the hardware writes zeros, so k and both tile edges need no branch.
 //
-// An operand stored along k has 32 k of a row in 64 bytes of LDS, 4 chunks
-// permuted by the row so that the rows of an operand read lie in different
-// banks.  An operand stored along m (the gradients' W, dz and x) stays so in
-// LDS, and ds_read_b64_tr_b16 transposes 4 k x 16 m as it is read: no
-// transposed copy is made in memory.
+// An operand stored along k has 128 bytes of a row's k side by side in LDS, 8
+// chunks permuted by the row so that the rows of an operand read lie in
+// different banks.  An operand stored along m (the gradients' W, dz and x)
+// stays so in LDS; ds_read_b64_tr_b16 transposes 4 k x 16 m as it is read, and
+// f32 reads its 4 k one by one: no transposed copy is made in memory.
 //
 // The second matrix is the matrix instruction's row operand, so that a lane
 // holds 4 consecutive columns of one row of C at a time.  The finished sums go
 // through LDS, 64 columns of each wave's tile at a time, for whole 128-byte
 // row pieces on the way out.  One wave a SIMD has nothing to hide latencies
-// behind there, so inside the matrix four rows' reads, loads and stores go
+// behind there, so inside the matrix several rows' reads, loads and stores go
 // together without a branch between them.
-constexpr int SK = 64;                          // k of a stage
 constexpr uint32_t OUTSIDE = 0x80000000u;       // an offset past every descriptor's range (2^31 bytes)
 
 // until at most LEFT of this wave's loads are on their way
@@ -193,11 +192,15 @@ __device__ __forceinline__ u32x4 descriptor(const char *base) {
                  (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(b >> 32) & 0xffffu)), OUTSIDE, 0x00020000u};
 }
 
+template <int TYPE> constexpr int stage_k() { return TYPE == BERT_AMD_F32 ? 32 : 64; }
+
 // one operand's tile of R rows (of the product; its contiguous axis if TRANS)
-template <bool TRANS, int R, int NT>
+template <int TYPE, bool TRANS, int R, int NT>
 struct Tile {
-    static constexpr int LOADS = R * SK * 2 / 16 / NT;  // 16-byte chunks a thread loads per stage
-    static constexpr int BYTES = R * SK * 2;
+    typedef typename Elem<TYPE>::T T;
+    static constexpr int SK = stage_k<TYPE>(), CH = Elem<TYPE>::CH, S = sizeof(T);
+    static constexpr int BYTES = R * 128, LOADS = BYTES / 16 / NT;  // 16-byte chunks a thread loads per stage
+    static constexpr int CHUNKS = R / CH;                           // of a k row, if TRANS
     const char *base;     // of the stage to load next
     int64_t step;         // bytes from a stage to the next
     uint32_t off[LOADS];  // from base
@@ -205,29 +208,29 @@ struct Tile {
 
     // the place of k chunk c (of 8) in row r's 128 bytes
     static __device__ __forceinline__ int spread(int r, int c) { return c ^ (r & 7); }
-    // the place of column chunk c in k row k
-    static __device__ __forceinline__ int spread_t(int k, int c) { return c ^ ((4 * (k & 3)) & (R / 8 - 1)); }
+    // the place of column chunk c in k row k: what a read takes at once (4 k of 32 columns; in f32 2 k, 4 apart) in different banks
+    static __device__ __forceinline__ int spread_t(int k, int c) { return c ^ ((TYPE == BERT_AMD_F32 ? 2 * (k & 4) : 4 * (k & 3)) & (CHUNKS - 1)); }
 
     __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t rows, int64_t k0) {
         const int t = threadIdx.x;
         if constexpr (!TRANS) {
-            base = (const char *)o.p + (row0 * o.ld + k0) * 2;
-            step = SK * 2;
+            base = (const char *)o.p + (row0 * o.ld + k0) * S;
+            step = SK * S;
         } else {
-            base = (const char *)o.p + (k0 * o.ld + row0) * 2;
-            step = SK * o.ld * 2;
+            base = (const char *)o.p + (k0 * o.ld + row0) * S;
+            step = SK * o.ld * S;
         }
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int q = i * NT + t;
             if constexpr (!TRANS) {
                 const int r = q >> 3, c = spread(r, q & 7);
-                at[i] = 8 * c;
-                off[i] = row0 + r < rows ? (uint32_t)(r * o.ld * 2) + 16 * c : OUTSIDE;
+                at[i] = CH * c;
+                off[i] = row0 + r < rows ? (uint32_t)(r * o.ld * S) + 16 * c : OUTSIDE;
             } else {
-                const int k = q / (R / 8), c = spread_t(k, q % (R / 8));
+                const int k = q / CHUNKS, c = spread_t(k, q % CHUNKS);
                 at[i] = k;
-                off[i] = row0 + 8 * c < rows ? (uint32_t)(k * o.ld * 2) + 16 * c : OUTSIDE;
+                off[i] = row0 + CH * c < rows ? (uint32_t)(k * o.ld * S) + 16 * c : OUTSIDE;
             }
         }
     }
@@ -240,11 +243,18 @@ struct Tile {
         for (int i = FROM; i < TO; i++) load_to_lds(d, at[i] < left ? off[i] : OUTSIDE, w + i * NT * 16);
         if (TO == LOADS) base += step;
     }
-    // operand registers of rows r0 .. r0 + 31, k 16 ks .. 16 ks + 15 of the stage at `lds`
+    // operand registers of rows r0 .. r0 + 31 and chunks 2 ks, 2 ks + 1 of the stage at `lds`: lane half h has chunk 2 ks + h's k
     static __device__ __forceinline__ u32x4 read(const char *lds, int r0, int ks) {
         const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
         if constexpr (!TRANS) {
             return *(const u32x4 *)(lds + (r0 + c) * 128 + spread(c, 2 * ks + h) * 16);
+        } else if constexpr (TYPE == BERT_AMD_F32) {
+            const int col = r0 + c;
+            const char *p = lds + (8 * ks + 4 * h) * (R * 4) + spread_t(4 * h, col >> 2) * 16 + (col & 3) * 4;
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = *(const uint32_t *)(p + i * R * 4);
+            return v;
         } else {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
@@ -266,12 +276,19 @@ __device__ __forceinline__ void for_const_(std::integer_sequence<int, I...>, con
 template <int N, typename F>
 __device__ __forceinline__ void for_const(const F &f) { for_const_(std::make_integer_sequence<int, N>(), f); }
 
+// c += the products of two operands' 32 rows over the 16 (f32: 8) k that `read` gave
 template <int TYPE>
-__device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c) {
-    if constexpr (TYPE == BERT_AMD_F16)
+__device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (TYPE == BERT_AMD_F16) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else
+    } else if constexpr (TYPE == BERT_AMD_BF16) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)  // k and k + 4 at a time, the same order in both operands
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+        return c;
+    }
 }
 
 // v = act(v), N at a time: one choice of the activation
@@ -338,8 +355,8 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_ker
     typedef typename Elem<TYPE>::T T;
     constexpr int NT = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
     static_assert(BN / WN % 64 == 0, "the epilogue takes 64 columns of a wave's tile at a time");
-    typedef Tile<TA, BM, NT> TileA;
-    typedef Tile<TBT, BN, NT> TileB;
+    typedef Tile<TYPE, TA, BM, NT> TileA;
+    typedef Tile<TYPE, TBT, BN, NT> TileB;
     constexpr int STAGE = TileA::BYTES + TileB::BYTES;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     // workgroups of one XCD take neighbouring tiles, 8 tile rows at a time: they share operand rows in its L2
@@ -364,7 +381,7 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_ker
 #pragma unroll
             for (int i = 0; i < 8; i++) biases[h][i] = e.bias[min(n0 + wn + 64 * h + 8 * (lane & 7) + i, N - 1)];
     f32x16 acc[TM][TN] = {};
-    constexpr int KS = SK / 16;
+    constexpr int SK = stage_k<TYPE>(), KS = 4;
     u32x4 a[2][TM], b[2][TN];
     const auto read_a = [&](int set, int i, int from, int ks) { a[set][i] = TileA::read(smem + from * STAGE, wm + 32 * i, ks); };
     const auto read_b = [&](int set, int i, int from, int ks) { b[set][i] = TileB::read(smem + from * STAGE + TileA::BYTES, wn + 32 * i, ks); };
@@ -383,7 +400,7 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_ker
     int buf = 0;
     for (int64_t k0 = ka; k0 < kb; k0 += SK, buf ^= 1) {
         // The loads of the stage after the next go out between the products of
-        // this stage's last 16 k (its second matrix, once the barrier has freed
+        // this stage's last quarter (its second matrix, once the barrier has freed
         // the buffer) and the next stage's first (its first matrix): a burst of them would hold up
         // the products behind it, and they have half a stage left to arrive in.
         // Past the end they write zeros, and the last reads take what nothing multiplies.
@@ -398,11 +415,12 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_ker
             for_const<TM>([&](auto ic) {
                 constexpr int i = ic.value;
                 if (ks == KS - 1) tb.template load<i * TileB::LOADS / TM, (i + 1) * TileB::LOADS / TM>(lds + buf * STAGE + TileA::BYTES, left_at(k0 + 2 * SK));
-                if (ks == 0) if (k0 > ka) ta.template load<i * TileA::LOADS / TM, (i + 1) * TileA::LOADS / TM>(lds + (buf ^ 1) * STAGE, left_at(k0 + SK));
-                if (i < TN) read_b(next, i, from, kn);
+                if (ks == 0 && k0 > ka) ta.template load<i * TileA::LOADS / TM, (i + 1) * TileA::LOADS / TM>(lds + (buf ^ 1) * STAGE, left_at(k0 + SK));
+#pragma unroll
+                for (int j = i * TN / TM; j < (i + 1) * TN / TM; j++) read_b(next, j, from, kn);
                 read_a(next, i, from, kn);
 #pragma unroll
-                for (int j = 0; j < TN; j++) acc[i][j] = mfma16<TYPE>(b[set][j], a[set][i], acc[i][j]);
+                for (int j = 0; j < TN; j++) acc[i][j] = multiply<TYPE>(b[set][j], a[set][i], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             });
         }
@@ -410,7 +428,7 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_ker
     wait_reads();
     wait_loads<0>();
     barrier();  // the stages' last loads and reads are done: the LDS is the epilogue's
-    constexpr int WR = BM / WM, G = 4;
+    constexpr int WR = BM / WM, G = sizeof(T) == 4 ? 2 : 4;
     float *out = (float *)smem + wave * WR * OUT_LD;
     const int row0 = lane >> 3, col = 8 * (lane & 7);
 #pragma unroll 1
@@ -502,7 +520,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
                     if (act) s[i] = (float)z[m * ldz + n + i];
                 }
         }
-        slope8(v, s, act);
+        slope8<T>(v, s, act);
         if (dz) {
             if (whole && N % 8 == 0) put8(dz + m * N + n, v);
             else
@@ -551,40 +569,61 @@ int dz_rows(int64_t M, int64_t N) {
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// How a product runs: its tile kernel and in how many parts k is split, where
-// the tiles alone leave most of the 256 CUs idle.  `fits`: both operands suit
-// the stage kernel.
+// How a product runs: its tile and in how many parts k is split.
 struct Plan {
-    int bm, bn;  // 64 x 64: tile_gemm_kernel
-    int splits;
-    int64_t per;  // k of a split
+    int tile = 64;      // rows and columns
+    bool stage = false; // stage_gemm_kernel; else tile_gemm_kernel, 64 x 64
+    int splits = 1;
+    int64_t per = 0;    // k of a split
 };
-Plan plan_for(bool fits, int64_t M, int64_t N, int64_t K) {
-    Plan p = {TB, TB, 1, 0};
-    if (fits) {
-        p.bm = p.bn = 256;
-        if (ceil_div<int64_t>(M, 256) * ceil_div<int64_t>(N, 256) < 192) p.bm = p.bn = 128;
+// The tile and split whose estimated time is least: rounds of workgroups over
+// the chip times (stages of k times a stage's time, and the time around them),
+// and where k is split the pass that joins the parts (written and read once).
+// A stage's time and the time around, in us, as measured on large products:
+// 256 x 256 tiles, one on a CU; 128 x 128, two; 64 x 64, four.
+Plan plan_for(int type, bool fits, int64_t M, int64_t N, int64_t K) {
+    Plan best;
+    best.per = ceil_div<int64_t>(std::max<int64_t>(K, 1), 64) * 64;
+    const struct { int tile, wgs; double stage, around; } forms[] = {
+        {256, 256, 1.7, 6}, {128, 512, 1.05, 4}, {64, 1024, 0.8, 3}};
+    double least = 1e30;
+    for (const auto &f : forms) {
+        if (fits ? type == BERT_AMD_F32 && f.tile == 256 : f.tile != 64) continue;
+        const double slower = type == BERT_AMD_F32 ? 4 : 1;  // f32 products run at an eighth of the rate, on half the k
+        const int64_t tiles = ceil_div<int64_t>(M, f.tile) * ceil_div<int64_t>(N, f.tile);
+        const int sk = type == BERT_AMD_F32 ? 32 : 64;
+        for (int splits = 1; splits <= 64; splits *= 2) {
+            if (splits > 1 && (K < splits * 4 * sk || tiles * splits > 2 * f.wgs)) break;
+            const int64_t per = std::max<int64_t>(64, ceil_div(ceil_div<int64_t>(K, splits), (int64_t)64) * 64);
+            const double join = splits > 1 ? 3 + 8e-6 / 4 * splits * M * N : 0;
+            const double t = ceil_div<int64_t>(tiles * splits, f.wgs) * (ceil_div<int64_t>(per, sk) * f.stage * slower + f.around) + join;
+            if (t < least) least = t, best.tile = f.tile, best.splits = splits, best.per = per;
+        }
     }
-    const int64_t tiles = ceil_div<int64_t>(M, p.bm) * ceil_div<int64_t>(N, p.bn);
-    if (tiles > 0 && tiles < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, K / 256));
-    p.per = ceil_div(ceil_div<int64_t>(K, p.splits), (int64_t)SK) * SK;
-    return p;
+    best.stage = fits;
+    best.splits = (int)std::max<int64_t>(1, ceil_div(K, best.per));  // rounding the parts up may leave the last ones empty
+    return best;
 }
-int64_t split_bytes(bool fits, int64_t M, int64_t N, int64_t K) {
-    const Plan p = plan_for(fits, M, N, K);
+int64_t split_bytes(int type, bool fits, int64_t M, int64_t N, int64_t K) {
+    const Plan p = plan_for(type, fits, M, N, K);
     return p.splits > 1 ? round256(p.splits * M * N * 4) : 0;
+}
+
+// split sums of a product, whatever its operands' alignment
+int64_t product_bytes(int type, int64_t M, int64_t N, int64_t K) {
+    return std::max(split_bytes(type, false, M, N, K), split_bytes(type, true, M, N, K));
 }
 
 // whether the stage kernel takes an operand: whole aligned chunks, and offsets within a tile under 2^31
 template <int TYPE>
 bool stage_operand(const Operand &o, bool trans, int64_t rows, int64_t k) {
-    return TYPE != BERT_AMD_F32 && o.vec && (trans ? rows : k) % 8 == 0 && o.ld < (1 << 22);
+    return o.vec && (trans ? rows : k) % Elem<TYPE>::CH == 0 && o.ld < (1 << 21);
 }
 
 template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
 void launch_stage(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, const Plan &p, float *part, const Epilogue &e,
                   bool vec, hipStream_t s) {
-    constexpr int lds = std::max(2 * (BM + BN) * SK * 2, BM * WN * OUT_LD * 4);
+    constexpr int lds = std::max(2 * (BM + BN) * 128, BM * WN * OUT_LD * 4);
     const auto k = stage_gemm_kernel<TYPE, TA, TBT, BM, BN, WM, WN>;
     (void)hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     const int64_t tiles = ceil_div<int64_t>(M, BM) * ceil_div<int64_t>(N, BN);
@@ -595,19 +634,19 @@ template <int TYPE, bool TA, bool TBT>
 hipError_t gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, void *ws, const Epilogue &e, hipStream_t s) {
     typedef typename Elem<TYPE>::T T;
     const bool fits = stage_operand<TYPE>(A, TA, M, K) && stage_operand<TYPE>(B, TBT, N, K);
-    const Plan p = plan_for(fits, M, N, K);
+    const Plan p = plan_for(TYPE, fits, M, N, K);
     float *part = p.splits > 1 ? (float *)ws : nullptr;
-    if constexpr (TYPE != BERT_AMD_F32) {
-        const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(T)); };
-        const bool vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr);
-        if (p.bn == 256)
-            launch_stage<TYPE, TA, TBT, 256, 256, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
-        else if (p.bn == 128)
-            launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
-    }
-    if (p.bn == TB) {
+    const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(T)); };
+    const bool vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr);
+    if (!p.stage) {
         const int64_t tiles = ceil_div<int64_t>(M, TB) * ceil_div<int64_t>(N, TB);
         hipLaunchKernelGGL((tile_gemm_kernel<TYPE, TA, TBT>), dim3(tiles, 1, p.splits), dim3(256), 0, s, A, B, M, N, K, p.per, part, e);
+    } else if (p.tile == 64) {
+        launch_stage<TYPE, TA, TBT, 64, 64, 2, 1>(A, B, M, N, K, p, part, e, vec, s);
+    } else if (p.tile == 128) {
+        launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
+    } else {
+        if constexpr (TYPE != BERT_AMD_F32) launch_stage<TYPE, TA, TBT, 256, 256, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
     }
     if (part)
         hipLaunchKernelGGL((split_join_kernel<T>), dim3(std::min<int64_t>(1024, ceil_div<int64_t>(M * N, 256))), dim3(256), 0, s, part, p.splits, M, N, e);
@@ -664,7 +703,7 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
 
 }  // namespace
 
-int64_t linear_ws_bytes(int, int64_t M, int N, int K) { return std::max(split_bytes(false, M, N, K), split_bytes(true, M, N, K)); }
+int64_t linear_ws_bytes(int type, int64_t M, int N, int K) { return product_bytes(type, M, N, K); }
 
 hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
     switch (a.type) {
@@ -676,8 +715,7 @@ hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
 
 int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K) {
     return (act ? round256(M * N * elem_size(type)) : 0) + round256(ceil_div<int64_t>(M, dz_rows(M, N)) * N * 4) +
-           std::max(std::max(split_bytes(false, M, K, N), split_bytes(true, M, K, N)),
-                    std::max(split_bytes(false, N, K, M), split_bytes(true, N, K, M)));
+           std::max(product_bytes(type, M, K, N), product_bytes(type, N, K, M));
 }
 
 hipError_t launch_linear_grad(const LinearGradArgs &a, hipStream_t s) {
