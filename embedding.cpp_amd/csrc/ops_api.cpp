@@ -60,7 +60,7 @@ const char *bad_matrix(const Matrix &m) {
 }
 
 constexpr int64_t MAX_M = ((int64_t)1 << 31) - 1;
-constexpr int32_t MAX_SIDE = (1 << 22) - 1, MAX_IDS = 1 << 30;
+constexpr int32_t MAX_SIDE = (1 << 22) - 1, MAX_IDS = 1 << 28, MAX_ROWS = 1 << 30;
 
 // the largest product's 64 x 64 tiles fit a launch (under 2^32 threads)
 constexpr int64_t MAX_AREA = (int64_t)1 << 34;
@@ -160,7 +160,7 @@ int32_t bert_amd_lookup(int32_t device, int32_t table_type, int32_t out_type, in
 }
 
 int64_t bert_amd_lookup_grad_workspace(int64_t n, int32_t n_rows, int32_t width) {
-    if (n < 0 || n > MAX_IDS || n_rows < 1 || n_rows > MAX_IDS || width < 1 || width > MAX_SIDE)
+    if (n < 0 || n > MAX_IDS || n_rows < 1 || n_rows > MAX_ROWS || width < 1 || width > MAX_SIDE)
         return refuse("bert_amd_lookup_grad_workspace: invalid size");
     return lookup_grad_ws_bytes(n, n_rows, width);
 }
@@ -169,7 +169,7 @@ int32_t bert_amd_lookup_grad(int32_t device, int32_t type, int64_t n, int32_t n_
                              const int32_t *ids, float scale, int32_t pad_id, int32_t accumulate, float *dtable, int64_t ldt,
                              void *workspace, int64_t workspace_bytes, void *hip_stream) {
     if (!is_float(type)) return refuse("bert_amd_lookup_grad: type %d is not supported", type);
-    if (n < 0 || n > MAX_IDS || n_rows < 1 || n_rows > MAX_IDS || width < 1 || width > MAX_SIDE)
+    if (n < 0 || n > MAX_IDS || n_rows < 1 || n_rows > MAX_ROWS || width < 1 || width > MAX_SIDE)
         return refuse("bert_amd_lookup_grad: invalid size (n %lld, n_rows %d, width %d)", (long long)n, n_rows, width);
     if (n > 0) {
         if (const char *bad = bad_matrix({"dout", dout, ldd, width, true, size_of(type)}))

@@ -23,6 +23,35 @@ inline bool aligned16(const void *p, int64_t stride_bytes) {
 template <typename T>
 constexpr T ceil_div(T a, T b) { return (a + b - 1) / b; }
 
+// 16 bytes of elements
+template <typename T, int CH>
+struct Chunk {
+    T v[CH];
+};
+
+// 8 elements in the type to or from an aligned row piece
+template <typename T>
+__device__ __forceinline__ void put8(T *p, const float *v) {
+    constexpr int CH = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += CH) {
+        Chunk<T, CH> o;
+#pragma unroll
+        for (int j = 0; j < CH; j++) o.v[j] = (T)v[i + j];
+        *(u32x4 *)(p + i) = __builtin_bit_cast(u32x4, o);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void add8(const T *p, float *v) {
+    constexpr int CH = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += CH) {
+        const auto o = __builtin_bit_cast(Chunk<T, CH>, *(const u32x4 *)(p + i));
+#pragma unroll
+        for (int j = 0; j < CH; j++) v[i + j] += (float)o.v[j];
+    }
+}
+
 // Activations and their slopes in f32.  gelu is the tanh form that the
 // encoder's feed-forward layer uses, written z * sigmoid(2u): no cancellation
 // in its lower tail.

@@ -60,11 +60,6 @@ __device__ __forceinline__ void epilogue_store(const Epilogue &e, int64_t m, int
     ((T *)e.y)[m * e.ldy + n] = (T)v;
 }
 
-template <typename T, int CH>
-struct Chunk {
-    T v[CH];
-};
-
 // CH elements of row r from column c of a [nr][nc] matrix
 template <typename T, int CH>
 __device__ __forceinline__ Chunk<T, CH> load_chunk(const T *p, int64_t ld, bool vec, int64_t r, int64_t c, int64_t nr, int64_t nc) {
@@ -305,29 +300,6 @@ __device__ __forceinline__ void act_n(float *v, int act) {
         case BERT_AMD_ACT_GELU_ERF: each(std::integral_constant<int, BERT_AMD_ACT_GELU_ERF>()); break;
         case BERT_AMD_ACT_SILU: each(std::integral_constant<int, BERT_AMD_ACT_SILU>()); break;
         case BERT_AMD_ACT_TANH: each(std::integral_constant<int, BERT_AMD_ACT_TANH>()); break;
-    }
-}
-
-// 8 elements in the type to or from an aligned row piece
-template <typename T>
-__device__ __forceinline__ void put8(T *p, const float *v) {
-    constexpr int CH = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8; i += CH) {
-        Chunk<T, CH> o;
-#pragma unroll
-        for (int j = 0; j < CH; j++) o.v[j] = (T)v[i + j];
-        *(u32x4 *)(p + i) = __builtin_bit_cast(u32x4, o);
-    }
-}
-template <typename T>
-__device__ __forceinline__ void add8(const T *p, float *v) {
-    constexpr int CH = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8; i += CH) {
-        const auto o = __builtin_bit_cast(Chunk<T, CH>, *(const u32x4 *)(p + i));
-#pragma unroll
-        for (int j = 0; j < CH; j++) v[i + j] += (float)o.v[j];
     }
 }
 

@@ -30,8 +30,39 @@ __device__ __forceinline__ float row_value(const char *row, int e) {
     }
 }
 
+// elements 8 c .. 8 c + 7 of a row whose float elements are 16-byte aligned (Q4 blocks: 2-byte)
+template <int TYPE>
+__device__ __forceinline__ void row_values8(const char *row, int c, float *v) {
+    if constexpr (RowType<TYPE>::BLOCKS) {
+        const char *b = row + (int64_t)(c >> 2) * RowType<TYPE>::SIZE;
+        const float d = (float)*(const _Float16 *)b;
+        const uint16_t *q = (const uint16_t *)(b + RowType<TYPE>::HEAD) + 4 * (c & 1);
+        const int shift = (c & 2) << 1;  // the block's second half is in the high nibbles
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const int two = q[i / 2] >> shift, lo = two & 15, hi = (two >> 8) & 15;
+            if constexpr (TYPE == BERT_AMD_Q4_0) {
+                v[i] = d * (float)(lo - 8), v[i + 1] = d * (float)(hi - 8);
+            } else {
+                const float m = (float)*(const _Float16 *)(b + 2);
+                v[i] = d * (float)lo + m, v[i + 1] = d * (float)hi + m;
+            }
+        }
+    } else {
+        typedef typename Elem<TYPE>::T T;
+        constexpr int CH = Elem<TYPE>::CH;
+#pragma unroll
+        for (int i = 0; i < 8; i += CH) {
+            const Chunk<T, CH> o = __builtin_bit_cast(Chunk<T, CH>, *(const u32x4 *)(row + (8 * c + i) * sizeof(T)));
+#pragma unroll
+            for (int j = 0; j < CH; j++) v[i + j] = (float)o.v[j];
+        }
+    }
+}
+
+// One thread an element: any width, stride and alignment.
 template <int TYPE, int OUT>
-__global__ __launch_bounds__(256) void lookup_kernel(LookupArgs a) {
+__global__ __launch_bounds__(256) void lookup_any_kernel(LookupArgs a) {
     const int64_t total = a.n * a.E;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / a.E;
@@ -41,26 +72,70 @@ __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs a) {
     }
 }
 
+// Eight elements a thread, `lanes` (8 .. 64) neighbours side by side on a row,
+// chosen so that they come out even: bound by memory, and enough rows are on
+// their way at once with no more than that.
+template <int TYPE, int OUT>
+__global__ __launch_bounds__(256) void lookup_kernel(LookupArgs a, int lanes_log2) {
+    const int lanes = 1 << lanes_log2, per = 256 >> lanes_log2, chunks = a.E / 8;
+    const int64_t row = (int64_t)blockIdx.x * per + (threadIdx.x >> lanes_log2);
+    if (row >= a.n) return;
+    const int id = a.ids[row];
+    const bool there = id >= 0 && id < a.V;
+    const char *from = (const char *)a.table + (there ? id : 0) * a.ld_bytes;
+    typename Elem<OUT>::T *to = (typename Elem<OUT>::T *)a.out + row * a.ldo;
+#pragma unroll 4
+    for (int c = threadIdx.x & (lanes - 1); c < chunks; c += lanes) {
+        float v[8] = {};
+        if (there) row_values8<TYPE>(from, c, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= there ? a.scale : 0.f;
+        if (!there)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = 0.f;
+        put8(to + 8 * c, v);
+    }
+}
+
+// lanes side by side on a row of `chunks`: the most, of those that leave the fewest without work
+int row_lanes_log2(int chunks) {
+    int best = 3;
+    for (int l = 3; l <= 6; l++)
+        if (ceil_div(chunks, 1 << l) << l <= ceil_div(chunks, 1 << best) << best) best = l;
+    return best;
+}
+
+template <int TYPE, int OUT>
+hipError_t lookup_tt(const LookupArgs &a, hipStream_t s) {
+    constexpr bool BLOCKS = RowType<TYPE>::BLOCKS;
+    const bool whole = a.E % 8 == 0 && (BLOCKS || aligned16(a.table, a.ld_bytes)) && aligned16(a.out, a.ldo * (int64_t)sizeof(typename Elem<OUT>::T));
+    const int l = row_lanes_log2(a.E / 8);
+    const int64_t groups = ceil_div<int64_t>(a.n, 256 >> l);
+    if (whole && groups <= 1 << 23)
+        hipLaunchKernelGGL((lookup_kernel<TYPE, OUT>), dim3(groups), dim3(256), 0, s, a, l);
+    else
+        hipLaunchKernelGGL((lookup_any_kernel<TYPE, OUT>), dim3(std::min<int64_t>(1 << 20, ceil_div<int64_t>(a.n * a.E, 256))), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
 template <int TYPE>
 hipError_t lookup_t(const LookupArgs &a, hipStream_t s) {
-    const dim3 grid(std::min<int64_t>(1 << 20, ceil_div<int64_t>(a.n * a.E, 256)));
     switch (a.out_type) {
-        case BERT_AMD_F32: hipLaunchKernelGGL((lookup_kernel<TYPE, BERT_AMD_F32>), grid, dim3(256), 0, s, a); break;
-        case BERT_AMD_F16: hipLaunchKernelGGL((lookup_kernel<TYPE, BERT_AMD_F16>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((lookup_kernel<TYPE, BERT_AMD_BF16>), grid, dim3(256), 0, s, a); break;
+        case BERT_AMD_F32: return lookup_tt<TYPE, BERT_AMD_F32>(a, s);
+        case BERT_AMD_F16: return lookup_tt<TYPE, BERT_AMD_F16>(a, s);
+        default: return lookup_tt<TYPE, BERT_AMD_BF16>(a, s);
     }
-    return hipGetLastError();
 }
 
 // ---- the places sorted by token --------------------------------------------
 //
 // A stable radix sort of (token, place) by digits of up to 9 bits: per digit a
-// histogram of each tile of 2048 places, each digit value's exclusive scan
+// histogram of each tile of 1024 places, each digit value's exclusive scan
 // over the tiles, and a scatter in which every place's rank counts the places
 // before it in its tile with the same digit.  No atomic's order enters the
 // result, so the sums below have one order.  Places without a gradient (ids
 // outside the table, the padding token) get the key V and sort last.
-constexpr int TILE = 2048, BINS = 512;
+constexpr int TILE = 1024, BINS = 512;
 
 __device__ __forceinline__ int sort_key(int id, int V, int pad) { return id >= 0 && id < V && id != pad ? id : V; }
 
@@ -69,11 +144,16 @@ struct SortPass {
     const int32_t *key_in, *place_in;
     int32_t *key_out, *place_out;
     int32_t *hist, *total;             // [BINS][tiles], [BINS]
+    uint8_t *used;                     // first pass: cleared; last: set for each token that has a place
+    bool last;
     int n, V, pad, tiles, shift, bits;
 };
 
 __global__ __launch_bounds__(256) void sort_hist_kernel(SortPass p) {
     __shared__ int h[BINS];
+    if (p.ids)
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < ceil_div(p.V, 16); i += (int64_t)gridDim.x * 256)
+            ((u32x4 *)p.used)[i] = u32x4{0, 0, 0, 0};
     for (int i = threadIdx.x; i < BINS; i += 256) h[i] = 0;
     __syncthreads();
     const int mask = (1 << p.bits) - 1, base = blockIdx.x * TILE;
@@ -161,31 +241,224 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortPass p) {
         for (int w = 0; w < wave; w++) at += seen[w][d];
         p.key_out[at] = key[j];
         p.place_out[at] = place[j];
+        if (p.last && key[j] < p.V) p.used[key[j]] = 1;
     }
 }
 
-__global__ __launch_bounds__(256) void fill_kernel(int32_t *p, int64_t n, int32_t v) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = v;
+// ---- the sums ---------------------------------------------------------------
+//
+// A workgroup sums SUM_TILE sorted places, a thread COLS columns of them in
+// order, eight rows' loads on their way at a time, and writes the row of each
+// token whose places end within the tile.  A token whose places go on past a
+// tile's end leaves its sums, one row for each tile it has places in, to
+// join_kernel, which adds them in order: a frequent token's long sum is spread
+// over many workgroups.  The same launch's other workgroups write zeros into
+// the rows of tokens that have no place (bound by memory: most of a table's
+// gradient is that).
+constexpr int SUM_TILE = 64, ZERO_ROWS = 64, AHEAD = 8;
+
+template <typename T, int COLS>
+__device__ __forceinline__ void load_cols(const T *p, float *v) {
+    if constexpr (COLS == 1) {
+        v[0] = (float)p[0];
+    } else {
+        struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; };
+        const Four f = *(const Four *)p;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (float)f.v[i];
+    }
+}
+template <int COLS>
+__device__ __forceinline__ void store_cols(float *p, const float *v) {
+    if constexpr (COLS == 1) p[0] = v[0];
+    else *(f32x4 *)p = f32x4{v[0], v[1], v[2], v[3]};
+}
+// a finished sum into its row of the table
+template <int COLS>
+__device__ __forceinline__ void store_row(const LookupGradArgs &a, int v, int e, const float *sum) {
+    float *p = a.dtable + (int64_t)v * a.ldt + e, o[COLS];
+    if (a.accumulate) load_cols<float, COLS>(p, o);
+#pragma unroll
+    for (int i = 0; i < COLS; i++) o[i] = a.accumulate ? o[i] + a.scale * sum[i] : a.scale * sum[i];
+    store_cols<COLS>(p, o);
+}
+template <int COLS>
+__device__ __forceinline__ void zero_rows(const LookupGradArgs &a, int first, const uint8_t *used /* of row `first` on */) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int v = first + wave; v < min(a.V, first + ZERO_ROWS); v += blockDim.x >> 6) {
+        if (used[v - first]) continue;
+        const float zero[4] = {};
+        for (int e = COLS * lane; e < a.E; e += 64 * COLS) store_cols<COLS>(a.dtable + (int64_t)v * a.ldt + e, zero);
+    }
 }
 
-__global__ __launch_bounds__(256) void starts_kernel(const int32_t *key, int n, int V, int32_t *start) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n && key[i] < V && (i == 0 || key[i - 1] != key[i])) start[key[i]] = i;
-}
+struct SumArgs {
+    const int32_t *key, *place;
+    const uint8_t *used;
+    float *part;  // [tiles][2][E]: of the token that goes on from the tile before; of the one that goes on past the end
+    int tiles;
+};
 
-template <int TYPE>
-__global__ __launch_bounds__(256) void lookup_grad_kernel(LookupGradArgs a, const int32_t *key, const int32_t *place, const int32_t *start) {
-    for (int v = blockIdx.x; v < a.V; v += gridDim.x) {
-        const int first = start[v];
-        if (first < 0 && a.accumulate) continue;
-        for (int e = threadIdx.x; e < a.E; e += 256) {
-            float sum = 0.f;
-            if (first >= 0)
-                for (int i = first; i < a.n && key[i] == v; i++)
-                    sum += (float)((const typename Elem<TYPE>::T *)a.dout)[place[i] * a.ldd + e];
-            float *o = a.dtable + (int64_t)v * a.ldt + e;
-            *o = a.accumulate ? *o + a.scale * sum : a.scale * sum;
+template <int TYPE, int COLS>
+__global__ __launch_bounds__(256) void sum_kernel(LookupGradArgs a, SumArgs s) {
+    typedef typename Elem<TYPE>::T T;
+    if ((int)blockIdx.x >= s.tiles) {
+        if (blockIdx.y == 0)
+            for (int64_t b = blockIdx.x - s.tiles; b * ZERO_ROWS < a.V; b += gridDim.x - s.tiles) zero_rows<COLS>(a, (int)b * ZERO_ROWS, s.used + b * ZERO_ROWS);
+        return;
+    }
+    __shared__ int key[SUM_TILE + 2], place[SUM_TILE];
+    const int n = (int)a.n, first = blockIdx.x * SUM_TILE, count = min(SUM_TILE, n - first);
+    for (int i = threadIdx.x; i < count; i += blockDim.x) key[i + 1] = s.key[first + i], place[i] = s.place[first + i];
+    if (threadIdx.x == 0) {
+        key[0] = first ? s.key[first - 1] : -1;
+        key[count + 1] = first + count < n ? s.key[first + count] : a.V;
+    }
+    __syncthreads();
+    const int e = (blockIdx.y * blockDim.x + threadIdx.x) * COLS;
+    if (e >= a.E) return;
+    const T *from = (const T *)a.dout + e;
+    float sum[COLS] = {};
+    bool from_before = key[0] == key[1];
+    for (int i = 0; i < count; i += AHEAD) {
+        if (key[i + 1] >= a.V) break;  // the places without a gradient are the last ones
+        float v[AHEAD][COLS] = {};
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++)
+            if (i + j < count && key[i + j + 1] < a.V) load_cols<T, COLS>(from + (int64_t)place[i + j] * a.ldd, v[j]);
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const int k = i + j < count ? key[i + j + 1] : a.V;
+            if (k >= a.V) break;
+#pragma unroll
+            for (int c = 0; c < COLS; c++) sum[c] += v[j][c];
+            if (i + j == count - 1 || key[i + j + 2] != k) {
+                const bool goes_on = key[i + j + 2] == k;
+                if (from_before) store_cols<COLS>(s.part + ((int64_t)blockIdx.x * 2) * a.E + e, sum);
+                else if (goes_on) store_cols<COLS>(s.part + ((int64_t)blockIdx.x * 2 + 1) * a.E + e, sum);
+                else store_row<COLS>(a, k, e, sum);
+                from_before = false;
+#pragma unroll
+                for (int c = 0; c < COLS; c++) sum[c] = 0.f;
+            }
         }
+    }
+}
+
+// The token that starts in this tile and goes on past its end: its sums of this
+// tile and the following ones, 64 columns' threads in four groups that take a
+// quarter of the tiles each.
+template <int COLS>
+__global__ __launch_bounds__(256) void join_kernel(LookupGradArgs a, SumArgs s) {
+    const int t = blockIdx.x, last = (t + 1) * SUM_TILE - 1, n = (int)a.n;
+    if (last + 1 >= n) return;
+    const int k = s.key[last];
+    if (k >= a.V || s.key[last + 1] != k) return;
+    if (s.key[t * SUM_TILE] == k && t > 0 && s.key[t * SUM_TILE - 1] == k) return;  // it started before this tile
+    int lo = t + 1, hi = s.tiles;  // the tiles after this one that begin with k end at lo
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s.key[mid * SUM_TILE] == k) lo = mid + 1;
+        else hi = mid;
+    }
+    __shared__ float sums[4][64][COLS + 1];
+    const int c = threadIdx.x & 63, g = threadIdx.x >> 6, e = (blockIdx.y * 64 + c) * COLS;
+    const int rows = lo - t - 1, per = ceil_div(rows, 4);
+    float sum[COLS] = {};
+    if (e < a.E) {
+        const float *head = s.part + (int64_t)(t + 1) * 2 * a.E + e;
+#pragma unroll 8
+        for (int i = g * per; i < min(rows, (g + 1) * per); i++) {
+            float v[COLS];
+            load_cols<float, COLS>(head + (int64_t)i * 2 * a.E, v);
+#pragma unroll
+            for (int j = 0; j < COLS; j++) sum[j] += v[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < COLS; j++) sums[g][c][j] = sum[j];
+    __syncthreads();
+    if (g || e >= a.E) return;
+    float v[COLS];
+    load_cols<float, COLS>(s.part + ((int64_t)t * 2 + 1) * a.E + e, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < COLS; j++) v[j] += sums[i][c][j];
+    store_row<COLS>(a, k, e, v);
+}
+
+// Few places (at most FEW): no sort.  A workgroup for each place looks through
+// all ids; only a token's first place goes on, its four waves each sum the
+// token's places of a quarter of the ids, in order, and the quarters are added
+// in order.  Again the other workgroups write the zeros, and find out from the
+// ids which rows are in use.
+constexpr int FEW = 4096;
+
+template <int TYPE, int COLS>
+__global__ __launch_bounds__(256) void few_kernel(LookupGradArgs a) {
+    typedef typename Elem<TYPE>::T T;
+    const int n = (int)a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if ((int)blockIdx.x >= n) {
+        __shared__ uint8_t used[256];
+        static_assert(ZERO_ROWS <= 256, "one thread clears one row's mark");
+        for (int64_t b = blockIdx.x - n; b * ZERO_ROWS < a.V; b += gridDim.x - n) {
+            const int first = (int)b * ZERO_ROWS;
+            __syncthreads();
+            used[threadIdx.x] = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += 256) {
+                const int id = a.ids[i];
+                if (id >= first && id < first + ZERO_ROWS && id != a.pad_id) used[id - first] = 1;
+            }
+            __syncthreads();
+            zero_rows<COLS>(a, first, used);
+        }
+        return;
+    }
+    const int k = sort_key(a.ids[blockIdx.x], a.V, a.pad_id);
+    if (k == a.V) return;
+    __shared__ uint16_t list[4][FEW / 4];
+    __shared__ int before[4];
+    __shared__ float sums[3][64][COLS + 1];
+    const int quarter = ceil_div(n, 256) * 64, from = wave * quarter;
+    int count = 0, earlier = 0;
+    for (int i = from; i < min(n, from + quarter); i += 64) {
+        const bool same = i + lane < n && a.ids[i + lane] == k;
+        const uint64_t mask = __ballot(same);
+        if (same) list[wave][count + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(i + lane);
+        if (mask && i + __ffsll((unsigned long long)mask) - 1 < (int)blockIdx.x) earlier = 1;
+        count += __popcll(mask);
+    }
+    before[wave] = earlier;
+    __syncthreads();
+    if (before[0] | before[1] | before[2] | before[3]) return;
+    for (int e0 = 0; e0 < a.E; e0 += 64 * COLS) {
+        const int e = e0 + lane * COLS;
+        float sum[COLS] = {};
+        if (e < a.E)
+            for (int i = 0; i < count; i += AHEAD) {
+                float v[AHEAD][COLS] = {};
+#pragma unroll
+                for (int j = 0; j < AHEAD; j++)
+                    if (i + j < count) load_cols<T, COLS>((const T *)a.dout + list[wave][i + j] * a.ldd + e, v[j]);
+#pragma unroll
+                for (int j = 0; j < AHEAD; j++)
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) sum[c] += v[j][c];
+            }
+        if (wave)
+#pragma unroll
+            for (int c = 0; c < COLS; c++) sums[wave - 1][lane][c] = sum[c];
+        __syncthreads();
+        if (!wave && e < a.E) {
+#pragma unroll
+            for (int w = 0; w < 3; w++)
+#pragma unroll
+                for (int c = 0; c < COLS; c++) sum[c] += sums[w][lane][c];
+            store_row<COLS>(a, k, e, sum);
+        }
+        __syncthreads();
     }
 }
 
@@ -203,52 +476,91 @@ hipError_t launch_lookup(const LookupArgs &a, hipStream_t s) {
     }
 }
 
-int64_t lookup_grad_ws_bytes(int64_t n, int V, int) {
-    const int64_t tiles = ceil_div<int64_t>(n, TILE);
-    return 4 * round256(n * 4) + round256(BINS * tiles * 4) + round256(BINS * 4) + round256((int64_t)V * 4);
+int64_t lookup_grad_ws_bytes(int64_t n, int V, int E) {
+    if (n <= FEW) return 0;
+    return 4 * round256(n * 4) + round256(BINS * ceil_div<int64_t>(n, TILE) * 4) + round256(BINS * 4) + round256((int64_t)V + 16) +
+           round256(ceil_div<int64_t>(n, SUM_TILE) * 2 * E * 4);
 }
 
+namespace {
+
+// workgroups beside the sums' that write zeros: all of a large table's rows at once, as far as a launch goes
+int zero_groups(const LookupGradArgs &a) {
+    return a.accumulate ? 0 : (int)std::min<int64_t>(1 << 20, ceil_div(a.V, ZERO_ROWS));
+}
+
+template <int TYPE, int COLS>
+hipError_t sum_t(const LookupGradArgs &a, const SumArgs &p, hipStream_t s) {
+    const int threads = std::min(256, ceil_div(ceil_div(a.E, COLS), 64) * 64);
+    const int across = ceil_div(ceil_div(a.E, COLS), threads);
+    hipLaunchKernelGGL((sum_kernel<TYPE, COLS>), dim3(p.tiles + zero_groups(a), across), dim3(threads), 0, s, a, p);
+    hipLaunchKernelGGL((join_kernel<COLS>), dim3(p.tiles, ceil_div(a.E, 64 * COLS)), dim3(256), 0, s, a, p);
+    return hipGetLastError();
+}
+template <int TYPE, int COLS>
+hipError_t few_t(const LookupGradArgs &a, hipStream_t s) {
+    const int groups = (int)a.n + zero_groups(a);
+    if (groups) hipLaunchKernelGGL((few_kernel<TYPE, COLS>), dim3(groups), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+// four columns a thread where rows and places allow it
+bool four_columns(const LookupGradArgs &a) {
+    const int64_t e = elem_size(a.type);
+    return a.E % 4 == 0 && a.ldd % 4 == 0 && ((uintptr_t)a.dout & (4 * e - 1)) == 0 && aligned16(a.dtable, a.ldt * 4);
+}
+
+}  // namespace
+
 hipError_t launch_lookup_grad(const LookupGradArgs &a, hipStream_t s) {
+    const bool four = four_columns(a);
+    if (a.n <= FEW) {
+        switch (a.type) {
+            case BERT_AMD_F32: return four ? few_t<BERT_AMD_F32, 4>(a, s) : few_t<BERT_AMD_F32, 1>(a, s);
+            case BERT_AMD_F16: return four ? few_t<BERT_AMD_F16, 4>(a, s) : few_t<BERT_AMD_F16, 1>(a, s);
+            default: return four ? few_t<BERT_AMD_BF16, 4>(a, s) : few_t<BERT_AMD_BF16, 1>(a, s);
+        }
+    }
     char *ws = (char *)a.ws;
-    const auto take = [&](int64_t ints) {
-        int32_t *p = (int32_t *)ws;
-        ws += round256(ints * 4);
+    const auto take = [&](int64_t bytes) {
+        char *p = ws;
+        ws += round256(bytes);
         return p;
     };
     const int tiles = (int)ceil_div<int64_t>(a.n, TILE);
     int32_t *key[2], *place[2];
-    for (int i = 0; i < 2; i++) key[i] = take(a.n), place[i] = take(a.n);
+    for (int i = 0; i < 2; i++) key[i] = (int32_t *)take(a.n * 4), place[i] = (int32_t *)take(a.n * 4);
     SortPass p = {};
-    p.hist = take((int64_t)BINS * tiles);
-    p.total = take(BINS);
-    int32_t *start = take(a.V);
-    hipLaunchKernelGGL(fill_kernel, dim3(std::min<int64_t>(1024, ceil_div(a.V, 256))), dim3(256), 0, s, start, (int64_t)a.V, -1);
+    p.hist = (int32_t *)take((int64_t)BINS * tiles * 4);
+    p.total = (int32_t *)take(BINS * 4);
+    p.used = (uint8_t *)take((int64_t)a.V + 16);
+    SumArgs q = {};
+    q.used = p.used;
+    q.part = (float *)take(ceil_div<int64_t>(a.n, SUM_TILE) * 2 * a.E * 4);
+    q.tiles = (int)ceil_div<int64_t>(a.n, SUM_TILE);
+    int key_bits = 1;
+    while ((int64_t)a.V >> key_bits) key_bits++;
+    const int passes = ceil_div(key_bits, 9);
+    p.n = (int)a.n, p.V = a.V, p.pad = a.pad_id, p.tiles = tiles;
+    p.bits = ceil_div(key_bits, passes);
     int at = 0;
-    if (a.n) {
-        int key_bits = 1;
-        while ((int64_t)a.V >> key_bits) key_bits++;
-        const int passes = ceil_div(key_bits, 9);
-        p.n = (int)a.n, p.V = a.V, p.pad = a.pad_id, p.tiles = tiles;
-        p.bits = ceil_div(key_bits, passes);
-        for (int i = 0; i < passes; i++) {
-            p.ids = i ? nullptr : a.ids;
-            p.key_in = key[at], p.place_in = place[at];
-            p.key_out = key[at ^ 1], p.place_out = place[at ^ 1];
-            p.shift = i * p.bits;
-            hipLaunchKernelGGL(sort_hist_kernel, dim3(tiles), dim3(256), 0, s, p);
-            hipLaunchKernelGGL(sort_scan_kernel, dim3(1 << p.bits), dim3(256), 0, s, p);
-            hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles), dim3(256), 0, s, p);
-            at ^= 1;
-        }
-        hipLaunchKernelGGL(starts_kernel, dim3(ceil_div<int64_t>(a.n, 256)), dim3(256), 0, s, key[at], (int)a.n, a.V, start);
+    for (int i = 0; i < passes; i++) {
+        p.ids = i ? nullptr : a.ids;
+        p.key_in = key[at], p.place_in = place[at];
+        p.key_out = key[at ^ 1], p.place_out = place[at ^ 1];
+        p.shift = i * p.bits;
+        p.last = i == passes - 1;
+        hipLaunchKernelGGL(sort_hist_kernel, dim3(tiles), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(sort_scan_kernel, dim3(1 << p.bits), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles), dim3(256), 0, s, p);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        at ^= 1;
     }
-    const int rows = std::min(a.V, 1 << 22);
+    q.key = key[at], q.place = place[at];
     switch (a.type) {
-        case BERT_AMD_F32: hipLaunchKernelGGL((lookup_grad_kernel<BERT_AMD_F32>), dim3(rows), dim3(256), 0, s, a, key[at], place[at], start); break;
-        case BERT_AMD_F16: hipLaunchKernelGGL((lookup_grad_kernel<BERT_AMD_F16>), dim3(rows), dim3(256), 0, s, a, key[at], place[at], start); break;
-        default: hipLaunchKernelGGL((lookup_grad_kernel<BERT_AMD_BF16>), dim3(rows), dim3(256), 0, s, a, key[at], place[at], start); break;
+        case BERT_AMD_F32: return four ? sum_t<BERT_AMD_F32, 4>(a, q, s) : sum_t<BERT_AMD_F32, 1>(a, q, s);
+        case BERT_AMD_F16: return four ? sum_t<BERT_AMD_F16, 4>(a, q, s) : sum_t<BERT_AMD_F16, 1>(a, q, s);
+        default: return four ? sum_t<BERT_AMD_BF16, 4>(a, q, s) : sum_t<BERT_AMD_BF16, 1>(a, q, s);
     }
-    return hipGetLastError();
 }
 
 }  // namespace bertamd

@@ -261,7 +261,7 @@ BERT_API int32_t bert_amd_lookup(int32_t device, int32_t table_type, int32_t out
    as zero.  accumulate != 0 adds it to dtable instead and leaves unused rows
    untouched.  Ids outside [0, n_rows) and pad_id (-1: none) have no gradient.
      dout     : [n][width] of type F32, F16 or BF16; dtable: f32 [n_rows][width]
-   n <= 2^30, n_rows <= 2^30. */
+   n <= 2^28, n_rows <= 2^30. */
 BERT_API int64_t bert_amd_lookup_grad_workspace(int64_t n, int32_t n_rows, int32_t width);
 BERT_API int32_t bert_amd_lookup_grad(int32_t device, int32_t type, int64_t n, int32_t n_rows, int32_t width,
                                       const void *dout, int64_t ldd, const int32_t *ids, float scale, int32_t pad_id,

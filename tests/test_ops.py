@@ -306,7 +306,7 @@ def check_grad(got, dout, ids, V, scale, pad, base=None):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,V,E,pad_ld", [(0, 5, 8, 0), (1, 1, 1, 0), (1, 30522, 384, 0), (7, 3, 33, 3), (64, 10, 384, 0), (1000, 100, 130, 8), (2048, 30522, 64, 0), (2049, 517, 96, 0), (5000, 2, 40, 0), (40000, 70000, 32, 0), (9000, 1, 300, 1), (30000, 900, 768, 0)])
+@pytest.mark.parametrize("n,V,E,pad_ld", [(0, 5, 8, 0), (1, 1, 1, 0), (1, 30522, 384, 0), (7, 3, 33, 3), (64, 10, 384, 0), (1000, 100, 130, 8), (2048, 30522, 64, 0), (4095, 517, 96, 0), (4096, 60, 30, 0), (4097, 511, 130, 0), (5000, 2, 40, 0), (40000, 70000, 32, 0), (66000, 300000, 20, 0), (9000, 1, 300, 1), (30000, 900, 768, 0)])
 def test_lookup_grad(n, V, E, pad_ld, dtype):
     g = gen(9)
     dout = normal(g, n, E).to(DTYPES[dtype])
@@ -677,7 +677,7 @@ def test_refusals_of_the_library():
     assert L.bert_amd_lookup(*{**ok, "n": 0, "ids": NULL}.values()) == 0
 
     ok = dict(device=0, type=0, n=4, V=10, E=8, dout=P, ldd=8, ids=P, scale=1.0, pad=-1, acc=0, dt=P, ldt=8, ws=P, nws=big, s=NULL)
-    for change, word in ((dict(type=2), "type"), (dict(n=-1), "size"), (dict(n=(1 << 30) + 1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(dout=NULL), "dout"), (dict(ldd=7), "dout"), (dict(ids=NULL), "ids"), (dict(dt=NULL), "dtable"), (dict(ldt=7), "dtable"), (dict(ws=NULL), "workspace"), (dict(nws=16), "workspace")):
+    for change, word in ((dict(type=2), "type"), (dict(n=-1), "size"), (dict(n=(1 << 28) + 1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(dout=NULL), "dout"), (dict(ldd=7), "dout"), (dict(ids=NULL), "ids"), (dict(dt=NULL), "dtable"), (dict(ldt=7), "dtable"), (dict(n=5000, ws=NULL), "workspace"), (dict(n=5000, nws=16), "workspace"), (dict(n=5000, ws=P + 8), "workspace")):
         refused(L.bert_amd_lookup_grad(*{**ok, **change}.values()), word)
     assert L.bert_amd_lookup_grad_workspace(-1, 10, 8) == -1
 
@@ -719,7 +719,7 @@ def test_workspace_sizes():
                 assert L.bert_amd_linear_workspace(t, M, N, K) >= 0
                 for act in (0, 2):
                     assert L.bert_amd_linear_backward_workspace(t, act, M, N, K) >= (M * N * (4 if t == 0 else 2) if act else 0)
-    for n in (0, 1, 2048, 2049, 1 << 30):
+    for n in (0, 1, 4096, 4097, 1 << 28):
         for V in (1, 511, 512, 1 << 30):
             assert L.bert_amd_lookup_grad_workspace(n, V, 8) >= 0
 
