@@ -43,7 +43,8 @@ struct Tensor {
     int64_t n;
     float keep;         // 1 - lr decay
     uint32_t key;       // the seed and the tensor's number, mixed
-    int64_t first;      // first chunk of this tensor in the launch
+    int32_t first;      // first chunk of this tensor in the launch
+    int32_t vec;        // every pointer is aligned to four of its elements
 };
 struct Table {
     Tensor t[TENSORS];
@@ -89,6 +90,22 @@ __device__ __forceinline__ void block_scale(uint32_t peak, float top, float &sca
     inv = scale > 0.f && peak < 0x7f800000u ? 1.f / scale : 0.f;
 }
 
+// four elements at p, aligned to as many bytes as they take
+template <typename T, typename V>
+__device__ __forceinline__ void get4(const T *p, V *v) {
+    struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; };
+    const Four f = *(const Four *)p;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = (V)f.v[j];
+}
+template <typename T, typename V>
+__device__ __forceinline__ void put4(T *p, const V *v) {
+    struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; } f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) f.v[j] = (T)v[j];
+    *(Four *)p = f;
+}
+
 struct Moments {
     float m, v, r;
 };
@@ -107,45 +124,56 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table a) {
     int lo = 0, hi = a.count - 1;
     while (lo < hi) {  // the tensor of this chunk
         const int mid = (lo + hi + 1) >> 1;
-        if (a.t[mid].first <= (int64_t)blockIdx.x) lo = mid;
+        if (a.t[mid].first <= (int)blockIdx.x) lo = mid;
         else hi = mid - 1;
     }
     const Tensor &t = a.t[lo];
     const float gs = a.grad_scale ? *a.grad_scale : 1.f;
-    const int64_t start = ((int64_t)blockIdx.x - t.first) * CHUNK;
+    const int64_t start = (int64_t)((int)blockIdx.x - t.first) * CHUNK;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int64_t b = start + wave * STATE_BLOCK; b < min(t.n, start + CHUNK); b += 4 * STATE_BLOCK) {
-        float mn[4], rn[4];
+        const int64_t i = b + 4 * lane;
+        const int count = (int)min((int64_t)4, t.n - i);  // this lane's elements; none past the end
+        const bool whole = t.vec && count == 4;
+        float p[4] = {}, g[4] = {}, m[4] = {}, v[4] = {}, r[4] = {};
+        uint32_t cm[4] = {}, cv[4] = {};
         float ms = 0.f, vs = 0.f;
         if constexpr (BITS == 8) ms = t.ms[b / STATE_BLOCK], vs = t.vs[b / STATE_BLOCK];
+        if (whole) {
+            get4(t.p + i, p);
+            get4((const G *)t.g + i, g);
+            if constexpr (BITS == 8) {
+                get4((const uint8_t *)t.m + i, cm);
+                get4((const uint8_t *)t.v + i, cv);
+            } else {
+                get4((const float *)t.m + i, m);
+                get4((const float *)t.v + i, v);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j >= count) continue;
+                p[j] = t.p[i + j];
+                g[j] = (float)((const G *)t.g)[i + j];
+                if constexpr (BITS == 8) cm[j] = ((const uint8_t *)t.m)[i + j], cv[j] = ((const uint8_t *)t.v)[i + j];
+                else m[j] = ((const float *)t.m)[i + j], v[j] = ((const float *)t.v)[i + j];
+            }
+        }
         uint32_t mpeak = 0, rpeak = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int64_t i = b + 4 * lane + j;
-            mn[j] = rn[j] = 0.f;
-            if (i >= t.n) continue;
-            float g = (float)((const G *)t.g)[i];
-            if (a.grad_scale) g *= gs;
-            float m, v, p = t.p[i];
             if constexpr (BITS == 8) {
-                const uint32_t cm = ((const uint8_t *)t.m)[i], cv = ((const uint8_t *)t.v)[i];
-                m = code_value<3>(cm & 127u) * ms;
-                m = cm & 128u ? -m : m;
-                const float r = code_value<4>(cv) * vs;
-                v = r * r;
-            } else {
-                m = ((const float *)t.m)[i], v = ((const float *)t.v)[i];
+                m[j] = code_value<3>(cm[j] & 127u) * ms;
+                m[j] = cm[j] & 128u ? -m[j] : m[j];
+                const float old = code_value<4>(cv[j]) * vs;
+                v[j] = old * old;
             }
-            const Moments o = step_one(a, t.keep, g, p, m, v);
-            t.p[i] = p;
-            if (t.copy) ((C *)t.copy)[i] = (C)p;
-            if constexpr (BITS == 8) {
-                mn[j] = o.m, rn[j] = o.r;
+            if (a.grad_scale) g[j] *= gs;
+            const Moments o = step_one(a, t.keep, g[j], p[j], m[j], v[j]);
+            m[j] = o.m, v[j] = o.v, r[j] = o.r;
+            if (BITS == 8 && j < count) {
                 mpeak = max(mpeak, __float_as_uint(o.m) & 0x7fffffffu);
                 rpeak = max(rpeak, __float_as_uint(o.r) & 0x7fffffffu);
-            } else {
-                ((float *)t.m)[i] = o.m;
-                ((float *)t.v)[i] = o.v;
             }
         }
         if constexpr (BITS == 8) {
@@ -155,31 +183,64 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table a) {
             if (lane == 0) t.ms[b / STATE_BLOCK] = ms, t.vs[b / STATE_BLOCK] = vs;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int64_t i = b + 4 * lane + j;
-                if (i >= t.n) continue;
-                const uint32_t h = mix((uint32_t)i ^ t.key ^ ((uint32_t)(i >> 32) * 0x9E3779B9u));
-                uint32_t cm = 0, cv = 0;
-                if (minv > 0.f) cm = code_of<3>(fabsf(mn[j]) * minv, h) | (mn[j] < 0.f ? 128u : 0u);
-                if (rinv > 0.f) cv = code_of<4>(rn[j] * rinv, mix(h ^ 0x9E3779B9u));
-                if (cv == 0 && rinv > 0.f && rn[j] > 0.f) cv = 1;
-                ((uint8_t *)t.m)[i] = (uint8_t)cm;
-                ((uint8_t *)t.v)[i] = (uint8_t)cv;
+                const uint32_t h = mix((uint32_t)(i + j) ^ t.key ^ ((uint32_t)((i + j) >> 32) * 0x9E3779B9u));
+                cm[j] = minv > 0.f ? code_of<3>(fabsf(m[j]) * minv, h) | (m[j] < 0.f ? 128u : 0u) : 0u;
+                cv[j] = rinv > 0.f ? code_of<4>(r[j] * rinv, mix(h ^ 0x9E3779B9u)) : 0u;
+                if (cv[j] == 0 && rinv > 0.f && r[j] > 0.f) cv[j] = 1;
+            }
+        }
+        if (whole) {
+            put4(t.p + i, p);
+            if (t.copy) put4((C *)t.copy + i, p);
+            if constexpr (BITS == 8) {
+                put4((uint8_t *)t.m + i, cm);
+                put4((uint8_t *)t.v + i, cv);
+            } else {
+                put4((float *)t.m + i, m);
+                put4((float *)t.v + i, v);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j >= count) continue;
+                t.p[i + j] = p[j];
+                if (t.copy) ((C *)t.copy)[i + j] = (C)p[j];
+                if constexpr (BITS == 8) ((uint8_t *)t.m)[i + j] = (uint8_t)cm[j], ((uint8_t *)t.v)[i + j] = (uint8_t)cv[j];
+                else ((float *)t.m)[i + j] = m[j], ((float *)t.v)[i + j] = v[j];
             }
         }
     }
 }
 
+// 8-bit moments as values, four of an element's place a thread
 __global__ __launch_bounds__(256) void moments_kernel(int64_t n, const uint8_t *m, const float *ms, const uint8_t *v, const float *vs,
-                                                      float *m_out, float *v_out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+                                                      float *m_out, float *v_out, bool vec) {
+    for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n; i += (int64_t)gridDim.x * 1024) {
+        const int count = (int)min((int64_t)4, n - i);
         if (m_out) {
-            const uint32_t c = m[i];
-            const float x = code_value<3>(c & 127u) * ms[i / STATE_BLOCK];
-            m_out[i] = c & 128u ? -x : x;
+            uint32_t c[4] = {};
+            float x[4];
+            if (vec && count == 4) get4(m + i, c);
+            else for (int j = 0; j < count; j++) c[j] = m[i + j];
+            const float scale = ms[i / STATE_BLOCK];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = code_value<3>(c[j] & 127u) * scale, x[j] = c[j] & 128u ? -x[j] : x[j];
+            if (vec && count == 4) put4(m_out + i, x);
+            else for (int j = 0; j < count; j++) m_out[i + j] = x[j];
         }
         if (v_out) {
-            const float r = code_value<4>(v[i]) * vs[i / STATE_BLOCK];
-            v_out[i] = r * r;
+            uint32_t c[4] = {};
+            float x[4];
+            if (vec && count == 4) get4(v + i, c);
+            else for (int j = 0; j < count; j++) c[j] = v[i + j];
+            const float scale = vs[i / STATE_BLOCK];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float r = code_value<4>(c[j]) * scale;
+                x[j] = r * r;
+            }
+            if (vec && count == 4) put4(v_out + i, x);
+            else for (int j = 0; j < count; j++) v_out[i + j] = x[j];
         }
     }
 }
@@ -224,8 +285,11 @@ hipError_t launch_adamw(const AdamwArgs &a, hipStream_t s) {
         if (i == a.n_tensors) break;
         const bert_amd_adamw_tensor &o = a.t[i];
         if (!o.n) continue;
+        const auto off = [](const void *p, int bytes) { return (uintptr_t)p & (4 * bytes - 1); };
+        const int state = a.bits == 8 ? 1 : 4;
+        const bool vec = !(off(o.p, 4) | off(o.grad, elem_size(a.grad_type)) | off(o.m, state) | off(o.v, state) | off(o.copy, 2));
         t.t[t.count++] = {o.p, o.grad, o.m, o.v, o.m_scale, o.v_scale, o.copy, o.n, (float)(1 - a.lr * o.weight_decay),
-                          mix((uint32_t)i * 0x9E3779B9u ^ a.seed), chunks};
+                          mix((uint32_t)i * 0x9E3779B9u ^ a.seed), (int32_t)chunks, vec};
         chunks += more;
     }
     return hipSuccess;
@@ -233,7 +297,9 @@ hipError_t launch_adamw(const AdamwArgs &a, hipStream_t s) {
 
 hipError_t launch_adamw_moments(int64_t n, const uint8_t *m, const float *ms, const uint8_t *v, const float *vs, float *m_out,
                                 float *v_out, hipStream_t s) {
-    hipLaunchKernelGGL(moments_kernel, dim3(std::min<int64_t>(1 << 16, ceil_div<int64_t>(n, 256))), dim3(256), 0, s, n, m, ms, v, vs, m_out, v_out);
+    const bool vec = !(((uintptr_t)m | (uintptr_t)v) & 3) && !(((uintptr_t)m_out | (uintptr_t)v_out) & 15);
+    hipLaunchKernelGGL(moments_kernel, dim3(std::min<int64_t>(1 << 16, ceil_div<int64_t>(n, 1024))), dim3(256), 0, s, n, m, ms, v, vs, m_out,
+                       v_out, vec);
     return hipGetLastError();
 }
 
