@@ -115,9 +115,9 @@ def lib() -> ctypes.CDLL:
     # the operators around the encoder (bertops.py)
     i32, i64, p, f64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_double
     for name, res, args in (
-        ("bert_amd_linear_workspace", i64, [i32, i64, i32, i32]),
+        ("bert_amd_linear_workspace", i64, [i32, i64, i32, i32, i32]),
         ("bert_amd_linear", i32, [i32, i32, i32, i64, i32, i32, p, i64, p, i64, p, p, i64, p, i64, p, i64, p, i64, p]),
-        ("bert_amd_linear_backward_workspace", i64, [i32, i32, i64, i32, i32]),
+        ("bert_amd_linear_backward_workspace", i64, [i32, i32, i64, i32, i32, i32]),
         ("bert_amd_linear_backward", i32, [i32, i32, i32, i64, i32, i32, p, i64, p, i64, p, i64, p, i64, p, i64, p, i64,
                                            p, p, i64, p]),
         ("bert_amd_lookup", i32, [i32, i32, i32, i64, i32, i32, p, i64, p, ctypes.c_float, p, i64, p]),

@@ -77,6 +77,16 @@ def _vector(name: str, t: torch.Tensor, device, n: int) -> int:
     return t.data_ptr()
 
 
+def _aligned(size: int, *matrices) -> int:
+    """Whether all (address, row stride) allow 16-byte pieces."""
+    bits = 0
+    for p, ld in matrices:
+        if ld >= 1 << 21:
+            return 0
+        bits |= p | ld * size
+    return int(bits & 15 == 0)
+
+
 def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
            act: str = "none", save_z: bool = False, out: Optional[torch.Tensor] = None):
     """act(x w^T + bias) + residual for x [M, K] and w [N, K] of one type; bias is float32.
@@ -91,10 +101,10 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     y = torch.empty(M, N, dtype=dt, device=dev) if out is None else out
     ldy = N if out is None else _matrix("out", out, dt, dev, M, N)
     z = torch.empty(M, N, dtype=dt, device=dev) if save_z else None
-    L = bertlib.lib()
-    keep, ws, nws = _room(L.bert_amd_linear_workspace(TYPES[dt], M, N, K), dev)
-    _check(L.bert_amd_linear(dev.index, TYPES[dt], a, M, N, K, x.data_ptr(), ldx, w.data_ptr(), ldw, b, r, ldr, y.data_ptr(),
-                             ldy, z.data_ptr() if save_z else None, N, ws, nws, _stream(dev)))
+    L, px, pw, typ = bertlib.lib(), x.data_ptr(), w.data_ptr(), TYPES[dt]
+    keep, ws, nws = _room(L.bert_amd_linear_workspace(typ, M, N, K, _aligned(x.element_size(), (px, ldx), (pw, ldw))), dev)
+    _check(L.bert_amd_linear(dev.index, typ, a, M, N, K, px, ldx, pw, ldw, b, r, ldr, y.data_ptr(), ldy,
+                             z.data_ptr() if save_z else None, N, ws, nws, _stream(dev)))
     return (y, z) if save_z else y
 
 
@@ -111,7 +121,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *, z: Op
     dw = torch.empty(N, K, dtype=dt, device=dev) if need[1] else None
     db = torch.empty(N, dtype=torch.float32, device=dev) if need[2] else None
     L = bertlib.lib()
-    keep, ws, nws = _room(L.bert_amd_linear_backward_workspace(TYPES[dt], a, M, N, K), dev)
+    aligned = _aligned(x.element_size(), (x.data_ptr(), ldx), (w.data_ptr(), ldw), (dy.data_ptr(), lddy))
+    keep, ws, nws = _room(L.bert_amd_linear_backward_workspace(TYPES[dt], a, M, N, K, aligned), dev)
     _check(L.bert_amd_linear_backward(dev.index, TYPES[dt], a, M, N, K, dy.data_ptr(), lddy, pz, ldz, x.data_ptr(), ldx,
                                       w.data_ptr(), ldw, dx.data_ptr() if need[0] else None, K,
                                       dw.data_ptr() if need[1] else None, K, db.data_ptr() if need[2] else None, ws, nws,

@@ -25,7 +25,9 @@ struct LinearArgs {
     int64_t ldx = 0, ldw = 0, ldr = 0, ldy = 0, ldz = 0;
     void *ws = nullptr;
 };
-int64_t linear_ws_bytes(int type, int64_t M, int N, int K);
+// whether a matrix's address and row stride allow whole 16-byte pieces; `aligned` below: those of all inputs do
+bool linear_aligned(const void *p, int64_t ld, int type);
+int64_t linear_ws_bytes(int type, int64_t M, int N, int K, bool aligned);
 hipError_t launch_linear(const LinearArgs &a, hipStream_t s);
 
 // dx = dz W, dw = dz^T x, db = sum of dz over rows, dz = dy act'(z)
@@ -39,7 +41,7 @@ struct LinearGradArgs {
     int64_t lddy = 0, ldz = 0, ldx = 0, ldw = 0, lddx = 0, lddw = 0;
     void *ws = nullptr;
 };
-int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K);
+int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K, bool aligned);
 hipError_t launch_linear_grad(const LinearGradArgs &a, hipStream_t s);
 
 struct LookupArgs {

@@ -77,9 +77,9 @@ bool workspace_ok(const void *p, int64_t bytes, int64_t need) {
 
 extern "C" {
 
-int64_t bert_amd_linear_workspace(int32_t type, int64_t M, int32_t N, int32_t K) {
+int64_t bert_amd_linear_workspace(int32_t type, int64_t M, int32_t N, int32_t K, int32_t aligned) {
     if (!linear_shape_ok(type, M, N, K)) return refuse("bert_amd_linear_workspace: invalid type or size");
-    return linear_ws_bytes(type, M, N, K);
+    return linear_ws_bytes(type, M, N, K, aligned != 0);
 }
 
 int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int64_t M, int32_t N, int32_t K, const void *x, int64_t ldx,
@@ -96,8 +96,9 @@ int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int64_t M, in
             if (const char *bad = bad_matrix(m)) return refuse("bert_amd_linear: %s is null, misaligned or has too short rows", bad);
     if (bias && off(bias, 4)) return refuse("bert_amd_linear: bias is misaligned");
     if (residual == y && ldr != ldy) return refuse("bert_amd_linear: residual is y with another row stride");
-    if (!workspace_ok(workspace, workspace_bytes, linear_ws_bytes(type, M, N, K)))
-        return refuse("bert_amd_linear: workspace is null, misaligned or under %lld bytes", (long long)linear_ws_bytes(type, M, N, K));
+    const int64_t need = linear_ws_bytes(type, M, N, K, linear_aligned(x, ldx, type) && linear_aligned(w, ldw, type));
+    if (!workspace_ok(workspace, workspace_bytes, need))
+        return refuse("bert_amd_linear: workspace is null, misaligned or under %lld bytes", (long long)need);
     LinearArgs a;
     a.type = type, a.act = act, a.M = M, a.N = N, a.K = K;
     a.x = x, a.w = w, a.r = residual, a.bias = bias, a.y = y, a.z = z, a.ws = workspace;
@@ -105,9 +106,9 @@ int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int64_t M, in
     return on_device("bert_amd_linear", device, [&] { return launch_linear(a, (hipStream_t)hip_stream); });
 }
 
-int64_t bert_amd_linear_backward_workspace(int32_t type, int32_t act, int64_t M, int32_t N, int32_t K) {
+int64_t bert_amd_linear_backward_workspace(int32_t type, int32_t act, int64_t M, int32_t N, int32_t K, int32_t aligned) {
     if (!linear_shape_ok(type, M, N, K)) return refuse("bert_amd_linear_backward_workspace: invalid type or size");
-    return linear_grad_ws_bytes(type, act, M, N, K);
+    return linear_grad_ws_bytes(type, act, M, N, K, aligned != 0);
 }
 
 int32_t bert_amd_linear_backward(int32_t device, int32_t type, int32_t act, int64_t M, int32_t N, int32_t K, const void *dy,
@@ -128,7 +129,8 @@ int32_t bert_amd_linear_backward(int32_t device, int32_t type, int32_t act, int6
         if (m.p)
             if (const char *bad = bad_matrix(m)) return refuse("bert_amd_linear_backward: %s is misaligned or has too short rows", bad);
     if (!dx && !dw && !dbias) return 0;
-    const int64_t need = linear_grad_ws_bytes(type, act, M, N, K);
+    const bool aligned = linear_aligned(dy, lddy, type) && (!dw || linear_aligned(x, ldx, type)) && (!dx || linear_aligned(w, ldw, type));
+    const int64_t need = linear_grad_ws_bytes(type, act, M, N, K, aligned);
     if (!workspace_ok(workspace, workspace_bytes, need))
         return refuse("bert_amd_linear_backward: workspace is null, misaligned or under %lld bytes", (long long)need);
     LinearGradArgs a;

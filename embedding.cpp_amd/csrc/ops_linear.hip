@@ -8,6 +8,7 @@
 #include "ops_common.h"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -31,17 +32,11 @@ __device__ __forceinline__ void slope8(float *v, const float *z, int act) {
     }
 }
 
-// ---- the tile kernel for any size, stride and alignment --------------------
-//
-// C[m][n] = sum over k of A(m, k) B(n, k) in 64 x 64 tiles, four waves of
-// 32 x 32 each; A(m, k) is at A[m lda + k], or at A[k lda + m] where TA.
-// Chunks of 16 bytes are loaded along the contiguous axis, whole where they are
-// inside and aligned, else by element with zeros outside.  gridDim.z splits k:
-// split sums go to `part` and split_join_kernel adds them in order.
 struct Operand {
     const void *p = nullptr;
     int64_t ld = 0;
     bool vec = false;  // p and ld allow 16-byte loads
+    bool padded = false;  // zeros follow a row up to a multiple of 16 bytes
 };
 struct Epilogue {
     int act = 0;
@@ -73,73 +68,62 @@ __device__ __forceinline__ Chunk<T, CH> load_chunk(const T *p, int64_t ld, bool 
     return o;
 }
 
-constexpr int TB = 64;  // tile rows and columns
-template <int TYPE> constexpr int tile_k() { return TYPE == BERT_AMD_F32 ? 16 : 32; }
-// LDS row length: one float or 16 bytes more than the tile, so that the lanes
-// of an operand read start in different banks
-template <int TYPE> constexpr int tile_ld() { return TYPE == BERT_AMD_F32 ? 17 : 40; }
+// ---- few rows ------------------------------------------------------------------
+//
+// Up to 8 rows of x, as a server's single requests have them: bound by reading
+// W once, so no tile and no second launch.  A wave takes COLS rows of W, its
+// lanes 16 bytes each of them at a time, and every row of x with them, in f32
+// on the vector units; the lanes' sums are joined by a butterfly.
+constexpr int FEW_ROWS = 8;
 
-template <int TYPE, bool TRANS>
-__device__ __forceinline__ void stage_tile(const Operand &o, int64_t row0, int64_t rows, int64_t k0, int64_t k1,
-                                           typename Elem<TYPE>::T *lds) {
+template <int TYPE, int ROWS, int COLS>
+__global__ __launch_bounds__(256) void few_rows_kernel(Operand X, Operand W, int M, int64_t N, int64_t K, Epilogue e) {
     typedef typename Elem<TYPE>::T T;
-    constexpr int CH = Elem<TYPE>::CH, BK = tile_k<TYPE>(), LD = tile_ld<TYPE>();
-    const int t = threadIdx.x;
-    if constexpr (!TRANS) {
-        const int r = t / (BK / CH), c = t % (BK / CH) * CH;
-        const auto v = load_chunk<T, CH>((const T *)o.p, o.ld, o.vec, row0 + r, k0 + c, rows, k1);
+    constexpr int CH = Elem<TYPE>::CH;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * COLS;
+    if (n0 >= N) return;
+    float acc[ROWS][COLS] = {};
+#pragma unroll 2
+    for (int64_t k = CH * lane; k < K; k += 64 * CH) {
+        Chunk<T, CH> w[COLS];
 #pragma unroll
-        for (int j = 0; j < CH; j++) lds[r * LD + c + j] = v.v[j];
-    } else {
-        const int r = t / (TB / CH), c = t % (TB / CH) * CH;
-        const auto v = load_chunk<T, CH>((const T *)o.p, o.ld, o.vec, k0 + r, row0 + c, k1, rows);
+        for (int c = 0; c < COLS; c++) w[c] = load_chunk<T, CH>((const T *)W.p, W.ld, W.vec, n0 + c, k, N, K);
 #pragma unroll
-        for (int j = 0; j < CH; j++) lds[(c + j) * LD + r] = v.v[j];
+        for (int r = 0; r < ROWS; r++) {
+            const auto x = load_chunk<T, CH>((const T *)X.p, X.ld, X.vec, r, k, M, K);
+#pragma unroll
+            for (int c = 0; c < COLS; c++)
+#pragma unroll
+                for (int j = 0; j < CH; j++) acc[r][c] = __builtin_fmaf((float)x.v[j], (float)w[c].v[j], acc[r][c]);
+        }
     }
+    float v = 0.f;  // lane r COLS + c: the sum of row r and column c
+#pragma unroll
+    for (int r = 0; r < ROWS; r++)
+#pragma unroll
+        for (int c = 0; c < COLS; c++) {
+            float a = acc[r][c];
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) a += __shfl_xor(a, d);
+            if (lane == r * COLS + c) v = a;
+        }
+    const int64_t n = n0 + lane % COLS;
+    if (lane < ROWS * COLS && lane / COLS < M && n < N) epilogue_store<T>(e, lane / COLS, n, v);
 }
 
-template <int TYPE, bool TA, bool TBT>
-__global__ __launch_bounds__(256) void tile_gemm_kernel(Operand A, Operand B, int64_t M, int64_t N, int64_t K,
-                                                        int64_t k_per_split, float *part, Epilogue e) {
-    typedef typename Elem<TYPE>::T T;
-    constexpr int BK = tile_k<TYPE>(), LD = tile_ld<TYPE>();
-    __shared__ T sa[TB * LD], sb[TB * LD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave & 1, wn = wave >> 1, r = lane & 31, h = lane >> 5;
-    const int64_t tiles_n = ceil_div<int64_t>(N, TB);
-    const int64_t m0 = blockIdx.x / tiles_n * TB, n0 = blockIdx.x % tiles_n * TB;
-    const int64_t ka = (int64_t)blockIdx.z * k_per_split, kb = min(K, ka + k_per_split);
-    f32x16 acc = {};
-    for (int64_t k0 = ka; k0 < kb; k0 += BK) {
-        stage_tile<TYPE, TA>(A, m0, M, k0, kb, sa);
-        stage_tile<TYPE, TBT>(B, n0, N, k0, kb, sb);
-        __syncthreads();
-        const T *pa = sa + (32 * wm + r) * LD, *pb = sb + (32 * wn + r) * LD;
-        if constexpr (TYPE == BERT_AMD_F32) {
-#pragma unroll
-            for (int k = 0; k < BK; k += 2) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(pa[k + h], pb[k + h], acc, 0, 0, 0);
-        } else {
-#pragma unroll
-            for (int k = 0; k < BK; k += 16) {
-                const u32x4 a = *(const u32x4 *)(pa + k + 8 * h), b = *(const u32x4 *)(pb + k + 8 * h);
-                if constexpr (TYPE == BERT_AMD_F16)
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
-                else
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
-            }
-        }
-        __syncthreads();
-    }
-    const int64_t n = n0 + 32 * wn + r;
-    if (n >= N) return;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int64_t m = m0 + 32 * wm + 8 * (i >> 2) + 4 * h + (i & 3);
-        if (m >= M) continue;
-        if (part)
-            part[((int64_t)blockIdx.z * M + m) * N + n] = acc[i];
-        else
-            epilogue_store<T>(e, m, n, acc[i]);
+// ---- rows in whole chunks -------------------------------------------------------
+//
+// A matrix whose rows are not aligned, or no whole chunks long, is copied into
+// the workspace with zeros up to the next chunk: one more pass over it, where
+// loads of single elements would slow the whole product down.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T *from, int64_t ld, int64_t rows, int64_t cols, T *to, int64_t ldt) {
+    constexpr int CH = 16 / sizeof(T);
+    const int64_t chunks = ldt / CH;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / chunks, c = (i - r * chunks) * CH;
+        *(u32x4 *)(to + r * ldt + c) = __builtin_bit_cast(u32x4, load_chunk<T, CH>(from, ld, false, r, c, rows, cols));
     }
 }
 
@@ -468,18 +452,21 @@ __global__ __launch_bounds__(256) void split_join_kernel(const float *part, int 
     }
 }
 
-// dz = dy act'(z) in the layer's type, and the unrounded dz's column sums over
-// `rows` rows at a time: 32 threads of 8 columns each, 8 rows side by side,
-// their sums joined in LDS in a fixed order.
-template <typename T>
+// dz = dy act'(z) in the layer's type, rows `lddz` apart with zeros past their
+// end, and the unrounded dz's column sums over `rows` rows at a time: CT
+// threads of 8 columns each, 256 / CT rows side by side, their sums joined in
+// LDS in a fixed order.
+template <typename T, int CT>
 __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, const T *z, int64_t ldz, int act, int64_t M, int64_t N,
-                                                 int rows, T *dz, float *part, bool vec) {
-    __shared__ float sums[8][32][9];
-    const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-    const int64_t n = (int64_t)blockIdx.x * 256 + 8 * c, m1 = min(M, (int64_t)(blockIdx.y + 1) * rows);
+                                                 int64_t rows, T *dz, int64_t lddz, float *part, bool vec) {
+    constexpr int RT = 256 / CT;
+    __shared__ float sums[RT][CT][9];
+    const int c = threadIdx.x % CT, r = threadIdx.x / CT;
+    const int64_t n = ((int64_t)blockIdx.x * CT + c) * 8, m1 = min(M, (int64_t)(blockIdx.y + 1) * rows);
     const bool whole = vec && n + 8 <= N;
     float sum[8] = {};
-    for (int64_t m = (int64_t)blockIdx.y * rows + r; m < m1; m += 8) {
+#pragma unroll 2
+    for (int64_t m = (int64_t)blockIdx.y * rows + r; m < m1; m += RT) {
         float v[8] = {}, s[8] = {};
         if (whole) {
             add8(dy + m * lddy + n, v);
@@ -492,13 +479,18 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
                     if (act) s[i] = (float)z[m * ldz + n + i];
                 }
         }
-        slope8<T>(v, s, act);
+        if (act) slope8<T>(v, s, act);
         if (dz) {
-            if (whole && N % 8 == 0) put8(dz + m * N + n, v);
-            else
+            if (n + 8 <= lddz) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    if (n + i < N) dz[m * N + n + i] = (T)v[i];
+                    if (n + i >= N) v[i] = 0.f;
+                put8(dz + m * lddz + n, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (n + i < lddz) dz[m * lddz + n + i] = n + i < N ? (T)v[i] : (T)0.f;
+            }
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) sum[i] += v[i];
@@ -507,11 +499,11 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
 #pragma unroll
     for (int i = 0; i < 8; i++) sums[r][c][i] = sum[i];
     __syncthreads();
-    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (col >= N) return;
+    const int64_t col = (int64_t)blockIdx.x * CT * 8 + threadIdx.x;
+    if (threadIdx.x >= CT * 8 || col >= N) return;
     float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) v += sums[i][threadIdx.x >> 3][threadIdx.x & 7];
+#pragma unroll 8
+    for (int i = 0; i < RT; i++) v += sums[i][threadIdx.x >> 3][threadIdx.x & 7];
     part[blockIdx.y * N + col] = v;
 }
 
@@ -531,12 +523,16 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const float *part, int6
     out[n] = v;
 }
 
-// rows of a dz_kernel workgroup: about 2048 workgroups, and no more partial sums than that
-int dz_rows(int64_t M, int64_t N) {
+// Rows of a dz_kernel workgroup.  Up to 1024 rows: all of them, 32 columns wide,
+// and the sums are the bias's gradient at once (a launch less: 4 us of about 30
+// for 256 x 384).  More: 256 columns wide, about 2048 workgroups.
+constexpr int64_t DZ_ONE = 1024;
+int64_t dz_rows(int64_t M, int64_t N) {
+    if (M <= DZ_ONE) return std::max<int64_t>(M, 1);
     int64_t rows = 8;
     while (rows < M && ceil_div(M, rows) * ceil_div<int64_t>(N, 256) > 2048) rows *= 2;
     while (ceil_div(M, rows) > 2048) rows *= 2;
-    return (int)std::min<int64_t>(rows, 1 << 30);
+    return rows;
 }
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -544,7 +540,6 @@ int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 // How a product runs: its tile and in how many parts k is split.
 struct Plan {
     int tile = 64;      // rows and columns
-    bool stage = false; // stage_gemm_kernel; else tile_gemm_kernel, 64 x 64
     int splits = 1;
     int64_t per = 0;    // k of a split
 };
@@ -553,84 +548,123 @@ struct Plan {
 // and where k is split the pass that joins the parts (written and read once).
 // A stage's time and the time around, in us, as measured on large products:
 // 256 x 256 tiles, one on a CU; 128 x 128, two; 64 x 64, four.
-Plan plan_for(int type, bool fits, int64_t M, int64_t N, int64_t K) {
+Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
     Plan best;
-    best.per = ceil_div<int64_t>(std::max<int64_t>(K, 1), 64) * 64;
     const struct { int tile, wgs; double stage, around; } forms[] = {
         {256, 256, 1.7, 6}, {128, 512, 1.05, 4}, {64, 1024, 0.8, 3}};
     double least = 1e30;
     for (const auto &f : forms) {
-        if (fits ? type == BERT_AMD_F32 && f.tile == 256 : f.tile != 64) continue;
+#ifdef FORCE_TILE
+        if (f.tile != FORCE_TILE) continue;
+#endif
+        if (type == BERT_AMD_F32 && f.tile == 256) continue;
         const double slower = type == BERT_AMD_F32 ? 4 : 1;  // f32 products run at an eighth of the rate, on half the k
         const int64_t tiles = ceil_div<int64_t>(M, f.tile) * ceil_div<int64_t>(N, f.tile);
         const int sk = type == BERT_AMD_F32 ? 32 : 64;
         for (int splits = 1; splits <= 64; splits *= 2) {
-            if (splits > 1 && (K < splits * 4 * sk || tiles * splits > 2 * f.wgs)) break;
+            if (splits > 1 && (K < splits * 2 * sk || tiles * splits > 2 * f.wgs)) break;
+#ifdef FORCE_SPLITS
+            if (splits != FORCE_SPLITS && K >= FORCE_SPLITS*2*sk) continue;
+#endif
             const int64_t per = std::max<int64_t>(64, ceil_div(ceil_div<int64_t>(K, splits), (int64_t)64) * 64);
-            const double join = splits > 1 ? 3 + 8e-6 / 4 * splits * M * N : 0;
+            const double join = splits > 1 ? 5 + 8e-6 / 4 * splits * M * N : 0;
             const double t = ceil_div<int64_t>(tiles * splits, f.wgs) * (ceil_div<int64_t>(per, sk) * f.stage * slower + f.around) + join;
             if (t < least) least = t, best.tile = f.tile, best.splits = splits, best.per = per;
         }
     }
-    best.stage = fits;
     best.splits = (int)std::max<int64_t>(1, ceil_div(K, best.per));  // rounding the parts up may leave the last ones empty
     return best;
 }
-int64_t split_bytes(int type, bool fits, int64_t M, int64_t N, int64_t K) {
-    const Plan p = plan_for(type, fits, M, N, K);
+// bytes of a product's split sums
+int64_t split_bytes(int type, int64_t M, int64_t N, int64_t K) {
+    const Plan p = plan_for(type, M, N, K);
     return p.splits > 1 ? round256(p.splits * M * N * 4) : 0;
 }
 
-// split sums of a product, whatever its operands' alignment
-int64_t product_bytes(int type, int64_t M, int64_t N, int64_t K) {
-    return std::max(split_bytes(type, false, M, N, K), split_bytes(type, true, M, N, K));
+int64_t padded(int type, int64_t n) {
+    const int64_t ch = 16 / elem_size(type);
+    return (n + ch - 1) / ch * ch;
+}
+int64_t packed_bytes(int type, int64_t rows, int64_t cols) { return round256(rows * padded(type, cols) * elem_size(type)); }
+
+// whether the stage kernel takes a matrix with rows of `cols` as it is: whole aligned chunks, offsets within a tile under 2^31
+bool whole_rows(const Operand &o, int type, int64_t cols) {
+    return o.padded || (o.vec && cols % (16 / elem_size(type)) == 0 && o.ld < (1 << 21));
 }
 
-// whether the stage kernel takes an operand: whole aligned chunks, and offsets within a tile under 2^31
-template <int TYPE>
-bool stage_operand(const Operand &o, bool trans, int64_t rows, int64_t k) {
-    return o.vec && (trans ? rows : k) % Elem<TYPE>::CH == 0 && o.ld < (1 << 21);
+// `o` as the stage kernel takes it; a copy goes to `ws`, which moves on
+template <typename T>
+Operand pack(const Operand &o, int type, int64_t rows, int64_t cols, char *&ws, hipStream_t s) {
+    if (whole_rows(o, type, cols)) return o;
+    const int64_t ld = padded(type, cols), chunks = rows * ld * (int64_t)sizeof(T) / 16;
+    const Operand to = {ws, ld, true, true};
+    if (chunks)
+        hipLaunchKernelGGL((pack_kernel<T>), dim3(std::min<int64_t>(1 << 14, ceil_div<int64_t>(chunks, 256))), dim3(256), 0, s, (const T *)o.p,
+                           o.ld, rows, cols, (T *)ws, ld);
+    ws += packed_bytes(type, rows, cols);
+    return to;
 }
 
 template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
-void launch_stage(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, const Plan &p, float *part, const Epilogue &e,
-                  bool vec, hipStream_t s) {
+hipError_t launch_stage(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, const Plan &p, float *part, const Epilogue &e,
+                        bool vec, hipStream_t s) {
     constexpr int lds = std::max(2 * (BM + BN) * 128, BM * WN * OUT_LD * 4);
     const auto k = stage_gemm_kernel<TYPE, TA, TBT, BM, BN, WM, WN>;
-    (void)hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (lds > 65536) {  // beyond a launch's default: asked for once on each device
+        static std::atomic<uint64_t> asked{0};
+        int dev = 0;
+        if (hipError_t r = hipGetDevice(&dev); r != hipSuccess) return r;
+        const uint64_t bit = 1ull << (dev & 63);
+        if (!(asked.load(std::memory_order_relaxed) & bit) || dev > 63) {
+            if (hipError_t r = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds); r != hipSuccess) return r;
+            asked.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     const int64_t tiles = ceil_div<int64_t>(M, BM) * ceil_div<int64_t>(N, BN);
     hipLaunchKernelGGL(k, dim3(tiles, 1, p.splits), dim3(WM * WN * 64), lds, s, A, B, M, N, K, p.per, part, e, vec);
+    return hipGetLastError();
 }
 
+// C = A B^T of two matrices in whole chunks
 template <int TYPE, bool TA, bool TBT>
 hipError_t gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, void *ws, const Epilogue &e, hipStream_t s) {
     typedef typename Elem<TYPE>::T T;
-    const bool fits = stage_operand<TYPE>(A, TA, M, K) && stage_operand<TYPE>(B, TBT, N, K);
-    const Plan p = plan_for(TYPE, fits, M, N, K);
+    const Plan p = plan_for(TYPE, M, N, K);
     float *part = p.splits > 1 ? (float *)ws : nullptr;
     const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(T)); };
     const bool vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr);
-    if (!p.stage) {
-        const int64_t tiles = ceil_div<int64_t>(M, TB) * ceil_div<int64_t>(N, TB);
-        hipLaunchKernelGGL((tile_gemm_kernel<TYPE, TA, TBT>), dim3(tiles, 1, p.splits), dim3(256), 0, s, A, B, M, N, K, p.per, part, e);
-    } else if (p.tile == 64) {
-        launch_stage<TYPE, TA, TBT, 64, 64, 2, 1>(A, B, M, N, K, p, part, e, vec, s);
-    } else if (p.tile == 128) {
-        launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
-    } else {
-        if constexpr (TYPE != BERT_AMD_F32) launch_stage<TYPE, TA, TBT, 256, 256, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
-    }
-    if (part)
-        hipLaunchKernelGGL((split_join_kernel<T>), dim3(std::min<int64_t>(1024, ceil_div<int64_t>(M * N, 256))), dim3(256), 0, s, part, p.splits, M, N, e);
+    hipError_t r = hipSuccess;
+    if (p.tile == 64) r = launch_stage<TYPE, TA, TBT, 64, 64, 2, 1>(A, B, M, N, K, p, part, e, vec, s);
+    else if (p.tile == 128) r = launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
+    else if constexpr (TYPE != BERT_AMD_F32) r = launch_stage<TYPE, TA, TBT, 256, 256, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
+    if (r != hipSuccess || !part) return r;
+    hipLaunchKernelGGL((split_join_kernel<T>), dim3(std::min<int64_t>(1024, ceil_div<int64_t>(M * N, 256))), dim3(256), 0, s, part, p.splits, M, N, e);
     return hipGetLastError();
 }
 
 Operand operand(const void *p, int64_t ld, int type) { return {p, ld, aligned16(p, ld * elem_size(type))}; }
 
+template <int TYPE, int COLS>
+hipError_t few_rows(const Operand &x, const Operand &w, const LinearArgs &a, const Epilogue &e, hipStream_t s) {
+    const dim3 grid(ceil_div(a.N, 4 * COLS));
+    const int M = (int)a.M;
+    if (M == 1) hipLaunchKernelGGL((few_rows_kernel<TYPE, 1, COLS>), grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
+    else if (M == 2) hipLaunchKernelGGL((few_rows_kernel<TYPE, 2, COLS>), grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
+    else if (M <= 4) hipLaunchKernelGGL((few_rows_kernel<TYPE, 4, COLS>), grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
+    else hipLaunchKernelGGL((few_rows_kernel<TYPE, 8, COLS>), grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
+    return hipGetLastError();
+}
+
 template <int TYPE>
 hipError_t linear_t(const LinearArgs &a, hipStream_t s) {
-    return gemm<TYPE, false, false>(operand(a.x, a.ldx, TYPE), operand(a.w, a.ldw, TYPE), a.M, a.N, a.K, a.ws,
-                                         {a.act, a.bias, a.r, a.y, a.z, a.ldr, a.ldy, a.ldz}, s);
+    typedef typename Elem<TYPE>::T T;
+    const Operand x = operand(a.x, a.ldx, TYPE), w = operand(a.w, a.ldw, TYPE);
+    const Epilogue e = {a.act, a.bias, a.r, a.y, a.z, a.ldr, a.ldy, a.ldz};
+    if (a.M <= FEW_ROWS)  // one column a wave fills the chip sooner, four read x a quarter as often
+        return a.N < 4096 ? few_rows<TYPE, 1>(x, w, a, e, s) : few_rows<TYPE, 4>(x, w, a, e, s);
+    char *ws = (char *)a.ws;
+    const Operand px = pack<T>(x, TYPE, a.M, a.K, ws, s), pw = pack<T>(w, TYPE, a.N, a.K, ws, s);
+    return gemm<TYPE, false, false>(px, pw, a.M, a.N, a.K, ws, e, s);
 }
 
 template <int TYPE>
@@ -639,43 +673,56 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
     char *ws = (char *)a.ws;
     Operand dz = operand(a.dy, a.lddy, TYPE);
     T *kept = nullptr;
-    if (a.act) {
+    const int64_t lddz = padded(TYPE, a.N);
+    if ((a.dx || a.dw) && (a.act || !whole_rows(dz, TYPE, a.N))) {
         kept = (T *)ws;
-        ws += round256(a.M * a.N * sizeof(T));
-        dz = operand(kept, a.N, TYPE);
+        ws += packed_bytes(TYPE, a.M, a.N);
+        dz = {kept, lddz, true, true};
     }
-    if (kept || a.db) {
-        const int rows = dz_rows(a.M, a.N);
-        const int64_t blocks = ceil_div<int64_t>(a.M, rows);
-        float *part = a.db ? (float *)ws : nullptr;
+    if ((kept || a.db) && a.M) {
+        const int64_t rows = dz_rows(a.M, a.N), blocks = ceil_div<int64_t>(a.M, rows);
+        float *part = !a.db || blocks == 1 ? a.db : (float *)ws;
         const bool vec = aligned16(a.dy, a.lddy * (int64_t)sizeof(T)) && (!a.act || aligned16(a.z, a.ldz * (int64_t)sizeof(T)));
-        if (blocks)
-            hipLaunchKernelGGL((dz_kernel<T>), dim3(ceil_div(a.N, 256), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z,
-                               a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, part, vec);
-        if (a.db) {
+        if (a.M <= DZ_ONE)
+            hipLaunchKernelGGL((dz_kernel<T, 4>), dim3(ceil_div(a.N, 32), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z,
+                               a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, lddz, part, vec);
+        else
+            hipLaunchKernelGGL((dz_kernel<T, 32>), dim3(ceil_div(a.N, 256), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy,
+                               (const T *)a.z, a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, lddz, part, vec);
+        if (a.db && blocks > 1) {
             hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 32)), dim3(256), 0, s, part, blocks, (int64_t)a.N, a.db);
             ws += round256(blocks * a.N * 4);
         }
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    } else if (a.db) {
+        hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 32)), dim3(256), 0, s, (const float *)nullptr, (int64_t)0, (int64_t)a.N, a.db);
     }
     if (a.dx && a.M) {
         Epilogue e;
         e.y = a.dx;
         e.ldy = a.lddx;
-        if (hipError_t r = gemm<TYPE, false, true>(dz, operand(a.w, a.ldw, TYPE), a.M, a.K, a.N, ws, e, s); r != hipSuccess) return r;
+        char *rest = ws;
+        const Operand w = pack<T>(operand(a.w, a.ldw, TYPE), TYPE, a.N, a.K, rest, s);
+        if (hipError_t r = gemm<TYPE, false, true>(dz, w, a.M, a.K, a.N, rest, e, s); r != hipSuccess) return r;
     }
     if (a.dw) {
         Epilogue e;
         e.y = a.dw;
         e.ldy = a.lddw;
-        if (hipError_t r = gemm<TYPE, true, true>(dz, operand(a.x, a.ldx, TYPE), a.N, a.K, a.M, ws, e, s); r != hipSuccess) return r;
+        char *rest = ws;
+        const Operand x = pack<T>(operand(a.x, a.ldx, TYPE), TYPE, a.M, a.K, rest, s);
+        if (hipError_t r = gemm<TYPE, true, true>(dz, x, a.N, a.K, a.M, rest, e, s); r != hipSuccess) return r;
     }
-    return hipSuccess;
+    return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t linear_ws_bytes(int type, int64_t M, int N, int K) { return product_bytes(type, M, N, K); }
+int64_t linear_ws_bytes(int type, int64_t M, int N, int K, bool aligned) {
+    if (M <= FEW_ROWS) return 0;
+    const bool whole = aligned && padded(type, K) == K;
+    return (whole ? 0 : packed_bytes(type, M, K) + packed_bytes(type, N, K)) + split_bytes(type, M, N, K);
+}
 
 hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
     switch (a.type) {
@@ -685,9 +732,11 @@ hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
     }
 }
 
-int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K) {
-    return (act ? round256(M * N * elem_size(type)) : 0) + round256(ceil_div<int64_t>(M, dz_rows(M, N)) * N * 4) +
-           std::max(product_bytes(type, M, K, N), product_bytes(type, N, K, M));
+int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K, bool aligned) {
+    const bool whole_n = aligned && padded(type, N) == N, whole_k = aligned && padded(type, K) == K;
+    return (act || !whole_n ? packed_bytes(type, M, N) : 0) + round256(ceil_div<int64_t>(M, dz_rows(M, N)) * N * 4) +
+           std::max((whole_k ? 0 : packed_bytes(type, N, K)) + split_bytes(type, M, K, N),
+                    (whole_k ? 0 : packed_bytes(type, M, K)) + split_bytes(type, N, K, M));
 }
 
 hipError_t launch_linear_grad(const LinearGradArgs &a, hipStream_t s) {
@@ -697,5 +746,8 @@ hipError_t launch_linear_grad(const LinearGradArgs &a, hipStream_t s) {
         default: return linear_grad_t<BERT_AMD_BF16>(a, s);
     }
 }
+
+// whether rows of type `type`, `ld` elements apart, are whole aligned chunks as far as address and stride go
+bool linear_aligned(const void *p, int64_t ld, int type) { return aligned16(p, ld * elem_size(type)) && ld < (1 << 21); }
 
 }  // namespace bertamd

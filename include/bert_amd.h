@@ -225,8 +225,11 @@ enum bert_amd_act {
      y        : [M][N]; z: [M][N] or NULL: the pre-activation, kept for
                 bert_amd_linear_backward
    M = 0 does nothing; M < 2^31, 1 <= N, K < 2^22, and none of M N, M K and N K
-   over 2^34. */
-BERT_API int64_t bert_amd_linear_workspace(int32_t type, int64_t M, int32_t N, int32_t K);
+   over 2^34.
+   The workspace takes copies of x and w where their rows are not 16-byte pieces
+   throughout: `aligned` != 0 says that both begin on 16 bytes and their row
+   strides are multiples of 16 bytes (and under 2^21 elements). */
+BERT_API int64_t bert_amd_linear_workspace(int32_t type, int64_t M, int32_t N, int32_t K, int32_t aligned);
 BERT_API int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int64_t M, int32_t N, int32_t K,
                                  const void *x, int64_t ldx, const void *w, int64_t ldw, const float *bias,
                                  const void *residual, int64_t ldr, void *y, int64_t ldy, void *z, int64_t ldz,
@@ -237,8 +240,9 @@ BERT_API int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int6
    over the rows, f32 [N].  z is not read (and may be NULL) for act NONE; it may
    be any [M][N] values.  Any of dx, dw, dbias may be NULL: not computed.  F16
    and BF16 round dz to the type before the two products.  M = 0 gives zero dw
-   and dbias. */
-BERT_API int64_t bert_amd_linear_backward_workspace(int32_t type, int32_t act, int64_t M, int32_t N, int32_t K);
+   and dbias.  `aligned` as above, of dy, x and w. */
+BERT_API int64_t bert_amd_linear_backward_workspace(int32_t type, int32_t act, int64_t M, int32_t N, int32_t K,
+                                                    int32_t aligned);
 BERT_API int32_t bert_amd_linear_backward(int32_t device, int32_t type, int32_t act, int64_t M, int32_t N, int32_t K,
                                           const void *dy, int64_t lddy, const void *z, int64_t ldz, const void *x,
                                           int64_t ldx, const void *w, int64_t ldw, void *dx, int64_t lddx, void *dw,

@@ -68,7 +68,7 @@ def close(got, want, tol, what):
 
 # ---- the dense layer
 
-ODD = [(1, 1, 1), (1, 384, 384), (3, 5, 7), (17, 33, 65), (64, 64, 64), (130, 200, 72), (257, 128, 96), (5, 4100, 31), (300, 31, 1030)]
+ODD = [(1, 1, 1), (1, 384, 384), (3, 5, 7), (17, 33, 65), (64, 64, 64), (130, 200, 72), (257, 128, 96), (5, 4100, 31), (300, 31, 1030), (8, 70, 4100), (2, 1026, 4096), (9, 1000, 300), (1, 8, 5000)]
 
 
 def make_layer(M, K, N, dtype, seed=0):
@@ -658,18 +658,22 @@ def test_refusals_of_the_library():
     ok = dict(device=0, type=0, act=0, M=4, N=8, K=8, x=P, ldx=8, w=P, ldw=8, bias=P, r=P, ldr=8, y=P + 4096, ldy=8, z=NULL, ldz=8, ws=P, nws=big, s=NULL)
     for change, word in ((dict(type=2), "type"), (dict(type=7), "type"), (dict(act=6), "activation"), (dict(act=-1), "activation"), (dict(M=-1), "size"), (dict(M=1 << 31), "size"), (dict(N=0), "size"), (dict(K=0), "size"), (dict(N=1 << 22), "size"), (dict(M=1 << 30, N=1 << 10), "size"), (dict(x=NULL), "x"), (dict(x=P + 2), "x"), (dict(ldx=7), "x"), (dict(ldx=-8), "x"), (dict(w=NULL), "w"), (dict(y=NULL), "y"), (dict(ldy=0), "y"), (dict(ldy=7), "y"), (dict(r=P + 1), "residual"), (dict(z=P, ldz=0), "z"), (dict(bias=P + 1), "bias"), (dict(r=P + 4096, ldr=9), "residual")):
         refused(L.bert_amd_linear(*{**ok, **change}.values()), word)
-    need = L.bert_amd_linear_workspace(0, 4, 8, 100000)
-    assert need >= 0 and L.bert_amd_linear_workspace(5, 4, 8, 8) == -1
-    if need:
+    assert L.bert_amd_linear_workspace(5, 4, 8, 8, 1) == -1
+    for K in (100000, 100001):  # parts of k; copies in whole pieces
+        need = L.bert_amd_linear_workspace(0, 40, 8, K, 1)
+        assert need > 0
         for change in (dict(ws=NULL), dict(nws=need - 1), dict(ws=P + 8)):
-            refused(L.bert_amd_linear(*{**ok, "K": 100000, "ldx": 100000, "ldw": 100000, **change}.values()), "workspace")
+            refused(L.bert_amd_linear(*{**ok, "M": 40, "K": K, "ldx": K, "ldw": K, **change}.values()), "workspace")
+    need = L.bert_amd_linear_workspace(0, 40, 8, 100000, 1)
+    for change in (dict(x=P + 4), dict(ldw=100001)):  # asked for as aligned, given otherwise
+        refused(L.bert_amd_linear(*{**ok, "M": 40, "K": 100000, "ldx": 100000, "ldw": 100000, "nws": need, **change}.values()), "workspace")
     assert L.bert_amd_linear(*{**ok, "M": 0, "x": NULL}.values()) == 0
 
     ok = dict(device=0, type=1, act=2, M=4, N=8, K=8, dy=P, lddy=8, z=P, ldz=8, x=P, ldx=8, w=P, ldw=8, dx=P, lddx=8, dw=P, lddw=8, db=P, ws=P, nws=big, s=NULL)
     for change, word in ((dict(type=3), "type"), (dict(act=9), "activation"), (dict(M=-1), "size"), (dict(dy=NULL), "dy"), (dict(dy=P + 1), "dy"), (dict(z=NULL), "z"), (dict(ldz=4), "z"), (dict(x=NULL), "x"), (dict(w=NULL), "w"), (dict(lddx=0), "dx"), (dict(lddw=7), "dw"), (dict(db=P + 2), "dbias"), (dict(ws=NULL), "workspace"), (dict(nws=1), "workspace")):
         refused(L.bert_amd_linear_backward(*{**ok, **change}.values()), word)
     assert L.bert_amd_linear_backward(*{**ok, "dx": NULL, "dw": NULL, "db": NULL}.values()) == 0
-    assert L.bert_amd_linear_backward_workspace(1, 2, -1, 8, 8) == -1
+    assert L.bert_amd_linear_backward_workspace(1, 2, -1, 8, 8, 1) == -1
 
     ok = dict(device=0, type=2, out=0, n=4, V=10, E=64, table=P, ld=36, ids=P, scale=1.0, o=P, ldo=64, s=NULL)
     for change, word in ((dict(type=8), "types"), (dict(out=2), "types"), (dict(n=-1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(E=40), "size"), (dict(table=NULL), "table"), (dict(table=P + 1), "table"), (dict(ld=35), "table"), (dict(ld=37), "table"), (dict(ids=NULL), "ids"), (dict(ids=P + 2), "ids"), (dict(o=NULL), "out"), (dict(ldo=63), "out"), (dict(ldo=0), "out")):
@@ -716,9 +720,10 @@ def test_workspace_sizes():
     for t in (0, 1, 30):
         for N, K in ((1, 1), (384, 384), (31, 4097), ((1 << 22) - 1, 4)):
             for M in (0, 1, 63, 64, 1000, 4096):
-                assert L.bert_amd_linear_workspace(t, M, N, K) >= 0
+                assert 0 <= L.bert_amd_linear_workspace(t, M, N, K, 1) <= L.bert_amd_linear_workspace(t, M, N, K, 0)
                 for act in (0, 2):
-                    assert L.bert_amd_linear_backward_workspace(t, act, M, N, K) >= (M * N * (4 if t == 0 else 2) if act else 0)
+                    least = M * N * (4 if t == 0 else 2) if act else 0
+                    assert least <= L.bert_amd_linear_backward_workspace(t, act, M, N, K, 1) <= L.bert_amd_linear_backward_workspace(t, act, M, N, K, 0)
     for n in (0, 1, 4096, 4097, 1 << 28):
         for V in (1, 511, 512, 1 << 30):
             assert L.bert_amd_lookup_grad_workspace(n, V, 8) >= 0
