@@ -543,36 +543,45 @@ struct Plan {
     int splits = 1;
     int64_t per = 0;    // k of a split
 };
-// The tile and split whose estimated time is least: rounds of workgroups over
-// the chip times (stages of k times a stage's time, and the time around them),
-// and where k is split the pass that joins the parts (written and read once).
-// A stage's time and the time around, in us, as measured on large products:
-// 256 x 256 tiles, one on a CU; 128 x 128, two; 64 x 64, four.
+// The tile and split whose estimated time is least.  A CU's share of the
+// workgroups runs in rounds of as many as it holds; a round takes its stages'
+// time and a time around them, and where k is split its parts are joined by
+// another pass (8 bytes a sum and part, at the rate of a copy).  A stage takes
+// `alone` us where a CU has one workgroup, else `shared` us of the CU for each.
+// The numbers are fitted to products of 16 .. 65536 rows, 384 .. 4096 wide, in
+// every tile and up to 64 parts (us a call): f32 4096 x 1024 x 1024 75 in 128
+// wide tiles, 76 in 64 wide, 92 in two parts of k; bf16 16384 x 1024 x 1024 37
+// in 256 wide, 40 in 128, 59 in 64; bf16 1536 x 384 over k = 65536 123 in 21
+// parts of 256 wide tiles, 549 unsplit in 64 wide.  The choice was on average
+// 2 % off the best measured.
 Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
+    struct Form {
+        int tile;
+        double alone, shared, around;
+        int holds;
+    };
+    static const Form half[] = {{256, 1.8, 1.8, 7, 1}, {128, .76, .53, 4, 2}, {64, .5, .21, 3, 4}};
+    static const Form f32[] = {{128, 2.15, 1.95, 4, 2}, {64, 1.3, .64, 3, 4}};
+    const bool wide = type == BERT_AMD_F32;
+    const int sk = wide ? 32 : 64;
     Plan best;
-    const struct { int tile, wgs; double stage, around; } forms[] = {
-        {256, 256, 1.7, 6}, {128, 512, 1.05, 4}, {64, 1024, 0.8, 3}};
     double least = 1e30;
-    for (const auto &f : forms) {
-#ifdef FORCE_TILE
-        if (f.tile != FORCE_TILE) continue;
-#endif
-        if (type == BERT_AMD_F32 && f.tile == 256) continue;
-        const double slower = type == BERT_AMD_F32 ? 4 : 1;  // f32 products run at an eighth of the rate, on half the k
+    for (int i = 0; i < (wide ? 2 : 3); i++) {
+        const Form &f = wide ? f32[i] : half[i];
         const int64_t tiles = ceil_div<int64_t>(M, f.tile) * ceil_div<int64_t>(N, f.tile);
-        const int sk = type == BERT_AMD_F32 ? 32 : 64;
-        for (int splits = 1; splits <= 64; splits *= 2) {
-            if (splits > 1 && (K < splits * 2 * sk || tiles * splits > 2 * f.wgs)) break;
-#ifdef FORCE_SPLITS
-            if (splits != FORCE_SPLITS && K >= FORCE_SPLITS*2*sk) continue;
-#endif
-            const int64_t per = std::max<int64_t>(64, ceil_div(ceil_div<int64_t>(K, splits), (int64_t)64) * 64);
-            const double join = splits > 1 ? 5 + 8e-6 / 4 * splits * M * N : 0;
-            const double t = ceil_div<int64_t>(tiles * splits, f.wgs) * (ceil_div<int64_t>(per, sk) * f.stage * slower + f.around) + join;
-            if (t < least) least = t, best.tile = f.tile, best.splits = splits, best.per = per;
+        if (!tiles) continue;
+        const int64_t splits[] = {1, 2, 4, 6, 8, 12, 16, 256 / tiles, 512 / tiles, 768 / tiles};
+        for (const int64_t n : splits) {
+            if (n < 1 || (n > 1 && (n > 64 || K < n * sk * 2 || tiles * n > 1600))) continue;
+            const int64_t per = std::max<int64_t>(64, ceil_div(ceil_div(K, n), (int64_t)64) * 64), parts = ceil_div(K, per);
+            const int64_t each = ceil_div(tiles * parts, (int64_t)256), left = each % f.holds;
+            const double stages = (double)ceil_div(per, (int64_t)sk);
+            const auto round = [&](int64_t wgs) { return stages * std::max(f.alone, wgs * f.shared) + f.around; };
+            const double t = each / f.holds * round(f.holds) + (left ? round(left) : 0) + (parts > 1 ? 3 + 2e-6 * parts * M * N : 0);
+            if (t < least) least = t, best.tile = f.tile, best.splits = (int)parts, best.per = per;
         }
     }
-    best.splits = (int)std::max<int64_t>(1, ceil_div(K, best.per));  // rounding the parts up may leave the last ones empty
+    best.splits = std::max(1, best.splits);
     return best;
 }
 // bytes of a product's split sums
