@@ -117,13 +117,20 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Operand X, Operand W, int
 // A matrix whose rows are not aligned, or no whole chunks long, is copied into
 // the workspace with zeros up to the next chunk: one more pass over it, where
 // loads of single elements would slow the whole product down.
+struct Packing {
+    const void *from = nullptr;
+    void *to = nullptr;
+    int64_t ld = 0, rows = 0, cols = 0, ldt = 0;
+};
+// one or two matrices (blockIdx.y)
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T *from, int64_t ld, int64_t rows, int64_t cols, T *to, int64_t ldt) {
+__global__ __launch_bounds__(256) void pack_kernel(Packing a, Packing b) {
     constexpr int CH = 16 / sizeof(T);
-    const int64_t chunks = ldt / CH;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
+    const Packing &p = blockIdx.y ? b : a;
+    const int64_t chunks = p.ldt / CH;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.rows * chunks; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / chunks, c = (i - r * chunks) * CH;
-        *(u32x4 *)(to + r * ldt + c) = __builtin_bit_cast(u32x4, load_chunk<T, CH>(from, ld, false, r, c, rows, cols));
+        *(u32x4 *)((T *)p.to + r * p.ldt + c) = __builtin_bit_cast(u32x4, load_chunk<T, CH>((const T *)p.from, p.ld, false, r, c, p.rows, p.cols));
     }
 }
 
@@ -150,9 +157,9 @@ __global__ __launch_bounds__(256) void pack_kernel(const T *from, int64_t ld, in
 // The second matrix is the matrix instruction's row operand, so that a lane
 // holds 4 consecutive columns of one row of C at a time.  The finished sums go
 // through LDS, 64 columns of each wave's tile at a time, for whole 128-byte
-// row pieces on the way out.  One wave a SIMD has nothing to hide latencies
-// behind there, so inside the matrix several rows' reads, loads and stores go
-// together without a branch between them.
+// row pieces on the way out.  One or two waves a SIMD have little to hide
+// latencies behind there, so inside the matrix several rows' reads, loads and
+// stores go together without a branch between them.
 constexpr uint32_t OUTSIDE = 0x80000000u;       // an offset past every descriptor's range (2^31 bytes)
 
 // until at most LEFT of this wave's loads are on their way
@@ -305,23 +312,37 @@ __device__ __forceinline__ void store_edge(const Epilogue &e, int64_t m, int64_t
 // LDS row of the epilogue: a wave's 64 columns and 16 bytes more, so that the rows of a write start in different banks
 constexpr int OUT_LD = 68;
 
+// C = A B^T as a launch has it: tiles times parts of k workgroups
+struct Product {
+    Operand A, B;
+    int64_t M = 0, N = 0, K = 0, per = 0;  // per: k of a part
+    int tiles = 0, parts = 1;
+    float *part = nullptr;                 // where the parts' sums go; else through `e`
+    Epilogue e;
+    bool vec = false;                      // the epilogue's rows are aligned
+};
+
+// `block` of p.tiles, part `split` of k
 template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_kernel(Operand A, Operand B, int64_t M, int64_t N, int64_t K,
-                                                                  int64_t k_per_split, float *part, Epilogue e, bool vec) {
+__device__ __forceinline__ void stage_product(const Product &p, char *smem, int block, int split) {
     typedef typename Elem<TYPE>::T T;
+    const Operand A = p.A, B = p.B;
+    const int64_t M = p.M, N = p.N, K = p.K;
+    float *part = p.part;
+    const Epilogue e = p.e;
+    const bool vec = p.vec;
     constexpr int NT = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
     static_assert(BN / WN % 64 == 0, "the epilogue takes 64 columns of a wave's tile at a time");
     typedef Tile<TYPE, TA, BM, NT> TileA;
     typedef Tile<TYPE, TBT, BN, NT> TileB;
     constexpr int STAGE = TileA::BYTES + TileB::BYTES;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
     // workgroups of one XCD take neighbouring tiles, 8 tile rows at a time: they share operand rows in its L2
     const int tm = (int)ceil_div<int64_t>(M, BM), tn = (int)ceil_div<int64_t>(N, BN), all = tm * tn;
-    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const int xcd = block & 7, slot = block >> 3;
     const int tile = xcd * (all >> 3) + min(xcd, all & 7) + slot;
     const int group = tile / (8 * tn), in_group = tile - group * 8 * tn, high = min(8, tm - 8 * group);
     const int64_t m0 = (int64_t)(8 * group + in_group % high) * BM, n0 = (int64_t)(in_group / high) * BN;
-    const int64_t ka = (int64_t)blockIdx.z * k_per_split, kb = min(K, ka + k_per_split);
+    const int64_t ka = split * p.per, kb = min(K, ka + p.per);
     TileA ta;
     TileB tb;
     ta.init(A, m0, M, ka);
@@ -384,23 +405,24 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_ker
     wait_reads();
     wait_loads<0>();
     barrier();  // the stages' last loads and reads are done: the LDS is the epilogue's
-    constexpr int WR = BM / WM, G = sizeof(T) == 4 ? 2 : 4;
+    constexpr int WR = std::min(BM / WM, 64), PARTS = BM / WM / WR, G = std::min(WR / 8, sizeof(T) == 4 ? 2 : 4);
     float *out = (float *)smem + wave * WR * OUT_LD;
     const int row0 = lane >> 3, col = 8 * (lane & 7);
 #pragma unroll 1
-    for (int half = 0; half < TN / 2; half++) {
-        const int64_t n = n0 + wn + 64 * half + col, m = m0 + wm + row0;
+    for (int pass = 0; pass < TN / 2 * PARTS; pass++) {
+        const int half = pass / PARTS, rows = pass % PARTS;
+        const int64_t n = n0 + wn + 64 * half + col, m = m0 + wm + WR * rows + row0;
         float bias[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) bias[i] = half ? biases[1 % (TN / 2)][i] : biases[0][i];
 #pragma unroll
         for (int j = 0; j < TN; j++)
-            if (j / 2 == half)
 #pragma unroll
-                for (int i = 0; i < TM; i++)
+            for (int i = 0; i < TM; i++)
+                if (j / 2 == half && 32 * i / WR == rows)
 #pragma unroll
                     for (int c = 0; c < 4; c++)
-                        *(f32x4 *)(out + (32 * i + (lane & 31)) * OUT_LD + 32 * (j & 1) + 8 * c + 4 * (lane >> 5)) =
+                        *(f32x4 *)(out + (32 * i % WR + (lane & 31)) * OUT_LD + 32 * (j & 1) + 8 * c + 4 * (lane >> 5)) =
                             f32x4{acc[i][j][4 * c], acc[i][j][4 * c + 1], acc[i][j][4 * c + 2], acc[i][j][4 * c + 3]};
         if (vec && !part && m0 + BM <= M && n0 + BN <= N) {
             const T *r = (const T *)e.r + m * e.ldr + n;
@@ -429,7 +451,7 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_ker
 #pragma unroll
                 for (int c = 0; c < 8; c++) v[c] = out[(g + row0) * OUT_LD + col + c] + bias[c];
                 if (part) {
-                    float *q = part + ((int64_t)blockIdx.z * M + m + g) * N + n;
+                    float *q = part + (split * M + m + g) * N + n;
                     if (N % 4 == 0 && n + 8 <= N) put8(q, v);
                     else
 #pragma unroll
@@ -443,12 +465,33 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? 1 : 2) void stage_gemm_ker
     }
 }
 
+template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Product p) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    stage_product<TYPE, TA, TBT, BM, BN, WM, WN>(p, smem, blockIdx.x, blockIdx.z);
+}
+
+// Both products of a small layer's gradients at once, 64 x 64 tiles: each alone
+// leaves most of the chip idle, and a launch less counts there.
+template <int TYPE>
+__global__ __launch_bounds__(128, 2) void pair_gemm_kernel(Product dx, Product dw) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int first = dx.tiles * dx.parts, b = blockIdx.x;
+    if (b < first)
+        stage_product<TYPE, false, true, 64, 64, 2, 1>(dx, smem, b % dx.tiles, b / dx.tiles);
+    else
+        stage_product<TYPE, true, true, 64, 64, 2, 1>(dw, smem, (b - first) % dw.tiles, (b - first) / dw.tiles);
+}
+
+// the parts of one or two products (blockIdx.y) added in order
 template <typename T>
-__global__ __launch_bounds__(256) void split_join_kernel(const float *part, int splits, int64_t M, int64_t N, Epilogue e) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * N; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void split_join_kernel(Product a, Product b) {
+    const Product &p = blockIdx.y ? b : a;
+    if (!p.part) return;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.M * p.N; i += (int64_t)gridDim.x * 256) {
         float v = 0.f;
-        for (int s = 0; s < splits; s++) v += part[s * M * N + i];
-        epilogue_store<T>(e, i / N, i % N, v);
+        for (int s = 0; s < p.parts; s++) v += p.part[s * p.M * p.N + i];
+        epilogue_store<T>(p.e, i / p.N, i % p.N, v);
     }
 }
 
@@ -590,6 +633,12 @@ int64_t split_bytes(int type, int64_t M, int64_t N, int64_t K) {
     return p.splits > 1 ? round256(p.splits * M * N * 4) : 0;
 }
 
+// whether a layer's two gradient products share a launch: both in 64 x 64 tiles
+// (256 x 384 x 384 in f32 29 -> 21 us for all three gradients)
+bool gradients_in_pair(int type, int64_t M, int64_t N, int64_t K) {
+    return M > 0 && plan_for(type, M, K, N).tile == 64 && plan_for(type, N, K, M).tile == 64;
+}
+
 int64_t padded(int type, int64_t n) {
     const int64_t ch = 16 / elem_size(type);
     return (n + ch - 1) / ch * ch;
@@ -601,23 +650,44 @@ bool whole_rows(const Operand &o, int type, int64_t cols) {
     return o.padded || (o.vec && cols % (16 / elem_size(type)) == 0 && o.ld < (1 << 21));
 }
 
-// `o` as the stage kernel takes it; a copy goes to `ws`, which moves on
+// one or two matrices with rows of `cols` as the stage kernel takes them; copies go to `ws`, which moves on
 template <typename T>
-Operand pack(const Operand &o, int type, int64_t rows, int64_t cols, char *&ws, hipStream_t s) {
-    if (whole_rows(o, type, cols)) return o;
-    const int64_t ld = padded(type, cols), chunks = rows * ld * (int64_t)sizeof(T) / 16;
-    const Operand to = {ws, ld, true, true};
-    if (chunks)
-        hipLaunchKernelGGL((pack_kernel<T>), dim3(std::min<int64_t>(1 << 14, ceil_div<int64_t>(chunks, 256))), dim3(256), 0, s, (const T *)o.p,
-                           o.ld, rows, cols, (T *)ws, ld);
-    ws += packed_bytes(type, rows, cols);
-    return to;
+hipError_t pack(int type, Operand *o, const int64_t *rows, int n, int64_t cols, char *&ws, hipStream_t s) {
+    Packing p[2];
+    int64_t most = 0;
+    int count = 0;
+    for (int i = 0; i < n; i++) {
+        if (whole_rows(o[i], type, cols)) continue;
+        const int64_t ld = padded(type, cols);
+        p[count++] = {o[i].p, ws, o[i].ld, rows[i], cols, ld};
+        o[i] = {ws, ld, true, true};
+        most = std::max(most, rows[i] * ld * (int64_t)sizeof(T) / 16);
+        ws += packed_bytes(type, rows[i], cols);
+    }
+    if (!most) return hipSuccess;
+    hipLaunchKernelGGL((pack_kernel<T>), dim3(std::min<int64_t>(1 << 14, ceil_div<int64_t>(most, 256)), count), dim3(256), 0, s, p[0], p[1]);
+    return hipGetLastError();
+}
+
+template <int TYPE>
+Product product(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, const Plan &plan, void *ws, const Epilogue &e) {
+    const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(typename Elem<TYPE>::T)); };
+    Product p;
+    p.A = A, p.B = B, p.M = M, p.N = N, p.K = K, p.per = plan.per, p.parts = plan.splits;
+    p.tiles = (int)(ceil_div<int64_t>(M, plan.tile) * ceil_div<int64_t>(N, plan.tile));
+    p.part = plan.splits > 1 ? (float *)ws : nullptr;
+    p.e = e;
+    p.vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr);
+    return p;
+}
+
+constexpr int stage_lds(int BM, int BN, int WM, int WN) {
+    return std::max(2 * (BM + BN) * 128, std::min(BM / WM, 64) * WM * WN * OUT_LD * 4);
 }
 
 template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
-hipError_t launch_stage(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, const Plan &p, float *part, const Epilogue &e,
-                        bool vec, hipStream_t s) {
-    constexpr int lds = std::max(2 * (BM + BN) * 128, BM * WN * OUT_LD * 4);
+hipError_t launch_stage(const Product &p, hipStream_t s) {
+    constexpr int lds = stage_lds(BM, BN, WM, WN);
     const auto k = stage_gemm_kernel<TYPE, TA, TBT, BM, BN, WM, WN>;
     if (lds > 65536) {  // beyond a launch's default: asked for once on each device
         static std::atomic<uint64_t> asked{0};
@@ -629,26 +699,28 @@ hipError_t launch_stage(const Operand &A, const Operand &B, int64_t M, int64_t N
             asked.fetch_or(bit, std::memory_order_relaxed);
         }
     }
-    const int64_t tiles = ceil_div<int64_t>(M, BM) * ceil_div<int64_t>(N, BN);
-    hipLaunchKernelGGL(k, dim3(tiles, 1, p.splits), dim3(WM * WN * 64), lds, s, A, B, M, N, K, p.per, part, e, vec);
+    hipLaunchKernelGGL(k, dim3(p.tiles, 1, p.parts), dim3(WM * WN * 64), lds, s, p);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t join(const Product &a, const Product &b, hipStream_t s) {
+    const int64_t most = std::max(a.part ? a.M * a.N : 0, b.part ? b.M * b.N : 0);
+    if (!most) return hipSuccess;
+    hipLaunchKernelGGL((split_join_kernel<T>), dim3(std::min<int64_t>(1024, ceil_div<int64_t>(most, 256)), b.part ? 2 : 1), dim3(256), 0, s, a, b);
     return hipGetLastError();
 }
 
 // C = A B^T of two matrices in whole chunks
 template <int TYPE, bool TA, bool TBT>
 hipError_t gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, void *ws, const Epilogue &e, hipStream_t s) {
-    typedef typename Elem<TYPE>::T T;
-    const Plan p = plan_for(TYPE, M, N, K);
-    float *part = p.splits > 1 ? (float *)ws : nullptr;
-    const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(T)); };
-    const bool vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr);
+    const Plan plan = plan_for(TYPE, M, N, K);
+    const Product p = product<TYPE>(A, B, M, N, K, plan, ws, e);
     hipError_t r = hipSuccess;
-    if (p.tile == 64) r = launch_stage<TYPE, TA, TBT, 64, 64, 2, 1>(A, B, M, N, K, p, part, e, vec, s);
-    else if (p.tile == 128) r = launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
-    else if constexpr (TYPE != BERT_AMD_F32) r = launch_stage<TYPE, TA, TBT, 256, 256, 2, 2>(A, B, M, N, K, p, part, e, vec, s);
-    if (r != hipSuccess || !part) return r;
-    hipLaunchKernelGGL((split_join_kernel<T>), dim3(std::min<int64_t>(1024, ceil_div<int64_t>(M * N, 256))), dim3(256), 0, s, part, p.splits, M, N, e);
-    return hipGetLastError();
+    if (plan.tile == 64) r = launch_stage<TYPE, TA, TBT, 64, 64, 2, 1>(p, s);
+    else if (plan.tile == 128) r = launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(p, s);
+    else if constexpr (TYPE != BERT_AMD_F32) r = launch_stage<TYPE, TA, TBT, 256, 256, 2, 4>(p, s);
+    return r != hipSuccess ? r : join<typename Elem<TYPE>::T>(p, Product(), s);
 }
 
 Operand operand(const void *p, int64_t ld, int type) { return {p, ld, aligned16(p, ld * elem_size(type))}; }
@@ -672,8 +744,10 @@ hipError_t linear_t(const LinearArgs &a, hipStream_t s) {
     if (a.M <= FEW_ROWS)  // one column a wave fills the chip sooner, four read x a quarter as often
         return a.N < 4096 ? few_rows<TYPE, 1>(x, w, a, e, s) : few_rows<TYPE, 4>(x, w, a, e, s);
     char *ws = (char *)a.ws;
-    const Operand px = pack<T>(x, TYPE, a.M, a.K, ws, s), pw = pack<T>(w, TYPE, a.N, a.K, ws, s);
-    return gemm<TYPE, false, false>(px, pw, a.M, a.N, a.K, ws, e, s);
+    Operand both[] = {x, w};
+    const int64_t rows[] = {a.M, a.N};
+    if (hipError_t r = pack<T>(TYPE, both, rows, 2, a.K, ws, s); r != hipSuccess) return r;
+    return gemm<TYPE, false, false>(both[0], both[1], a.M, a.N, a.K, ws, e, s);
 }
 
 template <int TYPE>
@@ -706,21 +780,32 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
     } else if (a.db) {
         hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 32)), dim3(256), 0, s, (const float *)nullptr, (int64_t)0, (int64_t)a.N, a.db);
     }
+    Epilogue ex, ew;
+    ex.y = a.dx, ex.ldy = a.lddx;
+    ew.y = a.dw, ew.ldy = a.lddw;
+    if (a.dx && a.dw && gradients_in_pair(TYPE, a.M, a.N, a.K)) {
+        Operand wx[] = {operand(a.w, a.ldw, TYPE), operand(a.x, a.ldx, TYPE)};
+        const int64_t rows[] = {a.N, a.M};
+        if (hipError_t r = pack<T>(TYPE, wx, rows, 2, a.K, ws, s); r != hipSuccess) return r;
+        const Product dx = product<TYPE>(dz, wx[0], a.M, a.K, a.N, plan_for(TYPE, a.M, a.K, a.N), ws, ex);
+        ws += split_bytes(TYPE, a.M, a.K, a.N);
+        const Product dw = product<TYPE>(dz, wx[1], a.N, a.K, a.M, plan_for(TYPE, a.N, a.K, a.M), ws, ew);
+        hipLaunchKernelGGL((pair_gemm_kernel<TYPE>), dim3(dx.tiles * dx.parts + dw.tiles * dw.parts), dim3(128), stage_lds(64, 64, 2, 1), s, dx, dw);
+        if (hipError_t r = hipGetLastError(); r != hipSuccess) return r;
+        return join<T>(dx, dw, s);
+    }
     if (a.dx && a.M) {
-        Epilogue e;
-        e.y = a.dx;
-        e.ldy = a.lddx;
         char *rest = ws;
-        const Operand w = pack<T>(operand(a.w, a.ldw, TYPE), TYPE, a.N, a.K, rest, s);
-        if (hipError_t r = gemm<TYPE, false, true>(dz, w, a.M, a.K, a.N, rest, e, s); r != hipSuccess) return r;
+        Operand w = operand(a.w, a.ldw, TYPE);
+        const int64_t rows = a.N;
+        if (hipError_t r = pack<T>(TYPE, &w, &rows, 1, a.K, rest, s); r != hipSuccess) return r;
+        if (hipError_t r = gemm<TYPE, false, true>(dz, w, a.M, a.K, a.N, rest, ex, s); r != hipSuccess) return r;
     }
     if (a.dw) {
-        Epilogue e;
-        e.y = a.dw;
-        e.ldy = a.lddw;
         char *rest = ws;
-        const Operand x = pack<T>(operand(a.x, a.ldx, TYPE), TYPE, a.M, a.K, rest, s);
-        if (hipError_t r = gemm<TYPE, true, true>(dz, x, a.N, a.K, a.M, rest, e, s); r != hipSuccess) return r;
+        Operand x = operand(a.x, a.ldx, TYPE);
+        if (hipError_t r = pack<T>(TYPE, &x, &a.M, 1, a.K, rest, s); r != hipSuccess) return r;
+        if (hipError_t r = gemm<TYPE, true, true>(dz, x, a.N, a.K, a.M, rest, ew, s); r != hipSuccess) return r;
     }
     return hipGetLastError();
 }
@@ -743,9 +828,10 @@ hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
 
 int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K, bool aligned) {
     const bool whole_n = aligned && padded(type, N) == N, whole_k = aligned && padded(type, K) == K;
+    const int64_t for_dx = (whole_k ? 0 : packed_bytes(type, N, K)) + split_bytes(type, M, K, N);
+    const int64_t for_dw = (whole_k ? 0 : packed_bytes(type, M, K)) + split_bytes(type, N, K, M);
     return (act || !whole_n ? packed_bytes(type, M, N) : 0) + round256(ceil_div<int64_t>(M, dz_rows(M, N)) * N * 4) +
-           std::max((whole_k ? 0 : packed_bytes(type, N, K)) + split_bytes(type, M, K, N),
-                    (whole_k ? 0 : packed_bytes(type, M, K)) + split_bytes(type, N, K, M));
+           (gradients_in_pair(type, M, N, K) ? for_dx + for_dw : std::max(for_dx, for_dw));
 }
 
 hipError_t launch_linear_grad(const LinearGradArgs &a, hipStream_t s) {
