@@ -17,7 +17,9 @@ OPS_OBJS := $(BUILD)/obj/ops_linear.o $(BUILD)/obj/ops_rows.o $(BUILD)/obj/ops_a
 SRC_HASH_FILES := $(sort $(wildcard $(SRC)/*.hip $(SRC)/*.cpp $(SRC)/*.h $(SRC)/*.inc include/*.h include/ggml/*.h)) Makefile
 CXXFLAGS := -O2 -std=c++17 -fPIC -fvisibility=hidden -ffp-contract=off -Wall -Wno-unused-function -Wno-unused-result \
             -D__HIP_PLATFORM_AMD__ -I/opt/rocm/include $(INC)
-HIPFLAGS := -O3 -std=c++17 -fno-slp-vectorize -mllvm -amdgpu-mfma-vgpr-form -Wno-unused-value -Wno-unused-result -fPIC -fvisibility=hidden -ffp-contract=off --offload-arch=$(ARCH) $(INC)
+# no packed f32 instructions (v_pk_add / mul / fma_f32): measured 1.3 % faster on the headline batch without them, bitwise the same
+NO_PACKED := -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS := $(NO_PACKED) -O3 -std=c++17 -fno-slp-vectorize -mllvm -amdgpu-mfma-vgpr-form -Wno-unused-value -Wno-unused-result -fPIC -fvisibility=hidden -ffp-contract=off --offload-arch=$(ARCH) $(INC)
 
 all: $(BUILD)/libbert.so $(BUILD)/div_check $(BUILD)/qkva_check $(BUILD)/mfma_bf16_split_probe $(BUILD)/tok_bench
 
@@ -31,9 +33,8 @@ $(BUILD)/obj/%.o: $(SRC)/%.hip $(SRC)/kernels.h $(SRC)/kernels_common.h $(SRC)/i
 	@mkdir -p $(dir $@)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
-# the operators are built without the packed f32 instructions, and with the matrix units'
-# sums where the compiler puts them (256 of them beside 113 other registers a lane)
-OPSFLAGS := $(filter-out -mllvm -amdgpu-mfma-vgpr-form,$(HIPFLAGS)) -Xclang -target-feature -Xclang -packed-fp32-ops
+# the operators are built with the matrix units' sums where the compiler puts them
+OPSFLAGS := $(filter-out -mllvm -amdgpu-mfma-vgpr-form,$(HIPFLAGS))
 $(BUILD)/obj/ops_%.o: $(SRC)/ops_%.hip $(SRC)/ops.h $(SRC)/ops_common.h include/bert_amd.h
 	@mkdir -p $(dir $@)
 	$(HIPCC) $(OPSFLAGS) -c $< -o $@
@@ -62,12 +63,12 @@ $(BUILD)/gemm_bench: tools/gemm_bench.hip embedding.cpp_amd/csrc/kernels.hip emb
 # device check that the short Q8 scale divisions equal IEEE division (tests/test_gpu_parity.py)
 $(BUILD)/div_check: tools/div_check.hip
 	@mkdir -p $(BUILD)
-	$(HIPCC) -O3 --offload-arch=$(ARCH) -Wno-unused-value -Wno-unused-result $< -o $@
+	$(HIPCC) $(NO_PACKED) -O3 --offload-arch=$(ARCH) -Wno-unused-value -Wno-unused-result $< -o $@
 
 # device probe of the bf16 partial-product scale products (tests/test_gpu_parity.py)
 $(BUILD)/mfma_bf16_split_probe: tools/mfma_bf16_split_probe.hip
 	@mkdir -p $(BUILD)
-	$(HIPCC) -O3 --offload-arch=$(ARCH) $< -o $@
+	$(HIPCC) $(NO_PACKED) -O3 --offload-arch=$(ARCH) $< -o $@
 
 # host-only tokenizer timing (development; DESIGN.md §6 consumer line)
 $(BUILD)/tok_bench: tools/tok_bench.cpp $(BUILD)/obj/gguf_io.o $(BUILD)/obj/tokenizer.o
@@ -115,7 +116,7 @@ $(BUILD)/qkva_time: tools/qkva_time.hip $(SRC)/kernels.hip $(SRC)/kernels.h $(SR
 # FETCH_SIZE / WRITE_SIZE calibration per access width (tools/pmc_calib.hip)
 $(BUILD)/pmc_calib: tools/pmc_calib.hip
 	@mkdir -p $(BUILD)
-	$(HIPCC) -O3 --offload-arch=gfx950 $< -o $@
+	$(HIPCC) $(NO_PACKED) -O3 --offload-arch=gfx950 $< -o $@
 
 # development per-phase stamps of the persistent int8 GEMMs (tools/phase_stamps.hip)
 $(BUILD)/phase_stamps: tools/phase_stamps.hip $(SRC)/gemm_i8.hip $(SRC)/kernels.h $(SRC)/kernels_common.h $(SRC)/i8_core.h
