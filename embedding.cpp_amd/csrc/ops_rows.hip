@@ -135,22 +135,58 @@ hipError_t lookup_t(const LookupArgs &a, hipStream_t s) {
 // before it in its tile with the same digit.  No atomic's order enters the
 // result, so the sums below have one order.  Places without a gradient (ids
 // outside the table, the padding token) get the key V and sort last.
+//
+// These launches wait for memory more than they move, so other workgroups of
+// theirs write the zeros of the rows that have no place (most of a table's
+// gradient): the first one clears the rows' marks, the second one's others set
+// them from the ids, the following ones' write.
 constexpr int TILE = 1024, BINS = 512;
 
 __device__ __forceinline__ int sort_key(int id, int V, int pad) { return id >= 0 && id < V && id != pad ? id : V; }
+
+// Rows first .. end - 1 of the gradient that no place belongs to, as zeros, by
+// `groups` workgroups of which this is number `g`; `used` marks the others.
+struct ZeroPart {
+    float *dtable = nullptr;
+    int64_t ldt = 0;
+    int E = 0, first = 0, end = 0;
+    const uint8_t *used = nullptr;
+    bool four = false;  // rows are whole aligned float4s
+};
+constexpr int ZERO_ROWS = 16;
+
+__device__ __forceinline__ void zero_rows(const ZeroPart &z, int first, const uint8_t *used /* of row `first` on */) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    static_assert(ZERO_ROWS <= 64, "a lane looks at one row's mark");
+    const bool mine = lane < ZERO_ROWS && first + lane < z.end;
+    const uint64_t unused = __ballot(mine && !used[mine ? lane : 0]);
+    for (int v = first + wave; v < min(z.end, first + ZERO_ROWS); v += blockDim.x >> 6) {
+        if (!(unused >> (v - first) & 1)) continue;
+        float *row = z.dtable + (int64_t)v * z.ldt;
+        if (z.four)
+            for (int e = 4 * lane; e < z.E; e += 256) *(f32x4 *)(row + e) = f32x4{0.f, 0.f, 0.f, 0.f};
+        else
+            for (int e = lane; e < z.E; e += 64) row[e] = 0.f;
+    }
+}
+__device__ __forceinline__ void zero_part(const ZeroPart &z, int g, int groups) {
+    for (int64_t v = z.first + (int64_t)g * ZERO_ROWS; v < z.end; v += (int64_t)groups * ZERO_ROWS) zero_rows(z, (int)v, z.used + v);
+}
+inline int zero_groups(const ZeroPart &z) { return std::min(1 << 20, ceil_div(std::max(0, z.end - z.first), ZERO_ROWS)); }
 
 struct SortPass {
     const int32_t *ids;                // first pass: the caller's ids, else null
     const int32_t *key_in, *place_in;
     int32_t *key_out, *place_out;
     int32_t *hist, *total;             // [BINS][tiles], [BINS]
-    uint8_t *used;                     // first pass: cleared; last: set for each token that has a place
-    bool last;
+    uint8_t *used;                     // marks of the rows that have a place: cleared and set in the first pass
+    ZeroPart zero;                     // what this launch's other workgroups write
     int n, V, pad, tiles, shift, bits;
 };
 
 __global__ __launch_bounds__(256) void sort_hist_kernel(SortPass p) {
     __shared__ int h[BINS];
+    if ((int)blockIdx.x >= p.tiles) return zero_part(p.zero, blockIdx.x - p.tiles, gridDim.x - p.tiles);
     if (p.ids)
         for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < ceil_div(p.V, 16); i += (int64_t)gridDim.x * 256)
             ((u32x4 *)p.used)[i] = u32x4{0, 0, 0, 0};
@@ -183,6 +219,15 @@ __device__ __forceinline__ int block_scan(int v, int *sums) {
 
 __global__ __launch_bounds__(256) void sort_scan_kernel(SortPass p) {
     __shared__ int sums[4], carry;
+    const int bins = 1 << p.bits;
+    if ((int)blockIdx.x >= bins) {
+        if (!p.ids) return zero_part(p.zero, blockIdx.x - bins, gridDim.x - bins);
+        for (int64_t i = (int64_t)(blockIdx.x - bins) * 256 + threadIdx.x; i < p.n; i += (int64_t)(gridDim.x - bins) * 256) {
+            const int k = sort_key(p.ids[i], p.V, p.pad);
+            if (k < p.V) p.used[k] = 1;
+        }
+        return;
+    }
     int32_t *h = p.hist + (int64_t)blockIdx.x * p.tiles;
     if (threadIdx.x == 0) carry = 0;
     __syncthreads();
@@ -201,6 +246,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortPass p) {
     __shared__ int first[BINS];       // where this tile's places of each digit value start
     __shared__ int seen[4][BINS];     // per wave: places of each digit value so far
     __shared__ int sums[4];
+    if ((int)blockIdx.x >= p.tiles) return zero_part(p.zero, blockIdx.x - p.tiles, gridDim.x - p.tiles);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int mask = (1 << p.bits) - 1, bins = 1 << p.bits;
     for (int i = threadIdx.x; i < 4 * BINS; i += 256) (&seen[0][0])[i] = 0;
@@ -241,7 +287,6 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortPass p) {
         for (int w = 0; w < wave; w++) at += seen[w][d];
         p.key_out[at] = key[j];
         p.place_out[at] = place[j];
-        if (p.last && key[j] < p.V) p.used[key[j]] = 1;
     }
 }
 
@@ -252,10 +297,8 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortPass p) {
 // token whose places end within the tile.  A token whose places go on past a
 // tile's end leaves its sums, one row for each tile it has places in, to
 // join_kernel, which adds them in order: a frequent token's long sum is spread
-// over many workgroups.  The same launch's other workgroups write zeros into
-// the rows of tokens that have no place (bound by memory: most of a table's
-// gradient is that).
-constexpr int SUM_TILE = 64, ZERO_ROWS = 64, AHEAD = 8;
+// over many workgroups.
+constexpr int SUM_TILE = 64, AHEAD = 8;
 
 template <typename T, int COLS>
 __device__ __forceinline__ void load_cols(const T *p, float *v) {
@@ -282,19 +325,8 @@ __device__ __forceinline__ void store_row(const LookupGradArgs &a, int v, int e,
     for (int i = 0; i < COLS; i++) o[i] = a.accumulate ? o[i] + a.scale * sum[i] : a.scale * sum[i];
     store_cols<COLS>(p, o);
 }
-template <int COLS>
-__device__ __forceinline__ void zero_rows(const LookupGradArgs &a, int first, const uint8_t *used /* of row `first` on */) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int v = first + wave; v < min(a.V, first + ZERO_ROWS); v += blockDim.x >> 6) {
-        if (used[v - first]) continue;
-        const float zero[4] = {};
-        for (int e = COLS * lane; e < a.E; e += 64 * COLS) store_cols<COLS>(a.dtable + (int64_t)v * a.ldt + e, zero);
-    }
-}
-
 struct SumArgs {
     const int32_t *key, *place;
-    const uint8_t *used;
     float *part;  // [tiles][2][E]: of the token that goes on from the tile before; of the one that goes on past the end
     int tiles;
 };
@@ -302,46 +334,46 @@ struct SumArgs {
 template <int TYPE, int COLS>
 __global__ __launch_bounds__(256) void sum_kernel(LookupGradArgs a, SumArgs s) {
     typedef typename Elem<TYPE>::T T;
-    if ((int)blockIdx.x >= s.tiles) {
-        if (blockIdx.y == 0)
-            for (int64_t b = blockIdx.x - s.tiles; b * ZERO_ROWS < a.V; b += gridDim.x - s.tiles) zero_rows<COLS>(a, (int)b * ZERO_ROWS, s.used + b * ZERO_ROWS);
-        return;
-    }
-    __shared__ int key[SUM_TILE + 2], place[SUM_TILE];
-    const int n = (int)a.n, first = blockIdx.x * SUM_TILE, count = min(SUM_TILE, n - first);
-    for (int i = threadIdx.x; i < count; i += blockDim.x) key[i + 1] = s.key[first + i], place[i] = s.place[first + i];
-    if (threadIdx.x == 0) {
-        key[0] = first ? s.key[first - 1] : -1;
-        key[count + 1] = first + count < n ? s.key[first + count] : a.V;
-    }
-    __syncthreads();
+    static_assert(SUM_TILE == 64, "a lane holds one place");
+    const int lane = threadIdx.x & 63, n = (int)a.n, i = blockIdx.x * SUM_TILE + lane;
+    const int key = i < n ? s.key[i] : a.V, next = i + 1 < n ? s.key[i + 1] : a.V, place = i < n ? s.place[i] : 0;
+    const int before = blockIdx.x ? s.key[blockIdx.x * SUM_TILE - 1] : -1;
+    const int count = __popcll(__ballot(key < a.V));  // the places without a gradient are the last ones
+    const uint64_t ends = __ballot(key != next) | 1ull << (SUM_TILE - 1);
     const int e = (blockIdx.y * blockDim.x + threadIdx.x) * COLS;
     if (e >= a.E) return;
     const T *from = (const T *)a.dout + e;
+    float *part = s.part + (int64_t)blockIdx.x * 2 * a.E + e;
     float sum[COLS] = {};
-    bool from_before = key[0] == key[1];
-    for (int i = 0; i < count; i += AHEAD) {
-        if (key[i + 1] >= a.V) break;  // the places without a gradient are the last ones
-        float v[AHEAD][COLS] = {};
+    bool from_before = before == __builtin_amdgcn_readlane(key, 0);
+    float now[AHEAD][COLS], then[AHEAD][COLS];
+    const auto load = [&](float (&v)[AHEAD][COLS], int at) {  // past the last place: its row again, not used
 #pragma unroll
-        for (int j = 0; j < AHEAD; j++)
-            if (i + j < count && key[i + j + 1] < a.V) load_cols<T, COLS>(from + (int64_t)place[i + j] * a.ldd, v[j]);
+        for (int j = 0; j < AHEAD; j++) load_cols<T, COLS>(from + __builtin_amdgcn_readlane(place, min(at + j, count - 1)) * a.ldd, v[j]);
+    };
+    if (!count) return;
+    load(now, 0);
+    for (int at = 0; at < count; at += AHEAD) {
+        if (at + AHEAD < count) load(then, at + AHEAD);
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) {
-            const int k = i + j < count ? key[i + j + 1] : a.V;
-            if (k >= a.V) break;
+            if (at + j >= count) break;
 #pragma unroll
-            for (int c = 0; c < COLS; c++) sum[c] += v[j][c];
-            if (i + j == count - 1 || key[i + j + 2] != k) {
-                const bool goes_on = key[i + j + 2] == k;
-                if (from_before) store_cols<COLS>(s.part + ((int64_t)blockIdx.x * 2) * a.E + e, sum);
-                else if (goes_on) store_cols<COLS>(s.part + ((int64_t)blockIdx.x * 2 + 1) * a.E + e, sum);
+            for (int c = 0; c < COLS; c++) sum[c] += now[j][c];
+            if (ends >> (at + j) & 1) {
+                const int k = __builtin_amdgcn_readlane(key, at + j);
+                if (from_before) store_cols<COLS>(part, sum);
+                else if (__builtin_amdgcn_readlane(next, at + j) == k) store_cols<COLS>(part + a.E, sum);
                 else store_row<COLS>(a, k, e, sum);
                 from_before = false;
 #pragma unroll
                 for (int c = 0; c < COLS; c++) sum[c] = 0.f;
             }
         }
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++)
+#pragma unroll
+            for (int c = 0; c < COLS; c++) now[j][c] = then[j][c];
     }
 }
 
@@ -396,7 +428,7 @@ __global__ __launch_bounds__(256) void join_kernel(LookupGradArgs a, SumArgs s) 
 constexpr int FEW = 4096;
 
 template <int TYPE, int COLS>
-__global__ __launch_bounds__(256) void few_kernel(LookupGradArgs a) {
+__global__ __launch_bounds__(256) void few_kernel(LookupGradArgs a, ZeroPart z) {
     typedef typename Elem<TYPE>::T T;
     const int n = (int)a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if ((int)blockIdx.x >= n) {
@@ -412,7 +444,7 @@ __global__ __launch_bounds__(256) void few_kernel(LookupGradArgs a) {
                 if (id >= first && id < first + ZERO_ROWS && id != a.pad_id) used[id - first] = 1;
             }
             __syncthreads();
-            zero_rows<COLS>(a, first, used);
+            zero_rows(z, first, used);
         }
         return;
     }
@@ -484,23 +516,18 @@ int64_t lookup_grad_ws_bytes(int64_t n, int V, int E) {
 
 namespace {
 
-// workgroups beside the sums' that write zeros: all of a large table's rows at once, as far as a launch goes
-int zero_groups(const LookupGradArgs &a) {
-    return a.accumulate ? 0 : (int)std::min<int64_t>(1 << 20, ceil_div(a.V, ZERO_ROWS));
-}
-
 template <int TYPE, int COLS>
 hipError_t sum_t(const LookupGradArgs &a, const SumArgs &p, hipStream_t s) {
     const int threads = std::min(256, ceil_div(ceil_div(a.E, COLS), 64) * 64);
     const int across = ceil_div(ceil_div(a.E, COLS), threads);
-    hipLaunchKernelGGL((sum_kernel<TYPE, COLS>), dim3(p.tiles + zero_groups(a), across), dim3(threads), 0, s, a, p);
+    hipLaunchKernelGGL((sum_kernel<TYPE, COLS>), dim3(p.tiles, across), dim3(threads), 0, s, a, p);
     hipLaunchKernelGGL((join_kernel<COLS>), dim3(p.tiles, ceil_div(a.E, 64 * COLS)), dim3(256), 0, s, a, p);
     return hipGetLastError();
 }
 template <int TYPE, int COLS>
-hipError_t few_t(const LookupGradArgs &a, hipStream_t s) {
-    const int groups = (int)a.n + zero_groups(a);
-    if (groups) hipLaunchKernelGGL((few_kernel<TYPE, COLS>), dim3(groups), dim3(256), 0, s, a);
+hipError_t few_t(const LookupGradArgs &a, const ZeroPart &z, hipStream_t s) {
+    const int groups = (int)a.n + zero_groups(z);
+    if (groups) hipLaunchKernelGGL((few_kernel<TYPE, COLS>), dim3(groups), dim3(256), 0, s, a, z);
     return hipGetLastError();
 }
 // four columns a thread where rows and places allow it
@@ -513,11 +540,14 @@ bool four_columns(const LookupGradArgs &a) {
 
 hipError_t launch_lookup_grad(const LookupGradArgs &a, hipStream_t s) {
     const bool four = four_columns(a);
+    ZeroPart zero;
+    zero.dtable = a.dtable, zero.ldt = a.ldt, zero.E = a.E, zero.end = a.accumulate ? 0 : a.V;
+    zero.four = a.E % 4 == 0 && aligned16(a.dtable, a.ldt * 4);
     if (a.n <= FEW) {
         switch (a.type) {
-            case BERT_AMD_F32: return four ? few_t<BERT_AMD_F32, 4>(a, s) : few_t<BERT_AMD_F32, 1>(a, s);
-            case BERT_AMD_F16: return four ? few_t<BERT_AMD_F16, 4>(a, s) : few_t<BERT_AMD_F16, 1>(a, s);
-            default: return four ? few_t<BERT_AMD_BF16, 4>(a, s) : few_t<BERT_AMD_BF16, 1>(a, s);
+            case BERT_AMD_F32: return four ? few_t<BERT_AMD_F32, 4>(a, zero, s) : few_t<BERT_AMD_F32, 1>(a, zero, s);
+            case BERT_AMD_F16: return four ? few_t<BERT_AMD_F16, 4>(a, zero, s) : few_t<BERT_AMD_F16, 1>(a, zero, s);
+            default: return four ? few_t<BERT_AMD_BF16, 4>(a, zero, s) : few_t<BERT_AMD_BF16, 1>(a, zero, s);
         }
     }
     char *ws = (char *)a.ws;
@@ -534,7 +564,6 @@ hipError_t launch_lookup_grad(const LookupGradArgs &a, hipStream_t s) {
     p.total = (int32_t *)take(BINS * 4);
     p.used = (uint8_t *)take((int64_t)a.V + 16);
     SumArgs q = {};
-    q.used = p.used;
     q.part = (float *)take(ceil_div<int64_t>(a.n, SUM_TILE) * 2 * a.E * 4);
     q.tiles = (int)ceil_div<int64_t>(a.n, SUM_TILE);
     int key_bits = 1;
@@ -542,16 +571,30 @@ hipError_t launch_lookup_grad(const LookupGradArgs &a, hipStream_t s) {
     const int passes = ceil_div(key_bits, 9);
     p.n = (int)a.n, p.V = a.V, p.pad = a.pad_id, p.tiles = tiles;
     p.bits = ceil_div(key_bits, passes);
+    // The zeros' rows over the launches after the marks, in proportion to what
+    // each can take beside its own work: scatter 4, histogram 1, scan 1.
+    zero.used = p.used;
+    const int rows = zero.end, shares = 6 * passes - 2;
+    int given = 0;
+    const auto share = [&](int n) {
+        p.zero = zero;
+        p.zero.first = (int)((int64_t)rows * given / shares);
+        p.zero.end = (int)((int64_t)rows * (given + n) / shares);
+        given += n;
+        return zero_groups(p.zero);
+    };
     int at = 0;
     for (int i = 0; i < passes; i++) {
         p.ids = i ? nullptr : a.ids;
         p.key_in = key[at], p.place_in = place[at];
         p.key_out = key[at ^ 1], p.place_out = place[at ^ 1];
         p.shift = i * p.bits;
-        p.last = i == passes - 1;
-        hipLaunchKernelGGL(sort_hist_kernel, dim3(tiles), dim3(256), 0, s, p);
-        hipLaunchKernelGGL(sort_scan_kernel, dim3(1 << p.bits), dim3(256), 0, s, p);
-        hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles), dim3(256), 0, s, p);
+        const int hist = i ? share(1) : 0;
+        hipLaunchKernelGGL(sort_hist_kernel, dim3(tiles + hist), dim3(256), 0, s, p);
+        const int scan = i ? share(1) : std::min(1024, tiles * 4);  // first pass: the marks
+        hipLaunchKernelGGL(sort_scan_kernel, dim3((1 << p.bits) + scan), dim3(256), 0, s, p);
+        const int scatter = share(4);
+        hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles + scatter), dim3(256), 0, s, p);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         at ^= 1;
     }
