@@ -168,14 +168,21 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)
 __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
-// 16 bytes a lane from `base` + off to LDS bytes lds .. lds + 1023
+// 16 bytes a lane from the descriptor's base + off to LDS bytes lds .. lds + 1023.
+// The compiler sees neither the load nor its M0: a write of M0 has to be one
+// wait state ahead of a load that reads it.
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
 }
+// A buffer descriptor of 2^31 bytes from `base` on.  Scalar registers that the
+// vector unit has written have to be five wait states old when a load reads
+// them, and here the compiler does not know of the load.
 __device__ __forceinline__ u32x4 descriptor(const char *base) {
     const uint64_t b = (uint64_t)base;
-    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b),
-                 (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(b >> 32) & 0xffffu)), OUTSIDE, 0x00020000u};
+    u32x4 d = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(b >> 32) & 0xffffu)), OUTSIDE, 0x00020000u};
+    asm volatile("s_nop 4" : "+s"(d));
+    return d;
 }
 
 template <int TYPE> constexpr int stage_k() { return TYPE == BERT_AMD_F32 ? 32 : 64; }
