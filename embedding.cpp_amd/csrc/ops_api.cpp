@@ -59,8 +59,22 @@ const char *bad_matrix(const Matrix &m) {
     return m.ld >= m.width || (m.input && m.ld == 0) ? nullptr : m.name;
 }
 
-constexpr int64_t MAX_M = ((int64_t)1 << 31) - 1;
-constexpr int32_t MAX_SIDE = (1 << 22) - 1, MAX_IDS = 1 << 28, MAX_ROWS = 1 << 30;
+// Whether any byte belongs to a row of both.  Rows of the same stride may lie
+// side by side, as columns of one wider matrix do; with different strides,
+// spans that meet count as overlapping.
+bool overlap(const Matrix &a, int64_t a_rows, const Matrix &b, int64_t b_rows) {
+    if (!a.p || !b.p || a_rows < 1 || b_rows < 1) return false;
+    const int64_t wa = a.width * a.size, wb = b.width * b.size, la = a.ld * a.size, lb = b.ld * b.size;
+    const char *pa = (const char *)a.p, *pb = (const char *)b.p;
+    if (pa + (a_rows - 1) * la + wa <= pb || pb + (b_rows - 1) * lb + wb <= pa) return false;
+    if (la != lb || la == 0) return true;
+    int64_t d = (pb - pa) % la;
+    if (d < 0) d += la;
+    return d < wa || d + wb > la;
+}
+
+constexpr int64_t MAX_M = (int64_t)1 << 30;
+constexpr int32_t MAX_SIDE = (1 << 22) - 1, MAX_WIDTH = (1 << 20) - 1, MAX_IDS = 1 << 28, MAX_ROWS = 1 << 30;
 
 // the largest product's 64 x 64 tiles fit a launch (under 2^32 threads)
 constexpr int64_t MAX_AREA = (int64_t)1 << 34;
@@ -69,6 +83,41 @@ bool linear_shape_ok(int32_t type, int64_t M, int32_t N, int32_t K) {
     return is_float(type) && M >= 0 && M <= MAX_M && N >= 1 && N <= MAX_SIDE && K >= 1 && K <= MAX_SIDE &&
            M * N <= MAX_AREA && M * K <= MAX_AREA && (int64_t)N * K <= MAX_AREA;
 }
+// The memory of an optimizer step: what is written must be disjoint, and what is
+// read must not lie in it.  Tensors usually follow each other in buffers of
+// their own, which one look at each tells; else the spans are sorted.
+struct Spans {
+    static constexpr int READ = 6;  // kinds 0 .. 5 are written
+    typedef std::pair<const char *, const char *> Span;
+    std::vector<Span> of[READ + 1];
+    void add(int kind, const void *p, int64_t bytes) { of[kind].emplace_back((const char *)p, (const char *)p + bytes); }
+    bool empty() const { return of[0].empty(); }
+    bool clash() {
+        std::vector<Span> whole;  // from each kind's first byte to its last
+        bool ordered = true;
+        for (int k = 0; k <= READ; k++) {
+            if (of[k].empty()) continue;
+            Span w = of[k][0];
+            for (size_t i = 1; i < of[k].size(); i++) {
+                ordered = ordered && (k == READ || of[k][i].first >= of[k][i - 1].second);
+                w.first = std::min(w.first, of[k][i].first), w.second = std::max(w.second, of[k][i].second);
+            }
+            for (const Span &o : whole) ordered = ordered && (w.first >= o.second || o.first >= w.second);
+            whole.push_back(w);
+        }
+        if (ordered) return false;
+        std::vector<Span> written;
+        for (int k = 0; k < READ; k++) written.insert(written.end(), of[k].begin(), of[k].end());
+        std::sort(written.begin(), written.end());
+        for (size_t i = 1; i < written.size(); i++)
+            if (written[i].first < written[i - 1].second) return true;
+        for (const Span &r : of[READ]) {  // the last written span that begins before r's end
+            auto at = std::lower_bound(written.begin(), written.end(), Span(r.second, nullptr));
+            if (at != written.begin() && (--at)->second > r.first) return true;
+        }
+        return false;
+    }
+};
 bool workspace_ok(const void *p, int64_t bytes, int64_t need) {
     return need == 0 || (p && bytes >= need && !off(p, 16));
 }
@@ -95,7 +144,15 @@ int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int64_t M, in
         if (m.p || (m.name[0] != 'r' && m.name[0] != 'z'))
             if (const char *bad = bad_matrix(m)) return refuse("bert_amd_linear: %s is null, misaligned or has too short rows", bad);
     if (bias && off(bias, 4)) return refuse("bert_amd_linear: bias is misaligned");
-    if (residual == y && ldr != ldy) return refuse("bert_amd_linear: residual is y with another row stride");
+    const Matrix vector = {"bias", bias, N, N, true, 4};
+    const int64_t rows[] = {M, N, M, M, M};
+    for (int out : {2, 4})
+        for (int in = 0; in < 5; in++) {
+            const bool same = out == 2 && in == 3 && residual == y && (ldr == ldy || M == 1);  // each element read before it is written
+            if (in != out && !same && overlap(all[out], M, all[in], rows[in]))
+                return refuse("bert_amd_linear: %s overlaps %s", all[out].name, all[in].name);
+            if (overlap(all[out], M, vector, 1)) return refuse("bert_amd_linear: %s overlaps bias", all[out].name);
+        }
     const int64_t need = linear_ws_bytes(type, M, N, K, linear_aligned(x, ldx, type) && linear_aligned(w, ldw, type));
     if (!workspace_ok(workspace, workspace_bytes, need))
         return refuse("bert_amd_linear: workspace is null, misaligned or under %lld bytes", (long long)need);
@@ -129,6 +186,15 @@ int32_t bert_amd_linear_backward(int32_t device, int32_t type, int32_t act, int6
         if (m.p)
             if (const char *bad = bad_matrix(m)) return refuse("bert_amd_linear_backward: %s is misaligned or has too short rows", bad);
     if (!dx && !dw && !dbias) return 0;
+    const int64_t in_rows[] = {M, M, M, N}, out_rows[] = {M, N, 1};
+    for (int o = 0; o < 3; o++) {
+        for (int i = 0; i < 4; i++)
+            if (reads[i] && overlap(outs[o], out_rows[o], ins[i], in_rows[i]))
+                return refuse("bert_amd_linear_backward: %s overlaps %s", outs[o].name, ins[i].name);
+        for (int i = 0; i < o; i++)
+            if (overlap(outs[o], out_rows[o], outs[i], out_rows[i]))
+                return refuse("bert_amd_linear_backward: %s overlaps %s", outs[o].name, outs[i].name);
+    }
     const bool aligned = linear_aligned(dy, lddy, type) && (!dw || linear_aligned(x, ldx, type)) && (!dx || linear_aligned(w, ldw, type));
     const int64_t need = linear_grad_ws_bytes(type, act, M, N, K, aligned);
     if (!workspace_ok(workspace, workspace_bytes, need))
@@ -155,6 +221,9 @@ int32_t bert_amd_lookup(int32_t device, int32_t table_type, int32_t out_type, in
     if (!ids || off(ids, 4)) return refuse("bert_amd_lookup: ids are null or misaligned");
     if (const char *bad = bad_matrix({"out", out, ldo, width, false, size_of(out_type)}))
         return refuse("bert_amd_lookup: %s is null, misaligned or has too short rows", bad);
+    const Matrix written = {"out", out, ldo, width, false, size_of(out_type)};
+    if (overlap(written, n, {"table", table, ld_table_bytes, row, true, 1}, n_rows) || overlap(written, n, {"ids", ids, n, n, true, 4}, 1))
+        return refuse("bert_amd_lookup: out overlaps the table or the ids");
     LookupArgs a;
     a.type = table_type, a.out_type = out_type, a.n = n, a.V = n_rows, a.E = width;
     a.table = table, a.ld_bytes = ld_table_bytes, a.ids = ids, a.scale = scale, a.out = out, a.ldo = ldo;
@@ -162,7 +231,7 @@ int32_t bert_amd_lookup(int32_t device, int32_t table_type, int32_t out_type, in
 }
 
 int64_t bert_amd_lookup_grad_workspace(int64_t n, int32_t n_rows, int32_t width) {
-    if (n < 0 || n > MAX_IDS || n_rows < 1 || n_rows > MAX_ROWS || width < 1 || width > MAX_SIDE)
+    if (n < 0 || n > MAX_IDS || n_rows < 1 || n_rows > MAX_ROWS || width < 1 || width > MAX_WIDTH)
         return refuse("bert_amd_lookup_grad_workspace: invalid size");
     return lookup_grad_ws_bytes(n, n_rows, width);
 }
@@ -171,7 +240,7 @@ int32_t bert_amd_lookup_grad(int32_t device, int32_t type, int64_t n, int32_t n_
                              const int32_t *ids, float scale, int32_t pad_id, int32_t accumulate, float *dtable, int64_t ldt,
                              void *workspace, int64_t workspace_bytes, void *hip_stream) {
     if (!is_float(type)) return refuse("bert_amd_lookup_grad: type %d is not supported", type);
-    if (n < 0 || n > MAX_IDS || n_rows < 1 || n_rows > MAX_ROWS || width < 1 || width > MAX_SIDE)
+    if (n < 0 || n > MAX_IDS || n_rows < 1 || n_rows > MAX_ROWS || width < 1 || width > MAX_WIDTH)
         return refuse("bert_amd_lookup_grad: invalid size (n %lld, n_rows %d, width %d)", (long long)n, n_rows, width);
     if (n > 0) {
         if (const char *bad = bad_matrix({"dout", dout, ldd, width, true, size_of(type)}))
@@ -180,6 +249,9 @@ int32_t bert_amd_lookup_grad(int32_t device, int32_t type, int64_t n, int32_t n_
     }
     if (const char *bad = bad_matrix({"dtable", dtable, ldt, width, false, 4}))
         return refuse("bert_amd_lookup_grad: %s is null, misaligned or has too short rows", bad);
+    const Matrix written = {"dtable", dtable, ldt, width, false, 4};
+    if (overlap(written, n_rows, {"dout", dout, ldd, width, true, size_of(type)}, n) || overlap(written, n_rows, {"ids", ids, n, n, true, 4}, 1))
+        return refuse("bert_amd_lookup_grad: dtable overlaps dout or the ids");
     const int64_t need = lookup_grad_ws_bytes(n, n_rows, width);
     if (!workspace_ok(workspace, workspace_bytes, need))
         return refuse("bert_amd_lookup_grad: workspace is null, misaligned or under %lld bytes", (long long)need);
@@ -200,7 +272,7 @@ int32_t bert_amd_adamw(int32_t device, int32_t n_tensors, const bert_amd_adamw_t
         return refuse("bert_amd_adamw: lr >= 0, 0 <= beta < 1, eps > 0 and step >= 1 are required");
     if (off(grad_scale, 4)) return refuse("bert_amd_adamw: grad_scale is misaligned");
     try {
-        std::vector<std::pair<const float *, const float *>> spans;
+        Spans spans;
         for (int i = 0; i < n_tensors; i++) {
             const bert_amd_adamw_tensor &t = tensors[i];
             if (t.n < 0 || t.n > MAX_AREA || !(t.weight_decay >= 0 && std::isfinite(t.weight_decay)))
@@ -213,12 +285,15 @@ int32_t bert_amd_adamw(int32_t device, int32_t n_tensors, const bert_amd_adamw_t
             if (t.copy && (copy_type != BERT_AMD_F16 && copy_type != BERT_AMD_BF16))
                 return refuse("bert_amd_adamw: copies of type %d are not supported", copy_type);
             if (t.copy && off(t.copy, 2)) return refuse("bert_amd_adamw: tensor %d has a misaligned copy", i);
-            spans.emplace_back(t.p, t.p + t.n);
+            const int64_t blocks = state_bits == 8 ? (t.n + 255) / 256 * 4 : 0;
+            spans.add(0, t.p, t.n * 4), spans.add(1, t.m, t.n * s), spans.add(2, t.v, t.n * s);
+            if (blocks) spans.add(3, t.m_scale, blocks), spans.add(4, t.v_scale, blocks);
+            if (t.copy) spans.add(5, t.copy, t.n * 2);
+            spans.add(Spans::READ, t.grad, t.n * size_of(grad_type));
         }
         if (spans.empty()) return 0;
-        std::sort(spans.begin(), spans.end());
-        for (size_t i = 1; i < spans.size(); i++)
-            if (spans[i].first < spans[i - 1].second) return refuse("bert_amd_adamw: two tensors share weights");
+        if (grad_scale) spans.add(Spans::READ, grad_scale, 4);
+        if (spans.clash()) return refuse("bert_amd_adamw: two tensors share memory, or a gradient lies in what is written");
     } catch (const std::exception &e) {
         return refuse("bert_amd_adamw: %s", e.what());
     }

@@ -193,7 +193,8 @@ BERT_API int32_t bert_amd_shard_cuts(int32_t n_seqs, const int32_t *n_tokens, in
    are `ld*` elements apart (at least its width; 0 for an input: the one row
    again for every row); nothing is written between them.  Results do not
    depend on the launch: the same inputs give the same bits.  Outputs must not
-   overlap inputs or each other unless a call says so.  Each returns 0, or
+   overlap inputs or each other unless a call says so (columns of one wider
+   matrix do not overlap).  Each returns 0, or
    negative without having launched anything: -1 an invalid argument, -3 a HIP
    error (message via bert_amd_last_error). */
 
@@ -224,7 +225,7 @@ enum bert_amd_act {
                 (may be y itself, with ldr = ldy)
      y        : [M][N]; z: [M][N] or NULL: the pre-activation, kept for
                 bert_amd_linear_backward
-   M = 0 does nothing; M < 2^31, 1 <= N, K < 2^22, and none of M N, M K and N K
+   M = 0 does nothing; M <= 2^30, 1 <= N, K < 2^22, and none of M N, M K and N K
    over 2^34.
    The workspace takes copies of x and w where their rows are not 16-byte pieces
    throughout: `aligned` != 0 says that both begin on 16 bytes and their row
@@ -265,7 +266,7 @@ BERT_API int32_t bert_amd_lookup(int32_t device, int32_t table_type, int32_t out
    as zero.  accumulate != 0 adds it to dtable instead and leaves unused rows
    untouched.  Ids outside [0, n_rows) and pad_id (-1: none) have no gradient.
      dout     : [n][width] of type F32, F16 or BF16; dtable: f32 [n_rows][width]
-   n <= 2^28, n_rows <= 2^30. */
+   n <= 2^28, n_rows <= 2^30, width < 2^20. */
 BERT_API int64_t bert_amd_lookup_grad_workspace(int64_t n, int32_t n_rows, int32_t width);
 BERT_API int32_t bert_amd_lookup_grad(int32_t device, int32_t type, int64_t n, int32_t n_rows, int32_t width,
                                       const void *dout, int64_t ldd, const int32_t *ids, float scale, int32_t pad_id,
@@ -273,7 +274,7 @@ BERT_API int32_t bert_amd_lookup_grad(int32_t device, int32_t type, int64_t n, i
                                       int64_t workspace_bytes, void *hip_stream);
 
 /* The word-embedding table of replica `slot` as bert_amd_lookup takes it (rows
-   contiguous); it belongs to the context and is read-only.  `type` is the
+   contiguous); it belongs to the context, until bert_free, and is read-only.  `type` is the
    file's row type, or F32 where the context keeps an f32 copy ("emb_raw" 0). */
 BERT_API int32_t bert_amd_word_table(struct bert_ctx *ctx, int32_t slot, const void **table, int32_t *type,
                                      int32_t *n_rows, int32_t *width, int32_t *device);
@@ -301,7 +302,10 @@ struct bert_amd_adamw_tensor {
    device memory; NULL: 1).  8-bit states store m and sqrt(v) as small floats,
    rounded up or down at random by `seed`, another one each step (unused with 32
    bits).  An infinity or NaN in g makes its weight and moments NaN, with 8-bit
-   states the moments of its whole block of 256.  n <= 2^34; tensors must not overlap. */
+   states the moments of its whole block of 256.  n <= 2^34; what is
+   written must not overlap, nor a gradient lie in it (copies of the same
+   gradient are fine).  Captured in a graph, step, lr and seed are those of the
+   capture. */
 BERT_API int32_t bert_amd_adamw(int32_t device, int32_t n_tensors, const struct bert_amd_adamw_tensor *tensors,
                                 int32_t state_bits, int32_t grad_type, int32_t copy_type, double lr, double beta1,
                                 double beta2, double eps, int64_t step, uint32_t seed, const float *grad_scale,

@@ -655,39 +655,39 @@ def test_refusals_of_the_library():
     def refused(rc, word):
         assert rc == -1 and word in bertlib.last_error(), (rc, bertlib.last_error())
 
-    ok = dict(device=0, type=0, act=0, M=4, N=8, K=8, x=P, ldx=8, w=P, ldw=8, bias=P, r=P, ldr=8, y=P + 4096, ldy=8, z=NULL, ldz=8, ws=P, nws=big, s=NULL)
-    for change, word in ((dict(type=2), "type"), (dict(type=7), "type"), (dict(act=6), "activation"), (dict(act=-1), "activation"), (dict(M=-1), "size"), (dict(M=1 << 31), "size"), (dict(N=0), "size"), (dict(K=0), "size"), (dict(N=1 << 22), "size"), (dict(M=1 << 30, N=1 << 10), "size"), (dict(x=NULL), "x"), (dict(x=P + 2), "x"), (dict(ldx=7), "x"), (dict(ldx=-8), "x"), (dict(w=NULL), "w"), (dict(y=NULL), "y"), (dict(ldy=0), "y"), (dict(ldy=7), "y"), (dict(r=P + 1), "residual"), (dict(z=P, ldz=0), "z"), (dict(bias=P + 1), "bias"), (dict(r=P + 4096, ldr=9), "residual")):
+    ok = dict(device=0, type=0, act=0, M=4, N=8, K=8, x=P, ldx=8, w=P, ldw=8, bias=P, r=P, ldr=8, y=P + 4096, ldy=8, z=NULL, ldz=8, ws=2 * P, nws=big, s=NULL)
+    for change, word in ((dict(type=2), "type"), (dict(type=7), "type"), (dict(act=6), "activation"), (dict(act=-1), "activation"), (dict(M=-1), "size"), (dict(M=(1 << 30) + 1), "size"), (dict(N=0), "size"), (dict(K=0), "size"), (dict(N=1 << 22), "size"), (dict(M=1 << 30, N=1 << 10), "size"), (dict(x=NULL), "x"), (dict(x=P + 2), "x"), (dict(ldx=7), "x"), (dict(ldx=-8), "x"), (dict(w=NULL), "w"), (dict(y=NULL), "y"), (dict(ldy=0), "y"), (dict(ldy=7), "y"), (dict(r=P + 1), "residual"), (dict(z=P, ldz=0), "z"), (dict(bias=P + 1), "bias"), (dict(r=P + 4096, ldr=9), "residual"), (dict(y=P), "overlaps x"), (dict(y=P + 32 * 3 + 28), "overlaps x"), (dict(x=P + 4096, ldx=16), "overlaps x"), (dict(y=P + 64, ldx=32, ldy=32, ldw=4096), "overlaps w"), (dict(r=P + 4096 + 4), "overlaps residual"), (dict(z=P + 4096 + 16), "overlaps"), (dict(bias=P + 4096 + 8), "overlaps bias")):
         refused(L.bert_amd_linear(*{**ok, **change}.values()), word)
     assert L.bert_amd_linear_workspace(5, 4, 8, 8, 1) == -1
     for K in (100000, 100001):  # parts of k; copies in whole pieces
         need = L.bert_amd_linear_workspace(0, 40, 8, K, 1)
         assert need > 0
         for change in (dict(ws=NULL), dict(nws=need - 1), dict(ws=P + 8)):
-            refused(L.bert_amd_linear(*{**ok, "M": 40, "K": K, "ldx": K, "ldw": K, **change}.values()), "workspace")
+            refused(L.bert_amd_linear(*{**ok, "M": 40, "K": K, "ldx": K, "ldw": K, "y": 64 * P, **change}.values()), "workspace")
     need = L.bert_amd_linear_workspace(0, 40, 8, 100000, 1)
     for change in (dict(x=P + 4), dict(ldw=100001)):  # asked for as aligned, given otherwise
-        refused(L.bert_amd_linear(*{**ok, "M": 40, "K": 100000, "ldx": 100000, "ldw": 100000, "nws": need, **change}.values()), "workspace")
+        refused(L.bert_amd_linear(*{**ok, "M": 40, "K": 100000, "ldx": 100000, "ldw": 100000, "y": 64 * P, "nws": need, **change}.values()), "workspace")
     assert L.bert_amd_linear(*{**ok, "M": 0, "x": NULL}.values()) == 0
 
-    ok = dict(device=0, type=1, act=2, M=4, N=8, K=8, dy=P, lddy=8, z=P, ldz=8, x=P, ldx=8, w=P, ldw=8, dx=P, lddx=8, dw=P, lddw=8, db=P, ws=P, nws=big, s=NULL)
-    for change, word in ((dict(type=3), "type"), (dict(act=9), "activation"), (dict(M=-1), "size"), (dict(dy=NULL), "dy"), (dict(dy=P + 1), "dy"), (dict(z=NULL), "z"), (dict(ldz=4), "z"), (dict(x=NULL), "x"), (dict(w=NULL), "w"), (dict(lddx=0), "dx"), (dict(lddw=7), "dw"), (dict(db=P + 2), "dbias"), (dict(ws=NULL), "workspace"), (dict(nws=1), "workspace")):
+    ok = dict(device=0, type=1, act=2, M=4, N=8, K=8, dy=P, lddy=8, z=P, ldz=8, x=P, ldx=8, w=P, ldw=8, dx=P + 4096, lddx=8, dw=P + 8192, lddw=8, db=P + 16384, ws=2 * P, nws=big, s=NULL)
+    for change, word in ((dict(type=3), "type"), (dict(act=9), "activation"), (dict(M=-1), "size"), (dict(dy=NULL), "dy"), (dict(dy=P + 1), "dy"), (dict(z=NULL), "z"), (dict(ldz=4), "z"), (dict(x=NULL), "x"), (dict(w=NULL), "w"), (dict(lddx=0), "dx"), (dict(lddw=7), "dw"), (dict(db=P + 2), "dbias"), (dict(ws=NULL), "workspace"), (dict(nws=1), "workspace"), (dict(dx=P), "overlaps"), (dict(dw=P + 4096 + 16), "overlaps"), (dict(db=P + 8192 + 64), "overlaps"), (dict(db=P + 16), "overlaps")):
         refused(L.bert_amd_linear_backward(*{**ok, **change}.values()), word)
     assert L.bert_amd_linear_backward(*{**ok, "dx": NULL, "dw": NULL, "db": NULL}.values()) == 0
     assert L.bert_amd_linear_backward_workspace(1, 2, -1, 8, 8, 1) == -1
 
-    ok = dict(device=0, type=2, out=0, n=4, V=10, E=64, table=P, ld=36, ids=P, scale=1.0, o=P, ldo=64, s=NULL)
-    for change, word in ((dict(type=8), "types"), (dict(out=2), "types"), (dict(n=-1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(E=40), "size"), (dict(table=NULL), "table"), (dict(table=P + 1), "table"), (dict(ld=35), "table"), (dict(ld=37), "table"), (dict(ids=NULL), "ids"), (dict(ids=P + 2), "ids"), (dict(o=NULL), "out"), (dict(ldo=63), "out"), (dict(ldo=0), "out")):
+    ok = dict(device=0, type=2, out=0, n=4, V=10, E=64, table=P, ld=36, ids=P, scale=1.0, o=P + 4096, ldo=64, s=NULL)
+    for change, word in ((dict(type=8), "types"), (dict(out=2), "types"), (dict(n=-1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(E=40), "size"), (dict(table=NULL), "table"), (dict(table=P + 1), "table"), (dict(ld=35), "table"), (dict(ld=37), "table"), (dict(ids=NULL), "ids"), (dict(ids=P + 2), "ids"), (dict(o=NULL), "out"), (dict(ldo=63), "out"), (dict(ldo=0), "out"), (dict(o=P + 352), "overlaps"), (dict(table=2 * P, o=P + 8), "overlaps")):
         refused(L.bert_amd_lookup(*{**ok, **change}.values()), word)
     assert L.bert_amd_lookup(*{**ok, "n": 0, "ids": NULL}.values()) == 0
 
-    ok = dict(device=0, type=0, n=4, V=10, E=8, dout=P, ldd=8, ids=P, scale=1.0, pad=-1, acc=0, dt=P, ldt=8, ws=P, nws=big, s=NULL)
-    for change, word in ((dict(type=2), "type"), (dict(n=-1), "size"), (dict(n=(1 << 28) + 1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(dout=NULL), "dout"), (dict(ldd=7), "dout"), (dict(ids=NULL), "ids"), (dict(dt=NULL), "dtable"), (dict(ldt=7), "dtable"), (dict(n=5000, ws=NULL), "workspace"), (dict(n=5000, nws=16), "workspace"), (dict(n=5000, ws=P + 8), "workspace")):
+    ok = dict(device=0, type=0, n=4, V=10, E=8, dout=P, ldd=8, ids=P, scale=1.0, pad=-1, acc=0, dt=P + 4096, ldt=8, ws=2 * P, nws=big, s=NULL)
+    for change, word in ((dict(type=2), "type"), (dict(n=-1), "size"), (dict(n=(1 << 28) + 1), "size"), (dict(V=0), "size"), (dict(E=0), "size"), (dict(dout=NULL), "dout"), (dict(ldd=7), "dout"), (dict(ids=NULL), "ids"), (dict(dt=NULL), "dtable"), (dict(ldt=7), "dtable"), (dict(n=5000, ws=NULL, dt=3 * P), "workspace"), (dict(n=5000, nws=16, dt=3 * P), "workspace"), (dict(n=5000, ws=2 * P + 8, dt=3 * P), "workspace"), (dict(dt=P + 64), "overlaps"), (dict(dout=2 * P, dt=P + 12), "overlaps"), (dict(E=1 << 20, ldd=1 << 20, ldt=1 << 20), "size")):
         refused(L.bert_amd_lookup_grad(*{**ok, **change}.values()), word)
     assert L.bert_amd_lookup_grad_workspace(-1, 10, 8) == -1
 
     row = np.zeros(2, bertops.AdamW._ROW)
-    for k in ("p", "g", "m", "v", "ms", "vs"):
-        row[k] = [P, P + (1 << 16)]
+    for i, k in enumerate(("p", "g", "m", "v", "ms", "vs")):
+        row[k] = [(2 + i) * P, (2 + i) * P + (1 << 16)]
     row["n"] = 100
 
     def adamw(rows=row, n=2, bits=32, grad=0, copy=30, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, step=1, scale=NULL):
@@ -703,11 +703,15 @@ def test_refusals_of_the_library():
             r[k][1] = v
         return r
 
-    for kw, word in ((dict(n=-1), "size"), (dict(n=(1 << 34) + 1), "size"), (dict(decay=nan), "decay"), (dict(decay=-1.0), "decay"), (dict(p=0), "pointer"), (dict(g=0), "pointer"), (dict(m=P + 2), "pointer"), (dict(copy=P + 1), "copy"), (dict(p=P + 396), "share")):
+    for kw, word in ((dict(n=-1), "size"), (dict(n=(1 << 34) + 1), "size"), (dict(decay=nan), "decay"), (dict(decay=-1.0), "decay"), (dict(p=0), "pointer"), (dict(g=0), "pointer"), (dict(m=P + 2), "pointer"), (dict(copy=P + 1), "copy"), (dict(p=2 * P + 396), "share"), (dict(m=5 * P + 8), "share"), (dict(v=5 * P), "share"), (dict(g=2 * P + 100), "share"), (dict(g=4 * P - 396), "share"), (dict(copy=3 * P - 200 + 400, g=3 * P), "share")):
         refused(adamw(with_(**kw)), word)
     refused(adamw(with_(copy=P), copy=0), "copies")
     refused(adamw(with_(ms=0), bits=8), "pointer")
     assert adamw(n=0) == 0
+    same = row.copy()  # in any order, one gradient for both: nothing is wrong, and only the missing GPU can refuse it
+    same["p"][1], same["g"][1], same["m"][1] = 2 * P - 4000, 3 * P, 4 * P - 400
+    if not torch.cuda.is_available():
+        assert adamw(same) == -3 and adamw(row) == -3
     refused(L.bert_amd_adamw_moments(0, -1, P, P, P, P, P, P, NULL), "size")
     refused(L.bert_amd_adamw_moments(0, 4, NULL, P, P, P, P, P, NULL), "pointer")
     out = [ctypes.c_void_p()] + [ctypes.c_int32() for _ in range(4)]
@@ -739,6 +743,20 @@ def test_refusals_on_tensors():
                  lambda: bertops._ids(torch.zeros(3, dtype=torch.int64), x.device), lambda: bertops._ids(torch.zeros(6, dtype=torch.int32)[::2], x.device)):
         with pytest.raises(ValueError):
             call()
+
+
+@gpu
+def test_columns_of_one_matrix():
+    """Inputs and outputs side by side in one wider matrix do not overlap; shifted into each other they are refused."""
+    x, w, r, b = make_layer(50, 64, 64, torch.float32, seed=20)
+    wide = torch.zeros(50, 192, device="cuda")
+    wide[:, :64], wide[:, 64:128] = x.cuda(), r.cuda()
+    bertops.linear(wide[:, :64], w.cuda(), b.cuda(), residual=wide[:, 64:128], act="gelu", out=wide[:, 128:])
+    check_linear(x, w, b, r, "gelu", wide[:, 128:])
+    assert torch.equal(wide[:, :64].cpu(), x) and torch.equal(wide[:, 64:128].cpu(), r)
+    for out in (wide[:, :64], wide[:, 32:96], wide[1:, :64]):
+        with pytest.raises(ValueError):
+            bertops.linear(wide[: len(out), :64], w.cuda(), out=out)
 
 
 @gpu
