@@ -227,14 +227,18 @@ struct Tile {
             }
         }
     }
+    // the descriptor of the next stage to load
+    __device__ __forceinline__ u32x4 next_stage() {
+        const u32x4 d = descriptor(base);
+        base += step;
+        return d;
+    }
     // loads FROM .. TO - 1 of a stage to `lds`; `left`: k from the stage's start to the end
     template <int FROM, int TO>
-    __device__ __forceinline__ void load(uint32_t lds, int left) {
-        const u32x4 d = descriptor(base);
+    __device__ __forceinline__ void load(u32x4 d, uint32_t lds, int left) const {
         const uint32_t w = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x >> 6) * 1024);
 #pragma unroll
         for (int i = FROM; i < TO; i++) load_to_lds(d, at[i] < left ? off[i] : OUTSIDE, w + i * NT * 16);
-        if (TO == LOADS) base += step;
     }
     // operand registers of rows r0 .. r0 + 31 and chunks 2 ks, 2 ks + 1 of the stage at `lds`: lane half h has chunk 2 ks + h's k
     static __device__ __forceinline__ u32x4 read(const char *lds, int r0, int ks) {
@@ -372,8 +376,8 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
     const auto left_at = [&](int64_t k0) { return (int)max((int64_t)0, min((int64_t)SK, kb - k0)); };
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        ta.template load<0, TileA::LOADS>(lds + i * STAGE, left_at(ka + i * SK));
-        tb.template load<0, TileB::LOADS>(lds + i * STAGE + TileA::BYTES, left_at(ka + i * SK));
+        ta.template load<0, TileA::LOADS>(ta.next_stage(), lds + i * STAGE, left_at(ka + i * SK));
+        tb.template load<0, TileB::LOADS>(tb.next_stage(), lds + i * STAGE + TileA::BYTES, left_at(ka + i * SK));
     }
     wait_loads<TileA::LOADS + TileB::LOADS>();
     barrier();
@@ -382,6 +386,7 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
 #pragma unroll
     for (int i = 0; i < TM; i++) read_a(0, i, 0, 0);
     int buf = 0;
+    u32x4 stage = {};
     for (int64_t k0 = ka; k0 < kb; k0 += SK, buf ^= 1) {
         // The loads of the stage after the next go out between the products of
         // this stage's last quarter (its second matrix, once the barrier has freed
@@ -395,11 +400,13 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
                 wait_reads();
                 wait_loads<0>();
                 barrier();
+                stage = tb.next_stage();
             }
+            if (ks == 0 && k0 > ka) stage = ta.next_stage();
             for_const<TM>([&](auto ic) {
                 constexpr int i = ic.value;
-                if (ks == KS - 1) tb.template load<i * TileB::LOADS / TM, (i + 1) * TileB::LOADS / TM>(lds + buf * STAGE + TileA::BYTES, left_at(k0 + 2 * SK));
-                if (ks == 0 && k0 > ka) ta.template load<i * TileA::LOADS / TM, (i + 1) * TileA::LOADS / TM>(lds + (buf ^ 1) * STAGE, left_at(k0 + SK));
+                if (ks == KS - 1) tb.template load<i * TileB::LOADS / TM, (i + 1) * TileB::LOADS / TM>(stage, lds + buf * STAGE + TileA::BYTES, left_at(k0 + 2 * SK));
+                if (ks == 0 && k0 > ka) ta.template load<i * TileA::LOADS / TM, (i + 1) * TileA::LOADS / TM>(stage, lds + (buf ^ 1) * STAGE, left_at(k0 + SK));
 #pragma unroll
                 for (int j = i * TN / TM; j < (i + 1) * TN / TM; j++) read_b(next, j, from, kn);
                 read_a(next, i, from, kn);
