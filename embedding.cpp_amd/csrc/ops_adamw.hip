@@ -90,22 +90,6 @@ __device__ __forceinline__ void block_scale(uint32_t peak, float top, float &sca
     inv = scale > 0.f && peak < 0x7f800000u ? 1.f / scale : 0.f;
 }
 
-// four elements at p, aligned to as many bytes as they take
-template <typename T, typename V>
-__device__ __forceinline__ void get4(const T *p, V *v) {
-    struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; };
-    const Four f = *(const Four *)p;
-#pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = (V)f.v[j];
-}
-template <typename T, typename V>
-__device__ __forceinline__ void put4(T *p, const V *v) {
-    struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; } f;
-#pragma unroll
-    for (int j = 0; j < 4; j++) f.v[j] = (T)v[j];
-    *(Four *)p = f;
-}
-
 struct Moments {
     float m, v, r;
 };
@@ -140,14 +124,14 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table a) {
         float ms = 0.f, vs = 0.f;
         if constexpr (BITS == 8) ms = t.ms[b / STATE_BLOCK], vs = t.vs[b / STATE_BLOCK];
         if (whole) {
-            get4(t.p + i, p);
-            get4((const G *)t.g + i, g);
+            get_n<float, 4>(t.p + i, p);
+            get_n<G, 4>((const G *)t.g + i, g);
             if constexpr (BITS == 8) {
-                get4((const uint8_t *)t.m + i, cm);
-                get4((const uint8_t *)t.v + i, cv);
+                get_n<uint8_t, 4>((const uint8_t *)t.m + i, cm);
+                get_n<uint8_t, 4>((const uint8_t *)t.v + i, cv);
             } else {
-                get4((const float *)t.m + i, m);
-                get4((const float *)t.v + i, v);
+                get_n<float, 4>((const float *)t.m + i, m);
+                get_n<float, 4>((const float *)t.v + i, v);
             }
         } else {
 #pragma unroll
@@ -190,14 +174,14 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table a) {
             }
         }
         if (whole) {
-            put4(t.p + i, p);
-            if (t.copy) put4((C *)t.copy + i, p);
+            put_n<float, 4>(t.p + i, p);
+            if (t.copy) put_n<C, 4>((C *)t.copy + i, p);
             if constexpr (BITS == 8) {
-                put4((uint8_t *)t.m + i, cm);
-                put4((uint8_t *)t.v + i, cv);
+                put_n<uint8_t, 4>((uint8_t *)t.m + i, cm);
+                put_n<uint8_t, 4>((uint8_t *)t.v + i, cv);
             } else {
-                put4((float *)t.m + i, m);
-                put4((float *)t.v + i, v);
+                put_n<float, 4>((float *)t.m + i, m);
+                put_n<float, 4>((float *)t.v + i, v);
             }
         } else {
 #pragma unroll
@@ -220,18 +204,18 @@ __global__ __launch_bounds__(256) void moments_kernel(int64_t n, const uint8_t *
         if (m_out) {
             uint32_t c[4] = {};
             float x[4];
-            if (vec && count == 4) get4(m + i, c);
+            if (vec && count == 4) get_n<uint8_t, 4>(m + i, c);
             else for (int j = 0; j < count; j++) c[j] = m[i + j];
             const float scale = ms[i / STATE_BLOCK];
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j] = code_value<3>(c[j] & 127u) * scale, x[j] = c[j] & 128u ? -x[j] : x[j];
-            if (vec && count == 4) put4(m_out + i, x);
+            if (vec && count == 4) put_n<float, 4>(m_out + i, x);
             else for (int j = 0; j < count; j++) m_out[i + j] = x[j];
         }
         if (v_out) {
             uint32_t c[4] = {};
             float x[4];
-            if (vec && count == 4) get4(v + i, c);
+            if (vec && count == 4) get_n<uint8_t, 4>(v + i, c);
             else for (int j = 0; j < count; j++) c[j] = v[i + j];
             const float scale = vs[i / STATE_BLOCK];
 #pragma unroll
@@ -239,7 +223,7 @@ __global__ __launch_bounds__(256) void moments_kernel(int64_t n, const uint8_t *
                 const float r = code_value<4>(c[j]) * scale;
                 x[j] = r * r;
             }
-            if (vec && count == 4) put4(v_out + i, x);
+            if (vec && count == 4) put_n<float, 4>(v_out + i, x);
             else for (int j = 0; j < count; j++) v_out[i + j] = x[j];
         }
     }

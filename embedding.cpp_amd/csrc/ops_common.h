@@ -52,6 +52,22 @@ __device__ __forceinline__ void add8(const T *p, float *v) {
     }
 }
 
+// N elements at p, aligned to as many bytes as they take, as values and back
+template <typename T, int N, typename V>
+__device__ __forceinline__ void get_n(const T *p, V *v) {
+    struct __attribute__((aligned(N * sizeof(T)))) Some { T v[N]; };
+    const Some f = *(const Some *)p;
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] = (V)f.v[j];
+}
+template <typename T, int N, typename V>
+__device__ __forceinline__ void put_n(T *p, const V *v) {
+    struct __attribute__((aligned(N * sizeof(T)))) Some { T v[N]; } f;
+#pragma unroll
+    for (int j = 0; j < N; j++) f.v[j] = (T)v[j];
+    *(Some *)p = f;
+}
+
 // Activations and their slopes in f32.  gelu is the tanh form that the
 // encoder's feed-forward layer uses, written z * sigmoid(2u): no cancellation
 // in its lower tail.

@@ -305,21 +305,6 @@ __device__ __forceinline__ void act_n(float *v, int act) {
     }
 }
 
-// 8 consecutive columns of row m, the bias added, some of them past the end or not aligned: z, activation, residual, y
-template <typename T>
-__device__ __forceinline__ void store_edge(const Epilogue &e, int64_t m, int64_t n, int64_t N, float *v) {
-    T *z = (T *)e.z + m * e.ldz + n, *y = (T *)e.y + m * e.ldy + n;
-    const T *r = (const T *)e.r + m * e.ldr + n;
-    if (e.z)
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (n + i < N) z[i] = (T)v[i];
-    act_n<T, 8>(v, e.act);
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (n + i < N) y[i] = (T)(v[i] + (e.r ? (float)r[i] : 0.f));
-}
-
 // LDS row of the epilogue: a wave's 64 columns and 16 bytes more, so that the rows of a write start in different banks
 constexpr int OUT_LD = 68;
 
@@ -458,23 +443,37 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
 #pragma unroll
                 for (int i = 0; i < G; i++) put8(y + (g + 8 * i) * e.ldy, v + 8 * i);
             }
-        } else if (n < N) {
+        } else {  // an edge of the matrix, rows that are not aligned, or parts: a lane a column, four rows at a time
+            const int64_t n1 = n0 + wn + 64 * half + lane, m1 = m0 + wm + WR * rows;
+            const float bias1 = e.bias && !part ? e.bias[min(n1, N - 1)] : 0.f;
+            const int there = (int)min((int64_t)WR, M - m1);
+            if (n1 < N)
 #pragma unroll 1
-            for (int g = 0; g < WR && m + g < M; g += 8) {
-                float v[8];
+                for (int g = 0; g < there; g += 4) {
+                    float v[4], add[4] = {};
 #pragma unroll
-                for (int c = 0; c < 8; c++) v[c] = out[(g + row0) * OUT_LD + col + c] + bias[c];
-                if (part) {
-                    float *q = part + (split * M + m + g) * N + n;
-                    if (N % 4 == 0 && n + 8 <= N) put8(q, v);
-                    else
+                    for (int i = 0; i < 4; i++) v[i] = out[(g + i) * OUT_LD + lane] + bias1;
+                    if (part) {
+                        float *q = part + (split * M + m1 + g) * N + n1;
 #pragma unroll
-                        for (int c = 0; c < 8; c++)
-                            if (n + c < N) q[c] = v[c];
-                } else {
-                    store_edge<T>(e, m + g, n, N, v);
+                        for (int i = 0; i < 4; i++)
+                            if (g + i < there) q[i * N] = v[i];
+                        continue;
+                    }
+                    const T *r = (const T *)e.r + (m1 + g) * e.ldr + n1;
+                    T *y = (T *)e.y + (m1 + g) * e.ldy + n1, *z = (T *)e.z + (m1 + g) * e.ldz + n1;
+                    if (e.r)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) add[i] = (float)r[min(i, there - g - 1) * e.ldr];
+                    if (e.z)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (g + i < there) z[i * e.ldz] = (T)v[i];
+                    act_n<T, 4>(v, e.act);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (g + i < there) y[i * e.ldy] = (T)(v[i] + add[i]);
                 }
-            }
         }
     }
 }
@@ -485,27 +484,49 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Product p) {
     stage_product<TYPE, TA, TBT, BM, BN, WM, WN>(p, smem, blockIdx.x, blockIdx.z);
 }
 
-// Both products of a small layer's gradients at once, 64 x 64 tiles: each alone
-// leaves most of the chip idle, and a launch less counts there.
-template <int TYPE>
-__global__ __launch_bounds__(128, 2) void pair_gemm_kernel(Product dx, Product dw) {
+// Both products of a small layer's gradients at once, in tiles of 64 x BN: each
+// alone leaves most of the chip idle, and a launch less counts there.
+template <int TYPE, int BN, int WN>
+__global__ __launch_bounds__(128 * WN, 2) void pair_gemm_kernel(Product dx, Product dw) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int first = dx.tiles * dx.parts, b = blockIdx.x;
     if (b < first)
-        stage_product<TYPE, false, true, 64, 64, 2, 1>(dx, smem, b % dx.tiles, b / dx.tiles);
+        stage_product<TYPE, false, true, 64, BN, 2, WN>(dx, smem, b % dx.tiles, b / dx.tiles);
     else
-        stage_product<TYPE, true, true, 64, 64, 2, 1>(dw, smem, (b - first) % dw.tiles, (b - first) / dw.tiles);
+        stage_product<TYPE, true, true, 64, BN, 2, WN>(dw, smem, (b - first) % dw.tiles, (b - first) / dw.tiles);
 }
 
-// the parts of one or two products (blockIdx.y) added in order
-template <typename T>
+// The parts of one or two products (blockIdx.y) added in order, COLS columns a
+// thread.  A product in parts has under 2^31 elements (plan_for).
+template <typename T, int COLS>
 __global__ __launch_bounds__(256) void split_join_kernel(Product a, Product b) {
     const Product &p = blockIdx.y ? b : a;
     if (!p.part) return;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.M * p.N; i += (int64_t)gridDim.x * 256) {
-        float v = 0.f;
-        for (int s = 0; s < p.parts; s++) v += p.part[s * p.M * p.N + i];
-        epilogue_store<T>(p.e, i / p.N, i % p.N, v);
+    const uint32_t across = (uint32_t)p.N / COLS, all = (uint32_t)p.M * across;
+    const int64_t size = p.M * p.N;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256) {
+        const uint32_t m = i / across, n = (i - m * across) * COLS;
+        const float *from = p.part + (int64_t)m * p.N + n;
+        float v[COLS] = {};
+#pragma unroll 4
+        for (int s = 0; s < p.parts; s++) {
+            float w[COLS];
+            get_n<float, COLS>(from + s * size, w);
+#pragma unroll
+            for (int c = 0; c < COLS; c++) v[c] += w[c];
+        }
+        const Epilogue &e = p.e;
+#pragma unroll
+        for (int c = 0; c < COLS; c++) v[c] += e.bias ? e.bias[n + c] : 0.f;
+        if (e.z) put_n<T, COLS>((T *)e.z + m * e.ldz + n, v);
+        act_n<T, COLS>(v, e.act);
+        if (e.r) {
+            float w[COLS];
+            get_n<T, COLS>((const T *)e.r + m * e.ldr + n, w);
+#pragma unroll
+            for (int c = 0; c < COLS; c++) v[c] += w[c];
+        }
+        put_n<T, COLS>((T *)e.y + m * e.ldy + n, v);
     }
 }
 
@@ -564,41 +585,48 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
     part[blockIdx.y * N + col] = v;
 }
 
-// the column sums of `part`: 32 columns, 8 rows side by side
-__global__ __launch_bounds__(256) void column_sum_kernel(const float *part, int64_t rows, int64_t N, float *out) {
-    __shared__ float sums[8][33];
-    const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-    const int64_t n = (int64_t)blockIdx.x * 32 + c;
+// the column sums of `part`: 16 columns, 64 rows side by side
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float *part, int64_t rows, int64_t N, float *out) {
+    __shared__ float sums[64][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+    const int64_t n = (int64_t)blockIdx.x * 16 + c;
     float v = 0.f;
     if (n < N)
-        for (int64_t b = r; b < rows; b += 8) v += part[b * N + n];
+#pragma unroll 4
+        for (int64_t b = r; b < rows; b += 64) v += part[b * N + n];
     sums[r][c] = v;
     __syncthreads();
     if (r || n >= N) return;
-#pragma unroll
-    for (int i = 1; i < 8; i++) v += sums[i][c];
+#pragma unroll 16
+    for (int i = 1; i < 64; i++) v += sums[i][c];
     out[n] = v;
 }
 
-// Rows of a dz_kernel workgroup.  Up to 1024 rows: all of them, 32 columns wide,
-// and the sums are the bias's gradient at once (a launch less: 4 us of about 30
-// for 256 x 384).  More: 256 columns wide, about 2048 workgroups.
-constexpr int64_t DZ_ONE = 1024;
-int64_t dz_rows(int64_t M, int64_t N) {
-    if (M <= DZ_ONE) return std::max<int64_t>(M, 1);
-    int64_t rows = 8;
-    while (rows < M && ceil_div(M, rows) * ceil_div<int64_t>(N, 256) > 2048) rows *= 2;
-    while (ceil_div(M, rows) > 2048) rows *= 2;
-    return rows;
+// How dz_kernel goes over its matrix.  Up to 1024 rows: 32 columns wide, all
+// rows, and the sums are the bias's gradient at once (a launch less: 4 us of
+// about 30 for 256 x 384).  More: 32 or, past 128 columns, 256 columns wide, at
+// least 64 rows, about 2048 workgroups (13102 x 32 with 8 rows each and one
+// narrow pass over 1638 partial sums: 75 us for all three gradients, so 24).
+struct DzPlan {
+    bool narrow;
+    int64_t rows;
+};
+DzPlan dz_plan(int64_t M, int64_t N) {
+    if (M <= 1024) return {true, std::max<int64_t>(M, 1)};
+    const bool narrow = N <= 128;
+    const int64_t across = ceil_div<int64_t>(N, narrow ? 32 : 256);
+    int64_t rows = 64;
+    while (ceil_div(M, rows) * across > 2048) rows *= 2;
+    return {narrow, rows};
 }
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // How a product runs: its tile and in how many parts k is split.
 struct Plan {
-    int tile = 64;      // rows and columns
+    int rows = 64, cols = 64;  // of a tile
     int splits = 1;
-    int64_t per = 0;    // k of a split
+    int64_t per = 0;           // k of a split
 };
 // The tile and split whose estimated time is least.  A CU's share of the
 // workgroups runs in rounds of as many as it holds; a round takes its stages'
@@ -613,19 +641,20 @@ struct Plan {
 // 2 % off the best measured.
 Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
     struct Form {
-        int tile;
+        int rows, cols;
         double alone, shared, around;
         int holds;
     };
-    static const Form half[] = {{256, 1.8, 1.8, 7, 1}, {128, .76, .53, 4, 2}, {64, .5, .21, 3, 4}};
-    static const Form f32[] = {{128, 2.15, 1.95, 4, 2}, {64, 1.3, .64, 3, 4}};
+    static const Form half[] = {{256, 256, 1.8, 1.8, 7, 1}, {128, 128, .76, .53, 4, 2}, {64, 64, .5, .21, 3, 4}};
+    static const Form f32[] = {{128, 128, 2.15, 1.95, 4, 2}, {64, 128, 1.1, 1.0, 3, 3}, {64, 64, 1.3, .64, 3, 4}};
     const bool wide = type == BERT_AMD_F32;
     const int sk = wide ? 32 : 64;
     Plan best;
+    best.per = 64;
     double least = 1e30;
-    for (int i = 0; i < (wide ? 2 : 3); i++) {
+    for (int i = 0; i < 3; i++) {
         const Form &f = wide ? f32[i] : half[i];
-        const int64_t tiles = ceil_div<int64_t>(M, f.tile) * ceil_div<int64_t>(N, f.tile);
+        const int64_t tiles = ceil_div<int64_t>(M, f.rows) * ceil_div<int64_t>(N, f.cols);
         if (!tiles) continue;
         const int64_t splits[] = {1, 2, 4, 6, 8, 12, 16, 256 / tiles, 512 / tiles, 768 / tiles};
         for (const int64_t n : splits) {
@@ -635,7 +664,7 @@ Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
             const double stages = (double)ceil_div(per, (int64_t)sk);
             const auto round = [&](int64_t wgs) { return stages * std::max(f.alone, wgs * f.shared) + f.around; };
             const double t = each / f.holds * round(f.holds) + (left ? round(left) : 0) + (parts > 1 ? 3 + 2e-6 * parts * M * N : 0);
-            if (t < least) least = t, best.tile = f.tile, best.splits = (int)parts, best.per = per;
+            if (t < least) least = t, best = {f.rows, f.cols, (int)parts, per};
         }
     }
     best.splits = std::max(1, best.splits);
@@ -647,10 +676,11 @@ int64_t split_bytes(int type, int64_t M, int64_t N, int64_t K) {
     return p.splits > 1 ? round256(p.splits * M * N * 4) : 0;
 }
 
-// whether a layer's two gradient products share a launch: both in 64 x 64 tiles
-// (256 x 384 x 384 in f32 29 -> 22 us for all three gradients)
+// whether a layer's two gradient products share a launch: both in the same
+// small tiles (256 x 384 x 384 in f32 29 -> 22 us for all three gradients)
 bool gradients_in_pair(int type, int64_t M, int64_t N, int64_t K) {
-    return M > 0 && plan_for(type, M, K, N).tile == 64 && plan_for(type, N, K, M).tile == 64;
+    const Plan dx = plan_for(type, M, K, N), dw = plan_for(type, N, K, M);
+    return M > 0 && dx.rows == 64 && dw.rows == 64 && dx.cols == dw.cols;
 }
 
 int64_t padded(int type, int64_t n) {
@@ -688,7 +718,7 @@ Product product(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_
     const auto ok = [](const void *q, int64_t ld) { return !q || aligned16(q, ld * (int64_t)sizeof(typename Elem<TYPE>::T)); };
     Product p;
     p.A = A, p.B = B, p.M = M, p.N = N, p.K = K, p.per = plan.per, p.parts = plan.splits;
-    p.tiles = (int)(ceil_div<int64_t>(M, plan.tile) * ceil_div<int64_t>(N, plan.tile));
+    p.tiles = (int)(ceil_div<int64_t>(M, plan.rows) * ceil_div<int64_t>(N, plan.cols));
     p.part = plan.splits > 1 ? (float *)ws : nullptr;
     p.e = e;
     p.vec = ok(e.y, e.ldy) && ok(e.z, e.ldz) && ok(e.r, e.ldr);
@@ -721,7 +751,12 @@ template <typename T>
 hipError_t join(const Product &a, const Product &b, hipStream_t s) {
     const int64_t most = std::max(a.part ? a.M * a.N : 0, b.part ? b.M * b.N : 0);
     if (!most) return hipSuccess;
-    hipLaunchKernelGGL((split_join_kernel<T>), dim3(std::min<int64_t>(1024, ceil_div<int64_t>(most, 256)), b.part ? 2 : 1), dim3(256), 0, s, a, b);
+    const auto four = [](const Product &p) { return !p.part || (p.vec && p.N % 4 == 0); };
+    const int two = b.part ? 2 : 1;
+    if (four(a) && four(b))
+        hipLaunchKernelGGL((split_join_kernel<T, 4>), dim3(std::min<int64_t>(4096, ceil_div<int64_t>(most, 1024)), two), dim3(256), 0, s, a, b);
+    else
+        hipLaunchKernelGGL((split_join_kernel<T, 1>), dim3(std::min<int64_t>(4096, ceil_div<int64_t>(most, 256)), two), dim3(256), 0, s, a, b);
     return hipGetLastError();
 }
 
@@ -731,9 +766,10 @@ hipError_t gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_
     const Plan plan = plan_for(TYPE, M, N, K);
     const Product p = product<TYPE>(A, B, M, N, K, plan, ws, e);
     hipError_t r = hipSuccess;
-    if (plan.tile == 64) r = launch_stage<TYPE, TA, TBT, 64, 64, 2, 1>(p, s);
-    else if (plan.tile == 128) r = launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(p, s);
-    else if constexpr (TYPE != BERT_AMD_F32) r = launch_stage<TYPE, TA, TBT, 256, 256, 2, 4>(p, s);
+    if (plan.cols == 64) r = launch_stage<TYPE, TA, TBT, 64, 64, 2, 1>(p, s);
+    else if (plan.rows == 128) r = launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(p, s);
+    else if constexpr (TYPE == BERT_AMD_F32) r = launch_stage<TYPE, TA, TBT, 64, 128, 2, 2>(p, s);
+    else r = launch_stage<TYPE, TA, TBT, 256, 256, 2, 4>(p, s);
     return r != hipSuccess ? r : join<typename Elem<TYPE>::T>(p, Product(), s);
 }
 
@@ -777,22 +813,23 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         dz = {kept, lddz, true, true};
     }
     if ((kept || a.db) && a.M) {
-        const int64_t rows = dz_rows(a.M, a.N), blocks = ceil_div<int64_t>(a.M, rows);
+        const DzPlan plan = dz_plan(a.M, a.N);
+        const int64_t rows = plan.rows, blocks = ceil_div<int64_t>(a.M, rows);
         float *part = !a.db || blocks == 1 ? a.db : (float *)ws;
         const bool vec = aligned16(a.dy, a.lddy * (int64_t)sizeof(T)) && (!a.act || aligned16(a.z, a.ldz * (int64_t)sizeof(T)));
-        if (a.M <= DZ_ONE)
+        if (plan.narrow)
             hipLaunchKernelGGL((dz_kernel<T, 4>), dim3(ceil_div(a.N, 32), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z,
                                a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, lddz, part, vec);
         else
             hipLaunchKernelGGL((dz_kernel<T, 32>), dim3(ceil_div(a.N, 256), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy,
                                (const T *)a.z, a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, lddz, part, vec);
         if (a.db && blocks > 1) {
-            hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 32)), dim3(256), 0, s, part, blocks, (int64_t)a.N, a.db);
+            hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 16)), dim3(1024), 0, s, part, blocks, (int64_t)a.N, a.db);
             ws += round256(blocks * a.N * 4);
         }
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     } else if (a.db) {
-        hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 32)), dim3(256), 0, s, (const float *)nullptr, (int64_t)0, (int64_t)a.N, a.db);
+        hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 16)), dim3(1024), 0, s, (const float *)nullptr, (int64_t)0, (int64_t)a.N, a.db);
     }
     Epilogue ex, ew;
     ex.y = a.dx, ex.ldy = a.lddx;
@@ -801,10 +838,15 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         Operand wx[] = {operand(a.w, a.ldw, TYPE), operand(a.x, a.ldx, TYPE)};
         const int64_t rows[] = {a.N, a.M};
         if (hipError_t r = pack<T>(TYPE, wx, rows, 2, a.K, ws, s); r != hipSuccess) return r;
-        const Product dx = product<TYPE>(dz, wx[0], a.M, a.K, a.N, plan_for(TYPE, a.M, a.K, a.N), ws, ex);
+        const Plan plan = plan_for(TYPE, a.M, a.K, a.N);
+        const Product dx = product<TYPE>(dz, wx[0], a.M, a.K, a.N, plan, ws, ex);
         ws += split_bytes(TYPE, a.M, a.K, a.N);
         const Product dw = product<TYPE>(dz, wx[1], a.N, a.K, a.M, plan_for(TYPE, a.N, a.K, a.M), ws, ew);
-        hipLaunchKernelGGL((pair_gemm_kernel<TYPE>), dim3(dx.tiles * dx.parts + dw.tiles * dw.parts), dim3(128), stage_lds(64, 64, 2, 1), s, dx, dw);
+        const dim3 grid(dx.tiles * dx.parts + dw.tiles * dw.parts);
+        if (plan.cols == 64)
+            hipLaunchKernelGGL((pair_gemm_kernel<TYPE, 64, 1>), grid, dim3(128), stage_lds(64, 64, 2, 1), s, dx, dw);
+        else if constexpr (TYPE == BERT_AMD_F32)
+            hipLaunchKernelGGL((pair_gemm_kernel<TYPE, 128, 2>), grid, dim3(256), stage_lds(64, 128, 2, 2), s, dx, dw);
         if (hipError_t r = hipGetLastError(); r != hipSuccess) return r;
         return join<T>(dx, dw, s);
     }
@@ -844,7 +886,7 @@ int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K, bool al
     const bool whole_n = aligned && padded(type, N) == N, whole_k = aligned && padded(type, K) == K;
     const int64_t for_dx = (whole_k ? 0 : packed_bytes(type, N, K)) + split_bytes(type, M, K, N);
     const int64_t for_dw = (whole_k ? 0 : packed_bytes(type, M, K)) + split_bytes(type, N, K, M);
-    return (act || !whole_n ? packed_bytes(type, M, N) : 0) + round256(ceil_div<int64_t>(M, dz_rows(M, N)) * N * 4) +
+    return (act || !whole_n ? packed_bytes(type, M, N) : 0) + round256(ceil_div<int64_t>(M, dz_plan(M, N).rows) * N * 4) +
            (gradients_in_pair(type, M, N, K) ? for_dx + for_dw : std::max(for_dx, for_dw));
 }
 

@@ -300,30 +300,14 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortPass p) {
 // over many workgroups.
 constexpr int SUM_TILE = 64, AHEAD = 8;
 
-template <typename T, int COLS>
-__device__ __forceinline__ void load_cols(const T *p, float *v) {
-    if constexpr (COLS == 1) {
-        v[0] = (float)p[0];
-    } else {
-        struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; };
-        const Four f = *(const Four *)p;
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = (float)f.v[i];
-    }
-}
-template <int COLS>
-__device__ __forceinline__ void store_cols(float *p, const float *v) {
-    if constexpr (COLS == 1) p[0] = v[0];
-    else *(f32x4 *)p = f32x4{v[0], v[1], v[2], v[3]};
-}
 // a finished sum into its row of the table
 template <int COLS>
 __device__ __forceinline__ void store_row(const LookupGradArgs &a, int v, int e, const float *sum) {
     float *p = a.dtable + (int64_t)v * a.ldt + e, o[COLS];
-    if (a.accumulate) load_cols<float, COLS>(p, o);
+    if (a.accumulate) get_n<float, COLS>(p, o);
 #pragma unroll
     for (int i = 0; i < COLS; i++) o[i] = a.accumulate ? o[i] + a.scale * sum[i] : a.scale * sum[i];
-    store_cols<COLS>(p, o);
+    put_n<float, COLS>(p, o);
 }
 struct SumArgs {
     const int32_t *key, *place;
@@ -349,7 +333,7 @@ __global__ __launch_bounds__(256) void sum_kernel(LookupGradArgs a, SumArgs s) {
     float now[AHEAD][COLS], then[AHEAD][COLS];
     const auto load = [&](float (&v)[AHEAD][COLS], int at) {  // past the last place: its row again, not used
 #pragma unroll
-        for (int j = 0; j < AHEAD; j++) load_cols<T, COLS>(from + __builtin_amdgcn_readlane(place, min(at + j, count - 1)) * a.ldd, v[j]);
+        for (int j = 0; j < AHEAD; j++) get_n<T, COLS>(from + __builtin_amdgcn_readlane(place, min(at + j, count - 1)) * a.ldd, v[j]);
     };
     if (!count) return;
     load(now, 0);
@@ -362,8 +346,8 @@ __global__ __launch_bounds__(256) void sum_kernel(LookupGradArgs a, SumArgs s) {
             for (int c = 0; c < COLS; c++) sum[c] += now[j][c];
             if (ends >> (at + j) & 1) {
                 const int k = __builtin_amdgcn_readlane(key, at + j);
-                if (from_before) store_cols<COLS>(part, sum);
-                else if (__builtin_amdgcn_readlane(next, at + j) == k) store_cols<COLS>(part + a.E, sum);
+                if (from_before) put_n<float, COLS>(part, sum);
+                else if (__builtin_amdgcn_readlane(next, at + j) == k) put_n<float, COLS>(part + a.E, sum);
                 else store_row<COLS>(a, k, e, sum);
                 from_before = false;
 #pragma unroll
@@ -402,7 +386,7 @@ __global__ __launch_bounds__(256) void join_kernel(LookupGradArgs a, SumArgs s) 
 #pragma unroll 8
         for (int i = g * per; i < min(rows, (g + 1) * per); i++) {
             float v[COLS];
-            load_cols<float, COLS>(head + (int64_t)i * 2 * a.E, v);
+            get_n<float, COLS>(head + (int64_t)i * 2 * a.E, v);
 #pragma unroll
             for (int j = 0; j < COLS; j++) sum[j] += v[j];
         }
@@ -412,7 +396,7 @@ __global__ __launch_bounds__(256) void join_kernel(LookupGradArgs a, SumArgs s) 
     __syncthreads();
     if (g || e >= a.E) return;
     float v[COLS];
-    load_cols<float, COLS>(s.part + ((int64_t)t * 2 + 1) * a.E + e, v);
+    get_n<float, COLS>(s.part + ((int64_t)t * 2 + 1) * a.E + e, v);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -473,7 +457,7 @@ __global__ __launch_bounds__(256) void few_kernel(LookupGradArgs a, ZeroPart z) 
                 float v[AHEAD][COLS] = {};
 #pragma unroll
                 for (int j = 0; j < AHEAD; j++)
-                    if (i + j < count) load_cols<T, COLS>((const T *)a.dout + list[wave][i + j] * a.ldd + e, v[j]);
+                    if (i + j < count) get_n<T, COLS>((const T *)a.dout + list[wave][i + j] * a.ldd + e, v[j]);
 #pragma unroll
                 for (int j = 0; j < AHEAD; j++)
 #pragma unroll
