@@ -577,12 +577,24 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
 #pragma unroll
     for (int i = 0; i < 8; i++) sums[r][c][i] = sum[i];
     __syncthreads();
-    const int64_t col = (int64_t)blockIdx.x * CT * 8 + threadIdx.x;
-    if (threadIdx.x >= CT * 8 || col >= N) return;
+    // eight rows' sums a thread, then (one column of threads: 32 such) those
+    constexpr int COLS = CT * 8, GROUPS = 256 / COLS;
+    const int mine = threadIdx.x % COLS, group = threadIdx.x / COLS;
     float v = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < RT; i++) v += sums[i][threadIdx.x >> 3][threadIdx.x & 7];
-    part[blockIdx.y * N + col] = v;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v += sums[8 * group + i][mine >> 3][mine & 7];
+    if constexpr (GROUPS > 1) {
+        __syncthreads();
+        float *joined = &sums[0][0][0];
+        joined[threadIdx.x] = v;
+        __syncthreads();
+        v = 0.f;
+        if (group == 0)
+#pragma unroll
+            for (int i = 0; i < GROUPS; i++) v += joined[i * COLS + mine];
+    }
+    const int64_t col = (int64_t)blockIdx.x * COLS + mine;
+    if (group == 0 && col < N) part[blockIdx.y * N + col] = v;
 }
 
 // the column sums of `part`: 16 columns, 64 rows side by side
@@ -602,11 +614,10 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const float *part, int
     out[n] = v;
 }
 
-// How dz_kernel goes over its matrix.  Up to 1024 rows: 32 columns wide, all
-// rows, and the sums are the bias's gradient at once (a launch less: 4 us of
-// about 30 for 256 x 384).  More: 32 or, past 128 columns, 256 columns wide, at
-// least 64 rows, about 2048 workgroups (13102 x 32 with 8 rows each and one
-// narrow pass over 1638 partial sums: 75 us for all three gradients, so 24).
+// How dz_kernel goes over its matrix.  Up to 1024 rows: 8 columns wide, all
+// rows, and the sums are the bias's gradient at once (256 x 384 in f32: 32
+// columns wide it took 8.8 us on 12 CUs).  More: 8 or, past 128 columns, 256
+// columns wide, about 2048 workgroups (16384 x 4096 in bf16: 403 MB in 75 us).
 struct DzPlan {
     bool narrow;
     int64_t rows;
@@ -614,8 +625,8 @@ struct DzPlan {
 DzPlan dz_plan(int64_t M, int64_t N) {
     if (M <= 1024) return {true, std::max<int64_t>(M, 1)};
     const bool narrow = N <= 128;
-    const int64_t across = ceil_div<int64_t>(N, narrow ? 32 : 256);
-    int64_t rows = 64;
+    const int64_t across = ceil_div<int64_t>(N, narrow ? 8 : 256);
+    int64_t rows = narrow ? 256 : 64;
     while (ceil_div(M, rows) * across > 2048) rows *= 2;
     return {narrow, rows};
 }
@@ -818,7 +829,7 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         float *part = !a.db || blocks == 1 ? a.db : (float *)ws;
         const bool vec = aligned16(a.dy, a.lddy * (int64_t)sizeof(T)) && (!a.act || aligned16(a.z, a.ldz * (int64_t)sizeof(T)));
         if (plan.narrow)
-            hipLaunchKernelGGL((dz_kernel<T, 4>), dim3(ceil_div(a.N, 32), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z,
+            hipLaunchKernelGGL((dz_kernel<T, 1>), dim3(ceil_div(a.N, 8), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z,
                                a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, lddz, part, vec);
         else
             hipLaunchKernelGGL((dz_kernel<T, 32>), dim3(ceil_div(a.N, 256), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy,
