@@ -16,8 +16,11 @@
 // half a code's step, and rounded to the nearest code it would stay for good.
 // r of a nonzero v is never stored as 0: it divides.
 //
-// Memory bound: 28 bytes an element with f32 states and gradients, 16 with
-// 8-bit states.
+// Memory bound: 28 bytes an element with f32 states and gradients, 14 to 16
+// with 8-bit states.  A wave takes 256 elements, four a lane in whole 16-byte
+// pieces: 22.6 M weights in 101 tensors (f32 states, bf16 copies) 151 us, 4.5
+// TB/s, three launches; 192 M weights with 8-bit states and bf16 gradients 625
+// us, 4.3 TB/s (single elements a lane took 1.7 times as long).
 #include "ops_common.h"
 
 #include <algorithm>

@@ -73,7 +73,9 @@ __device__ __forceinline__ Chunk<T, CH> load_chunk(const T *p, int64_t ld, bool 
 // Up to 8 rows of x, as a server's single requests have them: bound by reading
 // W once, so no tile and no second launch.  A wave takes COLS rows of W, its
 // lanes 16 bytes each of them at a time, and every row of x with them, in f32
-// on the vector units; the lanes' sums are joined by a butterfly.
+// on the vector units; the lanes' sums are joined by a butterfly.  f32 1 x 384
+// x 384: 3.6 us, a launch's own length (in 64 x 64 tiles and parts of k: two
+// launches, 19 us a call instead of 10).
 constexpr int FEW_ROWS = 8;
 
 template <int TYPE, int ROWS, int COLS>
@@ -116,7 +118,9 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Operand X, Operand W, int
 //
 // A matrix whose rows are not aligned, or no whole chunks long, is copied into
 // the workspace with zeros up to the next chunk: one more pass over it, where
-// loads of single elements would slow the whole product down.
+// loads of single elements would slow the whole product down (f16 777 x 1001 x
+// 513: 5.6 us for both copies and 15 for the product, 26 with single loads in
+// the product).
 struct Packing {
     const void *from = nullptr;
     void *to = nullptr;
@@ -160,6 +164,15 @@ __global__ __launch_bounds__(256) void pack_kernel(Packing a, Packing b) {
 // row pieces on the way out.  One or two waves a SIMD have little to hide
 // latencies behind there, so inside the matrix several rows' reads, loads and
 // stores go together without a branch between them.
+//
+// Measured (us): bf16 8192 x 8192 x 8192 861 (1.28 PFLOP/s; all-zero operands
+// run a fifth faster: the chip's power bounds it with the LDS reads, 96 of 128
+// bytes a clock at the full rate); 32768 x 1024 x 4096 270, of which 33 are the
+// way out's LDS passes and 15 its stores; four waves of 128 x 128 each instead
+// of eight of 128 x 64 took 5 % longer.  f32 65536 x 1536 x 384 590 (131
+// TFLOP/s, the matrix units busy 9 parts in 10).  With one workgroup on a CU a
+// wave's LDS reads bound a 128 x 128 stage (0.7 us, its products take 0.25);
+// three or four stages in LDS, or 16 waves, did not change that.
 constexpr uint32_t OUTSIDE = 0x80000000u;       // an offset past every descriptor's range (2^31 bytes)
 
 // until at most LEFT of this wave's loads are on their way
@@ -497,7 +510,7 @@ __global__ __launch_bounds__(128 * WN, 2) void pair_gemm_kernel(Product dx, Prod
 }
 
 // The parts of one or two products (blockIdx.y) added in order, COLS columns a
-// thread.  A product in parts has under 2^31 elements (plan_for).
+// thread: bound by memory (four parts of 4096 x 1024: 75 MB in 14.5 us).  A product in parts has under 2^31 elements (plan_for).
 template <typename T, int COLS>
 __global__ __launch_bounds__(256) void split_join_kernel(Product a, Product b) {
     const Product &p = blockIdx.y ? b : a;
@@ -597,7 +610,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
     if (group == 0 && col < N) part[blockIdx.y * N + col] = v;
 }
 
-// the column sums of `part`: 16 columns, 64 rows side by side
+// the column sums of `part`: 16 columns, 64 rows side by side (256 rows of 4096: 5.3 us, one dependent chain of loads)
 __global__ __launch_bounds__(1024) void column_sum_kernel(const float *part, int64_t rows, int64_t N, float *out) {
     __shared__ float sums[64][17];
     const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
@@ -642,22 +655,22 @@ struct Plan {
 // The tile and split whose estimated time is least.  A CU's share of the
 // workgroups runs in rounds of as many as it holds; a round takes its stages'
 // time and a time around them, and where k is split its parts are joined by
-// another pass (8 bytes a sum and part, at the rate of a copy).  A stage takes
-// `alone` us where a CU has one workgroup, else `shared` us of the CU for each.
+// another pass.  A stage takes `alone` us where a CU has one workgroup, and
+// `more` for each other one.
 // The numbers are fitted to products of 16 .. 65536 rows, 384 .. 4096 wide, in
 // every tile and up to 64 parts (us a call): f32 4096 x 1024 x 1024 75 in 128
 // wide tiles, 76 in 64 wide, 92 in two parts of k; bf16 16384 x 1024 x 1024 37
 // in 256 wide, 40 in 128, 59 in 64; bf16 1536 x 384 over k = 65536 123 in 21
 // parts of 256 wide tiles, 549 unsplit in 64 wide.  The choice was on average
-// 2 % off the best measured.
+// 1 % off the best measured, at most 9 %.
 Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
     struct Form {
         int rows, cols;
-        double alone, shared, around;
+        double alone, more, around;
         int holds;
     };
-    static const Form half[] = {{256, 256, 1.8, 1.8, 7, 1}, {128, 128, .76, .53, 4, 2}, {64, 64, .5, .21, 3, 4}};
-    static const Form f32[] = {{128, 128, 2.15, 1.95, 4, 2}, {64, 128, 1.1, 1.0, 3, 3}, {64, 64, 1.3, .64, 3, 4}};
+    static const Form half[] = {{256, 256, 1.8, 0, 7, 1}, {128, 128, .72, .33, 4, 2}, {64, 64, .5, .11, 3, 4}};
+    static const Form f32[] = {{128, 128, 2.15, 1.72, 4.5, 2}, {64, 128, 1.18, .89, 3, 3}, {64, 64, 1.3, .42, 2.7, 4}};
     const bool wide = type == BERT_AMD_F32;
     const int sk = wide ? 32 : 64;
     Plan best;
@@ -673,8 +686,8 @@ Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
             const int64_t per = std::max<int64_t>(64, ceil_div(ceil_div(K, n), (int64_t)64) * 64), parts = ceil_div(K, per);
             const int64_t each = ceil_div(tiles * parts, (int64_t)256), left = each % f.holds;
             const double stages = (double)ceil_div(per, (int64_t)sk);
-            const auto round = [&](int64_t wgs) { return stages * std::max(f.alone, wgs * f.shared) + f.around; };
-            const double t = each / f.holds * round(f.holds) + (left ? round(left) : 0) + (parts > 1 ? 3 + 2e-6 * parts * M * N : 0);
+            const auto round = [&](int64_t wgs) { return stages * (f.alone + (wgs - 1) * f.more) + f.around; };
+            const double t = each / f.holds * round(f.holds) + (left ? round(left) : 0) + (parts > 1 ? 3.7 + 1.6e-6 * parts * M * N : 0);
             if (t < least) least = t, best = {f.rows, f.cols, (int)parts, per};
         }
     }

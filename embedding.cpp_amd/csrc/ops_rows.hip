@@ -74,7 +74,9 @@ __global__ __launch_bounds__(256) void lookup_any_kernel(LookupArgs a) {
 
 // Eight elements a thread, `lanes` (8 .. 64) neighbours side by side on a row,
 // chosen so that they come out even: bound by memory, and enough rows are on
-// their way at once with no more than that.
+// their way at once with no more than that (131072 x 768 f16 rows of a 250002
+// row table: 62 us, 403 MB read and written at 6.4 TB/s with the rows that
+// caches repeat; one element a thread took 270).
 template <int TYPE, int OUT>
 __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs a, int lanes_log2) {
     const int lanes = 1 << lanes_log2, per = 256 >> lanes_log2, chunks = a.E / 8;
@@ -139,7 +141,8 @@ hipError_t lookup_t(const LookupArgs &a, hipStream_t s) {
 // These launches wait for memory more than they move, so other workgroups of
 // theirs write the zeros of the rows that have no place (most of a table's
 // gradient): the first one clears the rows' marks, the second one's others set
-// them from the ids, the following ones' write.
+// them from the ids, the following ones' write.  131072 places by 18 bits: 5 +
+// 5 + 9 us a digit without the zeros.
 constexpr int TILE = 1024, BINS = 512;
 
 __device__ __forceinline__ int sort_key(int id, int V, int pad) { return id >= 0 && id < V && id != pad ? id : V; }
@@ -297,7 +300,9 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortPass p) {
 // token whose places end within the tile.  A token whose places go on past a
 // tile's end leaves its sums, one row for each tile it has places in, to
 // join_kernel, which adds them in order: a frequent token's long sum is spread
-// over many workgroups.
+// over many workgroups.  131072 x 768 bf16 places of 67705 tokens: 115 us, 409
+// MB read and written at 3.6 TB/s, and 10 us of joins (a workgroup a token
+// instead took 1.6 ms: a token 1200 times in the batch is one chain of loads).
 constexpr int SUM_TILE = 64, AHEAD = 8;
 
 // a finished sum into its row of the table
@@ -408,7 +413,9 @@ __global__ __launch_bounds__(256) void join_kernel(LookupGradArgs a, SumArgs s) 
 // all ids; only a token's first place goes on, its four waves each sum the
 // token's places of a quarter of the ids, in order, and the quarters are added
 // in order.  Again the other workgroups write the zeros, and find out from the
-// ids which rows are in use.
+// ids which rows are in use.  2048 x 384 f32 places of a 30522 row table: 13.9
+// us, 50 MB at 3.6 TB/s, where the sort's launches alone would take 40; looking
+// through all ids grows with their square, 4 us at 4096 and 16 at 8192.
 constexpr int FEW = 4096;
 
 template <int TYPE, int COLS>
