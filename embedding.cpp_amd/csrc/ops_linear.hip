@@ -640,7 +640,7 @@ DzPlan dz_plan(int64_t M, int64_t N) {
     const bool narrow = N <= 128;
     const int64_t across = ceil_div<int64_t>(N, narrow ? 8 : 256);
     int64_t rows = narrow ? 256 : 64;
-    while (ceil_div(M, rows) * across > 2048) rows *= 2;
+    while (rows < M && ceil_div(M, rows) * across > 2048) rows *= 2;
     return {narrow, rows};
 }
 

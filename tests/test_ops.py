@@ -733,6 +733,25 @@ def test_workspace_sizes():
             assert L.bert_amd_lookup_grad_workspace(n, V, 8) >= 0
 
 
+def test_workspace_of_wide_layers():
+    """A layer so wide that one pass over its columns fills the chip: the bias gradient's sums have their room."""
+    L = bertlib.lib()
+    M, N = 1025, 600000  # parts of k take at most 64 M 4 floats here
+    assert L.bert_amd_linear_backward_workspace(0, 0, M, N, 4, 1) >= 4 * N > 4 * 64 * M * 4
+
+
+@gpu
+def test_wide_layer_backward():
+    """More columns than 2048 workgroups take; small integers, so that every f32 sum is exact in any order."""
+    M, N, K = 1100, 530000, 4
+    g = torch.Generator(device="cuda").manual_seed(21)
+    dy, x, w = (torch.randint(-2, 3, shape, generator=g, device="cuda").float() for shape in ((M, N), (M, K), (N, K)))
+    for act in ("none", "relu"):
+        dx, dw, db = bertops.linear_backward(dy, x, w, z=dy, act=act)
+        dz = dy.relu() if act == "relu" else dy
+        assert torch.equal(db, dz.sum(0)) and torch.equal(dw, dz.t() @ x) and torch.equal(dx, dz @ w)
+
+
 def test_refusals_on_tensors():
     """bertops refuses tensors of the wrong kind before it calls the library."""
     x = torch.zeros(4, 8)
