@@ -23,6 +23,12 @@ inline bool aligned16(const void *p, int64_t stride_bytes) {
 template <typename T>
 constexpr T ceil_div(T a, T b) { return (a + b - 1) / b; }
 
+// orders the LDS accesses of a wave's lanes before and after it (no instruction: they run in order)
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // 16 bytes of elements
 template <typename T, int CH>
 struct Chunk {

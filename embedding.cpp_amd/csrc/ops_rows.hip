@@ -276,9 +276,9 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortPass p) {
         }
         const int before = __popcll(same & ((1ull << lane) - 1)), so_far = seen[wave][d];
         rank[j] = so_far + before;
-        __builtin_amdgcn_wave_barrier();  // the wave's reads stay before the count's update by one lane per value
+        wave_sync();  // the wave's reads stay before the count's update by one lane per value
         if (in && before == 0) seen[wave][d] = so_far + __popcll(same);
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
     }
     __syncthreads();
 #pragma unroll
@@ -329,8 +329,11 @@ __global__ __launch_bounds__(256) void sum_kernel(LookupGradArgs a, SumArgs s) {
     const int before = blockIdx.x ? s.key[blockIdx.x * SUM_TILE - 1] : -1;
     const int count = __popcll(__ballot(key < a.V));  // the places without a gradient are the last ones
     const uint64_t ends = __ballot(key != next) | 1ull << (SUM_TILE - 1);
-    const int e = (blockIdx.y * blockDim.x + threadIdx.x) * COLS;
-    if (e >= a.E) return;
+    if (!count) return;
+    // Every lane stays on: a lane past the row's end holds a place that the others
+    // read, so it sums the row's last columns again and stores nothing.
+    const int own = (blockIdx.y * blockDim.x + threadIdx.x) * COLS, e = min(own, a.E - COLS);
+    const bool there = own < a.E;
     const T *from = (const T *)a.dout + e;
     float *part = s.part + (int64_t)blockIdx.x * 2 * a.E + e;
     float sum[COLS] = {};
@@ -340,7 +343,6 @@ __global__ __launch_bounds__(256) void sum_kernel(LookupGradArgs a, SumArgs s) {
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) get_n<T, COLS>(from + __builtin_amdgcn_readlane(place, min(at + j, count - 1)) * a.ldd, v[j]);
     };
-    if (!count) return;
     load(now, 0);
     for (int at = 0; at < count; at += AHEAD) {
         if (at + AHEAD < count) load(then, at + AHEAD);
@@ -350,10 +352,12 @@ __global__ __launch_bounds__(256) void sum_kernel(LookupGradArgs a, SumArgs s) {
 #pragma unroll
             for (int c = 0; c < COLS; c++) sum[c] += now[j][c];
             if (ends >> (at + j) & 1) {
-                const int k = __builtin_amdgcn_readlane(key, at + j);
-                if (from_before) put_n<float, COLS>(part, sum);
-                else if (__builtin_amdgcn_readlane(next, at + j) == k) put_n<float, COLS>(part + a.E, sum);
-                else store_row<COLS>(a, k, e, sum);
+                const int k = __builtin_amdgcn_readlane(key, at + j), after = __builtin_amdgcn_readlane(next, at + j);
+                if (there) {
+                    if (from_before) put_n<float, COLS>(part, sum);
+                    else if (after == k) put_n<float, COLS>(part + a.E, sum);
+                    else store_row<COLS>(a, k, e, sum);
+                }
                 from_before = false;
 #pragma unroll
                 for (int c = 0; c < COLS; c++) sum[c] = 0.f;
