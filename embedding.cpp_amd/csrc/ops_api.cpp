@@ -156,6 +156,10 @@ int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int64_t M, in
     const int64_t need = linear_ws_bytes(type, M, N, K, linear_aligned(x, ldx, type) && linear_aligned(w, ldw, type));
     if (!workspace_ok(workspace, workspace_bytes, need))
         return refuse("bert_amd_linear: workspace is null, misaligned or under %lld bytes", (long long)need);
+    const Matrix room = {"workspace", need ? workspace : nullptr, need, need, false, 1};
+    for (int i = 0; i < 5; i++)
+        if (overlap(room, 1, all[i], rows[i])) return refuse("bert_amd_linear: the workspace overlaps %s", all[i].name);
+    if (overlap(room, 1, vector, 1)) return refuse("bert_amd_linear: the workspace overlaps bias");
     LinearArgs a;
     a.type = type, a.act = act, a.M = M, a.N = N, a.K = K;
     a.x = x, a.w = w, a.r = residual, a.bias = bias, a.y = y, a.z = z, a.ws = workspace;
@@ -199,6 +203,11 @@ int32_t bert_amd_linear_backward(int32_t device, int32_t type, int32_t act, int6
     const int64_t need = linear_grad_ws_bytes(type, act, M, N, K, aligned);
     if (!workspace_ok(workspace, workspace_bytes, need))
         return refuse("bert_amd_linear_backward: workspace is null, misaligned or under %lld bytes", (long long)need);
+    const Matrix room = {"workspace", need ? workspace : nullptr, need, need, false, 1};
+    for (int i = 0; i < 4; i++)
+        if (reads[i] && overlap(room, 1, ins[i], in_rows[i])) return refuse("bert_amd_linear_backward: the workspace overlaps %s", ins[i].name);
+    for (int o = 0; o < 3; o++)
+        if (overlap(room, 1, outs[o], out_rows[o])) return refuse("bert_amd_linear_backward: the workspace overlaps %s", outs[o].name);
     LinearGradArgs a;
     a.type = type, a.act = act, a.M = M, a.N = N, a.K = K;
     a.dy = dy, a.z = z, a.x = x, a.w = w, a.dx = dx, a.dw = dw, a.db = dbias, a.ws = workspace;
@@ -255,6 +264,10 @@ int32_t bert_amd_lookup_grad(int32_t device, int32_t type, int64_t n, int32_t n_
     const int64_t need = lookup_grad_ws_bytes(n, n_rows, width);
     if (!workspace_ok(workspace, workspace_bytes, need))
         return refuse("bert_amd_lookup_grad: workspace is null, misaligned or under %lld bytes", (long long)need);
+    const Matrix room = {"workspace", need ? workspace : nullptr, need, need, false, 1};
+    if (overlap(room, 1, written, n_rows) || overlap(room, 1, {"dout", dout, ldd, width, true, size_of(type)}, n) ||
+        overlap(room, 1, {"ids", ids, n, n, true, 4}, 1))
+        return refuse("bert_amd_lookup_grad: the workspace overlaps dtable, dout or the ids");
     LookupGradArgs a;
     a.type = type, a.n = n, a.V = n_rows, a.E = width, a.dout = dout, a.ldd = ldd, a.ids = ids, a.scale = scale;
     a.pad_id = pad_id, a.accumulate = accumulate != 0, a.dtable = dtable, a.ldt = ldt, a.ws = workspace;
@@ -309,6 +322,14 @@ int32_t bert_amd_adamw_moments(int32_t device, int64_t n, const void *m, const f
     if (n == 0 || (!m_out && !v_out)) return 0;
     if ((m_out && (!m || !m_scale || off(m_scale, 4) || off(m_out, 4))) || (v_out && (!v || !v_scale || off(v_scale, 4) || off(v_out, 4))))
         return refuse("bert_amd_adamw_moments: a null or misaligned pointer");
+    const int64_t blocks = (n + 255) / 256;
+    const Matrix ins[] = {{"m", m_out ? m : nullptr, n, n, true, 1}, {"m_scale", m_out ? m_scale : nullptr, blocks, blocks, true, 4},
+                          {"v", v_out ? v : nullptr, n, n, true, 1}, {"v_scale", v_out ? v_scale : nullptr, blocks, blocks, true, 4}};
+    const Matrix outs[] = {{"m_out", m_out, n, n, false, 4}, {"v_out", v_out, n, n, false, 4}};
+    for (const Matrix &o : outs)
+        for (const Matrix &i : ins)
+            if (overlap(o, 1, i, 1)) return refuse("bert_amd_adamw_moments: %s overlaps %s", o.name, i.name);
+    if (overlap(outs[0], 1, outs[1], 1)) return refuse("bert_amd_adamw_moments: m_out overlaps v_out");
     return on_device("bert_amd_adamw_moments", device, [&] {
         return launch_adamw_moments(n, (const uint8_t *)m, m_scale, (const uint8_t *)v, v_scale, m_out, v_out, (hipStream_t)hip_stream);
     });

@@ -192,10 +192,9 @@ BERT_API int32_t bert_amd_shard_cuts(int32_t n_seqs, const int32_t *n_tokens, in
    at the same time (two streams, two graphs) need one each.  Rows of a matrix
    are `ld*` elements apart (at least its width; 0 for an input: the one row
    again for every row); nothing is written between them.  Results do not
-   depend on the launch: the same inputs give the same bits.  Outputs must not
-   overlap inputs or each other unless a call says so (columns of one wider
-   matrix do not overlap).  Each returns 0, or
-   negative without having launched anything: -1 an invalid argument, -3 a HIP
+   depend on the launch: the same inputs give the same bits.  Outputs and the
+   workspace must not overlap inputs or each other unless a call says so (columns
+   of one wider matrix do not overlap).  Each returns 0, or negative without having launched anything: -1 an invalid argument, -3 a HIP
    error (message via bert_amd_last_error). */
 
 /* element types of the operators' tensors (ggml's numbers, as in the model files) */

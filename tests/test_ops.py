@@ -733,6 +733,28 @@ def test_workspace_sizes():
             assert L.bert_amd_lookup_grad_workspace(n, V, 8) >= 0
 
 
+def test_refusals_of_shared_workspace():
+    """A workspace that lies in what a call reads or writes, and moments that are written over each other."""
+    L, P, NULL = bertlib.lib(), 1 << 24, None
+
+    def refused(rc, word):
+        assert rc == -1 and word in bertlib.last_error(), (rc, bertlib.last_error())
+
+    K = 100000  # parts of k
+    ok = dict(device=0, type=0, act=0, M=40, N=8, K=K, x=P, ldx=K, w=3 * P, ldw=K, bias=5 * P, r=6 * P, ldr=8, y=7 * P, ldy=8, z=8 * P, ldz=8, ws=9 * P, nws=P, s=NULL)
+    need = L.bert_amd_linear_workspace(0, 40, 8, K, 1)
+    for ws, word in ((P, "overlaps x"), (P + 16 * K - 16, "overlaps x"), (3 * P - need + 16, "overlaps w"), (5 * P + 16, "overlaps bias"), (6 * P, "overlaps residual"), (7 * P + 1264, "overlaps y"), (8 * P - need + 16, "overlaps z")):
+        refused(L.bert_amd_linear(*{**ok, "ws": ws}.values()), word)
+    ok = dict(device=0, type=1, act=2, M=40, N=8, K=8, dy=P, lddy=8, z=2 * P, ldz=8, x=3 * P, ldx=8, w=4 * P, ldw=8, dx=5 * P, lddx=8, dw=6 * P, lddw=8, db=7 * P, ws=8 * P, nws=P, s=NULL)
+    for i, word in enumerate(("dy", "z", "x", "w", "dx", "dw", "dbias"), 1):
+        refused(L.bert_amd_linear_backward(*{**ok, "ws": i * P + 16}.values()), "overlaps " + word)
+    ok = dict(device=0, type=0, n=5000, V=10, E=8, dout=P, ldd=8, ids=2 * P, scale=1.0, pad=-1, acc=0, dt=3 * P, ldt=8, ws=4 * P, nws=P, s=NULL)
+    for i in (1, 2, 3):
+        refused(L.bert_amd_lookup_grad(*{**ok, "ws": i * P + 16}.values()), "workspace overlaps")
+    for m_out, v_out, word in ((P, 6 * P, "m_out overlaps m"), (6 * P, 3 * P + 96, "v_out overlaps v"), (2 * P, 6 * P, "m_out overlaps m_scale"), (6 * P, P, "v_out overlaps m"), (6 * P, 6 * P + 396, "overlaps v_out")):
+        refused(L.bert_amd_adamw_moments(0, 100, P, 2 * P, 3 * P, 4 * P, m_out, v_out, NULL), word)
+
+
 def test_workspace_of_wide_layers():
     """A layer so wide that one pass over its columns fills the chip: the bias gradient's sums have their room."""
     L = bertlib.lib()
