@@ -197,7 +197,9 @@ class AdamW:
     weight_decay: one value, or one for each tensor.  copies: for each tensor a float16 / bfloat16 tensor
     that gets its updated values rounded (None: none).  seed: what 8-bit states are rounded by, with the
     step's number added.  The moments are buffers of their own, laid out once: tensor i's begin at
-    where[i], a multiple of 256."""
+    where[i], a multiple of 256; load saved ones with copy_.  Tensors, copies and states stay where they
+    are: step() refuses to run once one has moved.  A step captured in a graph repeats its own number,
+    learning rate and rounding."""
 
     _ROW = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("ms", "u8"), ("vs", "u8"), ("copy", "u8"), ("n", "i8"),
                      ("decay", "f8")])
@@ -246,7 +248,11 @@ class AdamW:
         if self.copies is not None:
             rows["copy"] = [t.data_ptr() for t in self.copies]
         rows["n"], rows["decay"] = sizes, decay
-        self._rows, self._shapes = rows, [t.shape for t in self.params]
+        self._rows, self._shapes, self._at = rows, [t.shape for t in self.params], self._addresses()
+
+    def _addresses(self) -> List[int]:
+        states = [self.m, self.v] + ([self.m_scale, self.v_scale] if self.bits == 8 else [])
+        return [t.data_ptr() for t in (*self.params, *(self.copies or ()), *states)]
 
     def step(self, grads: Sequence[torch.Tensor], grad_scale: Optional[torch.Tensor] = None) -> None:
         """One step; grads: one for each tensor, all of one float type.  grad_scale: one float32 on the device
@@ -257,6 +263,8 @@ class AdamW:
         for g, s in zip(grads, self._shapes):
             if g.dtype != dt or g.shape != s or g.device != dev or not g.is_contiguous():
                 raise ValueError("a gradient has another type, shape or device than the others or its tensor, or is not contiguous")
+        if self._addresses() != self._at:
+            raise ValueError("a tensor, copy or state is no longer where it was when the optimizer was made")
         if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.device != dev or grad_scale.numel() != 1):
             raise ValueError(f"grad_scale has to be one float32 on {dev}")
         self._rows["g"] = [g.data_ptr() for g in grads]

@@ -583,6 +583,33 @@ def test_together_in_a_graph(bits):
 
 
 @gpu
+def test_adamw_refuses_what_has_moved():
+    """Weights, copies and states that got other memory after the optimizer was made."""
+    def made():
+        p = torch.ones(600, device="cuda")
+        return bertops.AdamW([p], bits=8, copies=[p.bfloat16()]), torch.ones(600, device="cuda")
+
+    def move_weights(o):
+        o.params[0].data = torch.ones(600, device="cuda")
+
+    def move_copy(o):
+        o.copies[0] = o.copies[0].clone()
+
+    def move_state(o):
+        o.v_scale = o.v_scale.clone()
+
+    for move in (move_weights, move_copy, move_state):
+        o, g = made()
+        o.step([g])
+        before = [t.clone() for t in (*o.params, *o.copies, o.m, o.v)]
+        move(o)
+        with pytest.raises(ValueError, match="no longer"):
+            o.step([g])
+        torch.cuda.synchronize()
+        assert o.t == 1 and all(torch.equal(a, c) for a, c in zip(before[2:], (o.m, o.v)))
+
+
+@gpu
 def test_two_streams_at_once():
     """The same calls on two streams at a time give what each gives alone."""
     x, w, r, b = (t.cuda() for t in make_layer(700, 384, 384, torch.bfloat16, seed=16))
