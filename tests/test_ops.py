@@ -7,6 +7,9 @@ taken as two 16-bit halves, 22 bits or more of them, which three products leave 
 off; f32 evaluations of the activations by a few 2^-24 of the largest term in them (SLACK of them).
 """
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -580,6 +583,52 @@ def test_together_in_a_graph(bits):
         for o, gr in ((opts[0], want_g), (opts[1], g)):
             o.step(gr)
         assert all(torch.equal(a, c) for a, c in zip(opts[0].params, opts[1].params))
+
+
+FIRST_CALLS = """
+import sys
+sys.path[:0] = sys.argv[1:]
+import torch, bertops
+g = torch.Generator(device="cuda").manual_seed(22)
+def normal(*s, t=torch.float32): return torch.randn(*s, generator=g, device="cuda").to(t)
+x, w, r, b = normal(4100, 520, t=torch.float16), normal(2056, 520, t=torch.float16), normal(4100, 2056, t=torch.float16), normal(2056)
+xs, ws = normal(300, 77), normal(50, 77)
+ids = torch.randint(-1, 700, (9000,), generator=g, device="cuda").int()
+dout = normal(9000, 96, t=torch.bfloat16)
+params = [normal(5000), normal(300, 7)]
+grads = [normal(5000), normal(300, 7)]
+opts = [bertops.AdamW([p.clone() for p in params], bits=bits) for bits in (32, 8) for _ in range(2)]
+def calls(which):
+    out = [bertops.linear(x, w, b, residual=r, act="gelu"), bertops.linear(x[:1], w, b), bertops.linear(xs, ws)]
+    out += bertops.linear_backward(r, x, w, z=r, act="silu")
+    out += [bertops.lookup(w, ids), bertops.lookup_grad(dout, ids, 700), bertops.lookup_grad(dout[:900], ids[:900], 700)]
+    for o in (opts[which], opts[2 + which]):
+        o.t = 4
+        o.step(grads)
+    return out
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls(0)
+for k in range(4):
+    graph.replay()
+    want = calls(1)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want)), k
+    assert all(torch.equal(a, c) for i in (0, 2) for a, c in zip(opts[i].params + list(opts[i].moments()), opts[i + 1].params + list(opts[i + 1].moments()))), k
+    for t in (x, r, dout, grads[0]): t.mul_(-0.75)
+    ids.add_(1)
+    torch.cuda.synchronize()
+print("four replays")
+"""
+
+
+@gpu
+def test_first_calls_are_captured():
+    """A process whose first call of every kernel is recorded into a graph; the replays see new values."""
+    paths = [os.path.dirname(bertops.__file__)]
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS, *paths], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "four replays" in done.stdout, done.stderr[-2000:]
 
 
 @gpu
