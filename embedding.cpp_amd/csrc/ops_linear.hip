@@ -436,6 +436,7 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
                     for (int c = 0; c < 4; c++)
                         *(f32x4 *)(out + (32 * i % WR + (lane & 31)) * OUT_LD + 32 * (j & 1) + 8 * c + 4 * (lane >> 5)) =
                             f32x4{acc[i][j][4 * c], acc[i][j][4 * c + 1], acc[i][j][4 * c + 2], acc[i][j][4 * c + 3]};
+        wave_sync();
         if (vec && !part && m0 + BM <= M && n0 + BN <= N) {
             const T *r = (const T *)e.r + m * e.ldr + n;
             T *y = (T *)e.y + m * e.ldy + n, *z = (T *)e.z + m * e.ldz + n;
@@ -488,6 +489,7 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
                         if (g + i < there) y[i * e.ldy] = (T)(v[i] + add[i]);
                 }
         }
+        wave_sync();
     }
 }
 
