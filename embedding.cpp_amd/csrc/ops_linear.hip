@@ -1,8 +1,8 @@
 // ops_linear.hip — the dense layer y = act(x W^T + b) + r and its gradients
 // dx = dz W, dw = dz^T x, db = sum of dz over rows, with dz = dy act'(z).
 //
-// Sums run in f32 on the matrix units.  A 16-bit layer's dz is rounded to its
-// type before the two products, as the matrix units take 16-bit operands: an
+// Sums run in f32 on the matrix units.  Past 8 rows a 16-bit layer's dz is rounded
+// to its type before the two products, as the matrix units take 16-bit operands: an
 // error of half a step in each term, where the result is rounded by half a
 // step once more; db sums the unrounded dz.
 #include "ops_common.h"
@@ -112,6 +112,120 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Operand X, Operand W, int
         }
     const int64_t n = n0 + lane % COLS;
     if (lane < ROWS * COLS && lane / COLS < M && n < N) epilogue_store<T>(e, lane / COLS, n, v);
+}
+
+// The gradients for as few rows: bound by reading W and writing dw once each, so
+// one kernel does both, with dz in f32 throughout (no rounding between).  A wave
+// takes 4 rows of W at a time, each lane one of the 8 x 4 dz that belong to
+// them, then 4 elements of each row: a rank-ROWS dw leaves at once, dx stays in
+// registers, is joined over the workgroup's waves in LDS and over the
+// workgroups along N by split_join_kernel, in order.  All three gradients with
+// tanh, us a call (in tiles: dz, both products and a join): f32 1 x 384 x 384 8
+// (13), 8 x 1024 x 1024 13 (16), 8 x 4096 x 4096 36 (62); bf16 14 (11.4) and 40
+// (33) for the latter two, kept for the dz, as over so few terms its rounding
+// showed (up to 1.67 times the error of the result's own).
+struct FewGrads {
+    const void *dy, *z;
+    int64_t lddy, ldz;
+    int act, M;
+    int64_t N, K, rows;  // rows: of W in a workgroup, a multiple of 32
+    Operand x, w;
+    void *dw;            // or null: not wanted
+    int64_t lddw;
+    bool vec;            // dw's rows are aligned
+    float *db, *part;    // or null
+};
+constexpr int FEW_COLS = 4;
+// FEW_COLS elements of row r from column c of a [nr][nc] matrix
+template <typename T>
+__device__ __forceinline__ void load_few(const Operand &o, int64_t r, int64_t c, int64_t nr, int64_t nc, T *v) {
+    const T *p = (const T *)o.p + r * o.ld + c;
+    if (r < nr && o.vec && c + FEW_COLS <= nc) {
+        get_n<T, FEW_COLS>(p, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < FEW_COLS; j++) v[j] = r < nr && c + j < nc ? p[j] : (T)0.f;
+    }
+}
+template <int TYPE, int ROWS>
+__global__ __launch_bounds__(512) void few_rows_grad_kernel(FewGrads a) {
+    typedef typename Elem<TYPE>::T T;
+    constexpr int CH = FEW_COLS, EACH = ROWS * CH;
+    __shared__ float sums[4][EACH][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t k = ((int64_t)blockIdx.x * 64 + lane) * CH, end = min(a.N, (int64_t)(blockIdx.y + 1) * a.rows);
+    float x[ROWS][CH] = {}, dx[ROWS][CH] = {};
+    if (a.dw)
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            T v[CH];
+            load_few(a.x, r, k, a.M, a.K, v);
+#pragma unroll
+            for (int c = 0; c < CH; c++) x[r][c] = (float)v[c];
+        }
+    for (int64_t n0 = (int64_t)blockIdx.y * a.rows + 4 * wave; n0 < end; n0 += 32) {
+        T w[4][CH] = {};
+        if (a.part)
+#pragma unroll
+            for (int j = 0; j < 4; j++) load_few(a.w, n0 + j, k, a.N, a.K, w[j]);
+        const int m = lane >> 2;
+        const int64_t n = n0 + (lane & 3);
+        float dz = 0.f;
+        if (m < a.M && n < a.N) {
+            dz = (float)((const T *)a.dy)[m * a.lddy + n];
+            if (a.act) dz *= act_slope_f((float)((const T *)a.z)[m * a.ldz + n], a.act);
+        }
+        if (a.db && blockIdx.x == 0) {
+            float v = dz;
+#pragma unroll
+            for (int d = 4; d < 64; d <<= 1) v += __shfl_xor(v, d);
+            if (lane < 4 && n < a.N) a.db[n] = v;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float g[ROWS], v[CH] = {};
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) g[r] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(dz), 4 * r + j));
+#pragma unroll
+            for (int r = 0; r < ROWS; r++)
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    v[c] = __builtin_fmaf(g[r], x[r][c], v[c]);
+                    dx[r][c] = __builtin_fmaf(g[r], (float)w[j][c], dx[r][c]);
+                }
+            if (!a.dw || n0 + j >= a.N) continue;
+            T *to = (T *)a.dw + (n0 + j) * a.lddw + k;
+            if (a.vec && k + CH <= a.K) {
+                put_n<T, CH>(to, v);
+            } else {
+#pragma unroll
+                for (int c = 0; c < CH; c++)
+                    if (k + c < a.K) to[c] = (T)v[c];
+            }
+        }
+    }
+    if (!a.part) return;
+    const auto leave = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < EACH; i++) sums[at][i][lane] = dx[i / CH][i % CH];
+    };
+    const auto take = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < EACH; i++) dx[i / CH][i % CH] += sums[at][i][lane];
+    };
+#pragma unroll 1
+    for (int half = 4; half; half >>= 1) {
+        if (wave >= half && wave < 2 * half) leave(wave - half);
+        __syncthreads();
+        if (wave < half) take(wave);
+        __syncthreads();
+    }
+    if (wave) return;
+#pragma unroll
+    for (int r = 0; r < ROWS; r++)
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+            if (r < a.M && k + c < a.K) a.part[((int64_t)blockIdx.y * a.M + r) * a.K + k + c] = dx[r][c];
 }
 
 // ---- rows in whole chunks -------------------------------------------------------
@@ -709,6 +823,15 @@ bool gradients_in_pair(int type, int64_t M, int64_t N, int64_t K) {
     return M > 0 && dx.rows == 64 && dw.rows == 64 && dx.cols == dw.cols;
 }
 
+// Up to 8 rows, and no more than 8192 columns of dz: with more the tiles' workgroups
+// win (bf16 1 x 768 x 65536: 67 us, 134 here) and dz's roundings average out.
+bool few_grads(int64_t M, int64_t N) { return M > 0 && M <= FEW_ROWS && N <= 8192; }
+// workgroups along N, at most 64, as their sums are joined one after the other
+int64_t few_grad_parts(int64_t N, int64_t K) {
+    const int64_t across = ceil_div<int64_t>(K, 64 * FEW_COLS);
+    return std::min(ceil_div(N, (int64_t)32), std::max((int64_t)8, std::min((int64_t)64, 256 / across)));
+}
+
 int64_t padded(int type, int64_t n) {
     const int64_t ch = 16 / elem_size(type);
     return (n + ch - 1) / ch * ch;
@@ -827,8 +950,31 @@ hipError_t linear_t(const LinearArgs &a, hipStream_t s) {
 }
 
 template <int TYPE>
+hipError_t few_rows_grad(const LinearGradArgs &a, hipStream_t s) {
+    typedef typename Elem<TYPE>::T T;
+    const int64_t e = sizeof(T), parts = few_grad_parts(a.N, a.K);
+    FewGrads f = {};
+    f.dy = a.dy, f.z = a.z, f.lddy = a.lddy, f.ldz = a.ldz, f.act = a.act, f.M = (int)a.M, f.N = a.N, f.K = a.K;
+    f.rows = ceil_div(ceil_div<int64_t>(a.N, parts), (int64_t)32) * 32;
+    f.x = operand(a.x, a.ldx, TYPE), f.w = operand(a.w, a.ldw, TYPE);
+    f.dw = a.dw, f.lddw = a.lddw, f.vec = aligned16(a.dw, a.lddw * e), f.db = a.db;
+    f.part = a.dx ? (float *)a.ws : nullptr;
+    const dim3 grid(a.dx || a.dw ? ceil_div(a.K, 64 * FEW_COLS) : 1, ceil_div<int64_t>(a.N, f.rows));
+    if (a.M == 1) hipLaunchKernelGGL((few_rows_grad_kernel<TYPE, 1>), grid, dim3(512), 0, s, f);
+    else if (a.M == 2) hipLaunchKernelGGL((few_rows_grad_kernel<TYPE, 2>), grid, dim3(512), 0, s, f);
+    else if (a.M <= 4) hipLaunchKernelGGL((few_rows_grad_kernel<TYPE, 4>), grid, dim3(512), 0, s, f);
+    else hipLaunchKernelGGL((few_rows_grad_kernel<TYPE, 8>), grid, dim3(512), 0, s, f);
+    if (hipError_t r = hipGetLastError(); r != hipSuccess) return r;
+    Product dx;
+    dx.M = a.M, dx.N = a.K, dx.parts = (int)grid.y, dx.part = f.part;
+    dx.e.y = a.dx, dx.e.ldy = a.lddx, dx.vec = aligned16(a.dx, a.lddx * e);
+    return join<T>(dx, Product(), s);
+}
+
+template <int TYPE>
 hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
     typedef typename Elem<TYPE>::T T;
+    if (few_grads(a.M, a.N)) return few_rows_grad<TYPE>(a, s);
     char *ws = (char *)a.ws;
     Operand dz = operand(a.dy, a.lddy, TYPE);
     T *kept = nullptr;
@@ -909,6 +1055,7 @@ hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
 }
 
 int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K, bool aligned) {
+    if (few_grads(M, N)) return round256(few_grad_parts(N, K) * M * K * 4);
     const bool whole_n = aligned && padded(type, N) == N, whole_k = aligned && padded(type, K) == K;
     const int64_t for_dx = (whole_k ? 0 : packed_bytes(type, N, K)) + split_bytes(type, M, K, N);
     const int64_t for_dw = (whole_k ? 0 : packed_bytes(type, M, K)) + split_bytes(type, N, K, M);

@@ -210,6 +210,26 @@ def test_linear_backward(M, K, N, pad, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N,pad", [(1, 25, 133, 0), (1, 768, 1, 0), (2, 32, 32, 3), (4, 2144, 33, 8), (5, 513, 2100, 0), (7, 8, 8192, 0), (8, 1000, 777, 5), (8, 4096, 4096, 0)])
+def test_few_rows_backward(M, K, N, pad, dtype):
+    """Up to 8 rows dz is not rounded before the products: only sums in f32 and each result's own rounding remain."""
+    dt = DTYPES[dtype]
+    x, w, dy, _ = make_layer(M, K, N, dt, seed=23)
+    z = normal(gen(24), M, N).to(dt)
+    dev = (lambda t: strided(t.cuda(), pad)) if pad else (lambda t: t.cuda())
+    for act in bertops.ACTS:
+        dx, dw, db = bertops.linear_backward(dev(dy), dev(x), dev(w), z=dev(z), act=act)
+        at = z.to(F64).clone().requires_grad_(True)
+        (dz,) = torch.autograd.grad(act64(at, act), at, dy.to(F64))
+        off = SLACK * U32 * (1 + z.to(F64).abs()) * dy.to(F64).abs() * (act != "none")
+        for got, a, o, b, n, what in ((dx, dz, off, w, N, "dx"), (dw, dz.t(), off.t(), x, M, "dw")):
+            want, far = a @ b.to(F64), (o + (n + 1) * U32 * (a.abs() + o)) @ b.to(F64).abs()
+            close(got, want, far + u(dt) * (want.abs() + far) + tiny(dt), f"{what} {act}")
+        close(db, dz.sum(0), off.sum(0) + (M + 1) * U32 * (dz.abs() + off).sum(0), f"db {act}")
+
+
+@gpu
 def test_linear_backward_by_differences():
     """The loss sum(c y) changes along each input as its gradient says."""
     M, K, N = 6, 11, 9
