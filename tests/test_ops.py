@@ -911,3 +911,44 @@ def test_refusals_on_the_gpu():
                  lambda: bertops.AdamW([x]).step([x], torch.ones(2, device="cuda")), lambda: bertops.Adapter(4).step(), lambda: bertops.Adapter(4).backward(x)):
         with pytest.raises(ValueError):
             call()
+
+
+# ---- the dense layer's bounds without room to spare
+
+
+def rounded_between(v, off, dtype):
+    """v rounded to `dtype` in 64 bits, and how far apart the roundings of v - off and v + off are."""
+    lo, hi = ((v + s * off).to(dtype).to(F64) for s in (-1, 1))
+    return v.to(dtype).to(F64), hi - lo
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N,pad", [(1, 40, 9000, 0), (5, 72, 8200, 3), (8, 8, 9001, 0), (9, 96, 130, 0), (12, 1000, 48, 1), (40, 384, 384, 0), (63, 130, 257, 8), (64, 512, 64, 0), (700, 256, 512, 0)])
+def test_linear_backward_rounds_dz_once(M, K, N, pad, dtype):
+    """Past 8 rows or 8192 columns: dz rounded to the layer's type (f32: not at all), and from there on nothing is
+    lost but sums in f32 and each result's own rounding.  f32 operands are taken whole."""
+    dt = DTYPES[dtype]
+    x, w, dy, _ = make_layer(M, K, N, dt, seed=30)
+    z = normal(gen(31), M, N).to(dt)
+    dev = (lambda t: strided(t.cuda(), pad)) if pad else (lambda t: t.cuda())
+    for act in bertops.ACTS:
+        dx, dw, db = bertops.linear_backward(dev(dy), dev(x), dev(w), z=dev(z), act=act)
+        at = z.to(F64).clone().requires_grad_(True)
+        (dz,) = torch.autograd.grad(act64(at, act), at, dy.to(F64))
+        off = SLACK * U32 * (1 + z.to(F64).abs()) * dy.to(F64).abs() * (act != "none")
+        kept, apart = rounded_between(dz, off, dt) if dt != torch.float32 else (dz, off)
+        for got, a, o, b, n, what in ((dx, kept, apart, w, N, "dx"), (dw, kept.t(), apart.t(), x, M, "dw")):
+            want, far = a @ b.to(F64), (o + (n + 1) * U32 * (a.abs() + o)) @ b.to(F64).abs()
+            close(got, want, far + u(dt) * (want.abs() + far) + tiny(dt), f"{what} {act}")
+        close(db, dz.sum(0), off.sum(0) + (M + 1) * U32 * (dz.abs() + off).sum(0), f"db {act}")
+
+
+@gpu
+@pytest.mark.parametrize("M,K,N", [(1, 1000, 300), (8, 384, 384), (9, 130, 70), (300, 384, 384), (1030, 520, 260)])
+def test_linear_f32_operands_are_taken_whole(M, K, N):
+    """f32 sums: at most K + 2 roundings of the terms' magnitudes, none for the operands."""
+    x, w, _, b = make_layer(M, K, N, torch.float32, seed=32)
+    y = bertops.linear(x.cuda(), w.cuda(), b.cuda())
+    terms = x.to(F64).abs() @ w.to(F64).abs().t() + b.to(F64).abs()
+    close(y, x.to(F64) @ w.to(F64).t() + b.to(F64), (K + 2) * U32 * terms, "y")
