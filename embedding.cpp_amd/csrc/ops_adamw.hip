@@ -233,18 +233,12 @@ __global__ __launch_bounds__(256) void moments_kernel(int64_t n, const uint8_t *
 }
 
 template <int GRAD, int COPY>
-void launch_table(const Table &a, int64_t chunks, int bits, hipStream_t s) {
-    if (bits == 8)
-        hipLaunchKernelGGL((adamw_kernel<GRAD, COPY, 8>), dim3(chunks), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL((adamw_kernel<GRAD, COPY, 32>), dim3(chunks), dim3(256), 0, s, a);
+hipError_t launch_table(const Table &a, int64_t chunks, int bits, hipStream_t s) {
+    return launch(bits == 8 ? adamw_kernel<GRAD, COPY, 8> : adamw_kernel<GRAD, COPY, 32>, dim3(chunks), dim3(256), 0, s, a);
 }
 template <int GRAD>
-void launch_table(const Table &a, int64_t chunks, int copy_type, int bits, hipStream_t s) {
-    if (copy_type == BERT_AMD_F16)
-        launch_table<GRAD, BERT_AMD_F16>(a, chunks, bits, s);
-    else
-        launch_table<GRAD, BERT_AMD_BF16>(a, chunks, bits, s);
+hipError_t launch_table(const Table &a, int64_t chunks, int copy_type, int bits, hipStream_t s) {
+    return copy_type == BERT_AMD_F16 ? launch_table<GRAD, BERT_AMD_F16>(a, chunks, bits, s) : launch_table<GRAD, BERT_AMD_BF16>(a, chunks, bits, s);
 }
 
 }  // namespace
@@ -261,12 +255,10 @@ hipError_t launch_adamw(const AdamwArgs &a, hipStream_t s) {
     for (int i = 0; i <= a.n_tensors; i++) {
         const int64_t more = i < a.n_tensors ? ceil_div<int64_t>(a.t[i].n, CHUNK) : 0;
         if (t.count == TENSORS || (t.count && (i == a.n_tensors || chunks + more > MAX_CHUNKS))) {
-            switch (a.grad_type) {
-                case BERT_AMD_F32: launch_table<BERT_AMD_F32>(t, chunks, a.copy_type, a.bits, s); break;
-                case BERT_AMD_F16: launch_table<BERT_AMD_F16>(t, chunks, a.copy_type, a.bits, s); break;
-                default: launch_table<BERT_AMD_BF16>(t, chunks, a.copy_type, a.bits, s); break;
-            }
-            if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+            const hipError_t e = a.grad_type == BERT_AMD_F32   ? launch_table<BERT_AMD_F32>(t, chunks, a.copy_type, a.bits, s)
+                                 : a.grad_type == BERT_AMD_F16 ? launch_table<BERT_AMD_F16>(t, chunks, a.copy_type, a.bits, s)
+                                                               : launch_table<BERT_AMD_BF16>(t, chunks, a.copy_type, a.bits, s);
+            if (e != hipSuccess) return e;
             t.count = 0, chunks = 0;
         }
         if (i == a.n_tensors) break;
@@ -285,9 +277,8 @@ hipError_t launch_adamw(const AdamwArgs &a, hipStream_t s) {
 hipError_t launch_adamw_moments(int64_t n, const uint8_t *m, const float *ms, const uint8_t *v, const float *vs, float *m_out,
                                 float *v_out, hipStream_t s) {
     const bool vec = !(((uintptr_t)m | (uintptr_t)v) & 3) && !(((uintptr_t)m_out | (uintptr_t)v_out) & 15);
-    hipLaunchKernelGGL(moments_kernel, dim3(std::min<int64_t>(1 << 16, ceil_div<int64_t>(n, 1024))), dim3(256), 0, s, n, m, ms, v, vs, m_out,
-                       v_out, vec);
-    return hipGetLastError();
+    return launch(moments_kernel, dim3(std::min<int64_t>(1 << 16, ceil_div<int64_t>(n, 1024))), dim3(256), 0, s, n, m, ms, v, vs, m_out, v_out,
+                  vec);
 }
 
 }  // namespace bertamd

@@ -37,6 +37,7 @@ int32_t on_device(const char *who, int32_t device, const F &launch) {
         if (before != device) (void)hipSetDevice(before);
     }
     if (e == hipSuccess) return 0;
+    (void)hipGetLastError();  // reported here: not left for the thread's next caller to find
     refuse("%s: %s", who, hipGetErrorString(e));
     return -3;
 }

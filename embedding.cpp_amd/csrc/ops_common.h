@@ -23,6 +23,15 @@ inline bool aligned16(const void *p, int64_t stride_bytes) {
 template <typename T>
 constexpr T ceil_div(T a, T b) { return (a + b - 1) / b; }
 
+// A kernel's launch and its own status: hipGetLastError() behind a launch would
+// also give what an earlier call on this thread, anyone's, has left there.
+template <typename T> struct AsIs { typedef T type; };
+template <typename... P>
+hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, uint32_t lds, hipStream_t s, typename AsIs<P>::type... args) {
+    void *each[] = {&args...};
+    return hipLaunchKernel((const void *)kernel, grid, block, each, lds, s);
+}
+
 // orders the LDS accesses of a wave's lanes before and after it (no instruction: they run in order)
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -861,8 +861,7 @@ hipError_t pack(int type, Operand *o, const int64_t *rows, int n, int64_t cols, 
         ws += packed_bytes(type, rows[i], cols);
     }
     if (!most) return hipSuccess;
-    hipLaunchKernelGGL((pack_kernel<T>), dim3(std::min<int64_t>(1 << 14, ceil_div<int64_t>(most, 256)), count), dim3(256), 0, s, p[0], p[1]);
-    return hipGetLastError();
+    return launch(pack_kernel<T>, dim3(std::min<int64_t>(1 << 14, ceil_div<int64_t>(most, 256)), count), dim3(256), 0, s, p[0], p[1]);
 }
 
 template <int TYPE>
@@ -895,8 +894,7 @@ hipError_t launch_stage(const Product &p, hipStream_t s) {
             asked.fetch_or(bit, std::memory_order_relaxed);
         }
     }
-    hipLaunchKernelGGL(k, dim3(p.tiles, 1, p.parts), dim3(WM * WN * 64), lds, s, p);
-    return hipGetLastError();
+    return launch(k, dim3(p.tiles, 1, p.parts), dim3(WM * WN * 64), lds, s, p);
 }
 
 template <typename T>
@@ -906,10 +904,8 @@ hipError_t join(const Product &a, const Product &b, hipStream_t s) {
     const auto four = [](const Product &p) { return !p.part || (p.vec && p.N % 4 == 0); };
     const int two = b.part ? 2 : 1;
     if (four(a) && four(b))
-        hipLaunchKernelGGL((split_join_kernel<T, 4>), dim3(std::min<int64_t>(4096, ceil_div<int64_t>(most, 1024)), two), dim3(256), 0, s, a, b);
-    else
-        hipLaunchKernelGGL((split_join_kernel<T, 1>), dim3(std::min<int64_t>(4096, ceil_div<int64_t>(most, 256)), two), dim3(256), 0, s, a, b);
-    return hipGetLastError();
+        return launch(split_join_kernel<T, 4>, dim3(std::min<int64_t>(4096, ceil_div<int64_t>(most, 1024)), two), dim3(256), 0, s, a, b);
+    return launch(split_join_kernel<T, 1>, dim3(std::min<int64_t>(4096, ceil_div<int64_t>(most, 256)), two), dim3(256), 0, s, a, b);
 }
 
 // C = A B^T of two matrices in whole chunks
@@ -931,11 +927,10 @@ template <int TYPE, int COLS>
 hipError_t few_rows(const Operand &x, const Operand &w, const LinearArgs &a, const Epilogue &e, hipStream_t s) {
     const dim3 grid(ceil_div(a.N, 4 * COLS));
     const int M = (int)a.M;
-    if (M == 1) hipLaunchKernelGGL((few_rows_kernel<TYPE, 1, COLS>), grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
-    else if (M == 2) hipLaunchKernelGGL((few_rows_kernel<TYPE, 2, COLS>), grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
-    else if (M <= 4) hipLaunchKernelGGL((few_rows_kernel<TYPE, 4, COLS>), grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
-    else hipLaunchKernelGGL((few_rows_kernel<TYPE, 8, COLS>), grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
-    return hipGetLastError();
+    if (M == 1) return launch(few_rows_kernel<TYPE, 1, COLS>, grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
+    if (M == 2) return launch(few_rows_kernel<TYPE, 2, COLS>, grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
+    if (M <= 4) return launch(few_rows_kernel<TYPE, 4, COLS>, grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
+    return launch(few_rows_kernel<TYPE, 8, COLS>, grid, dim3(256), 0, s, x, w, M, a.N, a.K, e);
 }
 
 template <int TYPE>
@@ -963,11 +958,11 @@ hipError_t few_rows_grad(const LinearGradArgs &a, hipStream_t s) {
     f.dw = a.dw, f.lddw = a.lddw, f.vec = aligned16(a.dw, a.lddw * e), f.db = a.db;
     f.part = a.dx ? (float *)a.ws : nullptr;
     const dim3 grid(a.dx || a.dw ? ceil_div(a.K, 64 * FEW_COLS) : 1, ceil_div<int64_t>(a.N, f.rows));
-    if (a.M == 1) hipLaunchKernelGGL((few_rows_grad_kernel<TYPE, 1>), grid, dim3(512), 0, s, f);
-    else if (a.M == 2) hipLaunchKernelGGL((few_rows_grad_kernel<TYPE, 2>), grid, dim3(512), 0, s, f);
-    else if (a.M <= 4) hipLaunchKernelGGL((few_rows_grad_kernel<TYPE, 4>), grid, dim3(512), 0, s, f);
-    else hipLaunchKernelGGL((few_rows_grad_kernel<TYPE, 8>), grid, dim3(512), 0, s, f);
-    if (hipError_t r = hipGetLastError(); r != hipSuccess) return r;
+    const auto kernel = a.M == 1   ? few_rows_grad_kernel<TYPE, 1>
+                        : a.M == 2 ? few_rows_grad_kernel<TYPE, 2>
+                        : a.M <= 4 ? few_rows_grad_kernel<TYPE, 4>
+                                   : few_rows_grad_kernel<TYPE, 8>;
+    if (hipError_t r = launch(kernel, grid, dim3(512), 0, s, f); r != hipSuccess) return r;
     Product dx;
     dx.M = a.M, dx.N = a.K, dx.parts = (int)grid.y, dx.part = f.part;
     dx.e.y = a.dx, dx.e.ldy = a.lddx, dx.vec = aligned16(a.dx, a.lddx * e);
@@ -992,19 +987,18 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         const int64_t rows = plan.rows, blocks = ceil_div<int64_t>(a.M, rows);
         float *part = !a.db || blocks == 1 ? a.db : (float *)ws;
         const bool vec = aligned16(a.dy, a.lddy * (int64_t)sizeof(T)) && (!a.act || aligned16(a.z, a.ldz * (int64_t)sizeof(T)));
-        if (plan.narrow)
-            hipLaunchKernelGGL((dz_kernel<T, 1>), dim3(ceil_div(a.N, 8), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z,
-                               a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, lddz, part, vec);
-        else
-            hipLaunchKernelGGL((dz_kernel<T, 32>), dim3(ceil_div(a.N, 256), blocks), dim3(256), 0, s, (const T *)a.dy, a.lddy,
-                               (const T *)a.z, a.ldz, a.act, a.M, (int64_t)a.N, rows, kept, lddz, part, vec);
+        const auto kernel = plan.narrow ? dz_kernel<T, 1> : dz_kernel<T, 32>;
+        const dim3 grid(ceil_div(a.N, plan.narrow ? 8 : 256), blocks);
+        if (hipError_t r = launch(kernel, grid, dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z, a.ldz, a.act, a.M, a.N, rows, kept,
+                                  lddz, part, vec);
+            r != hipSuccess)
+            return r;
         if (a.db && blocks > 1) {
-            hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 16)), dim3(1024), 0, s, part, blocks, (int64_t)a.N, a.db);
+            if (hipError_t r = launch(column_sum_kernel, dim3(ceil_div(a.N, 16)), dim3(1024), 0, s, part, blocks, a.N, a.db); r != hipSuccess) return r;
             ws += round256(blocks * a.N * 4);
         }
-        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     } else if (a.db) {
-        hipLaunchKernelGGL(column_sum_kernel, dim3(ceil_div(a.N, 16)), dim3(1024), 0, s, (const float *)nullptr, (int64_t)0, (int64_t)a.N, a.db);
+        if (hipError_t r = launch(column_sum_kernel, dim3(ceil_div(a.N, 16)), dim3(1024), 0, s, nullptr, 0, a.N, a.db); r != hipSuccess) return r;
     }
     Epilogue ex, ew;
     ex.y = a.dx, ex.ldy = a.lddx;
@@ -1018,12 +1012,12 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         ws += split_bytes(TYPE, a.M, a.K, a.N);
         const Product dw = product<TYPE>(dz, wx[1], a.N, a.K, a.M, plan_for(TYPE, a.N, a.K, a.M), ws, ew);
         const dim3 grid(dx.tiles * dx.parts + dw.tiles * dw.parts);
+        hipError_t r = hipErrorInvalidValue;
         if (plan.cols == 64)
-            hipLaunchKernelGGL((pair_gemm_kernel<TYPE, 64, 1>), grid, dim3(128), stage_lds(64, 64, 2, 1), s, dx, dw);
+            r = launch(pair_gemm_kernel<TYPE, 64, 1>, grid, dim3(128), stage_lds(64, 64, 2, 1), s, dx, dw);
         else if constexpr (TYPE == BERT_AMD_F32)
-            hipLaunchKernelGGL((pair_gemm_kernel<TYPE, 128, 2>), grid, dim3(256), stage_lds(64, 128, 2, 2), s, dx, dw);
-        if (hipError_t r = hipGetLastError(); r != hipSuccess) return r;
-        return join<T>(dx, dw, s);
+            r = launch(pair_gemm_kernel<TYPE, 128, 2>, grid, dim3(256), stage_lds(64, 128, 2, 2), s, dx, dw);
+        return r != hipSuccess ? r : join<T>(dx, dw, s);
     }
     if (a.dx && a.M) {
         char *rest = ws;
@@ -1038,7 +1032,7 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         if (hipError_t r = pack<T>(TYPE, &x, &a.M, 1, a.K, rest, s); r != hipSuccess) return r;
         if (hipError_t r = gemm<TYPE, true, true>(dz, x, a.N, a.K, a.M, rest, ew, s); r != hipSuccess) return r;
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace

@@ -113,11 +113,8 @@ hipError_t lookup_tt(const LookupArgs &a, hipStream_t s) {
     const bool whole = a.E % 8 == 0 && (BLOCKS || aligned16(a.table, a.ld_bytes)) && aligned16(a.out, a.ldo * (int64_t)sizeof(typename Elem<OUT>::T));
     const int l = row_lanes_log2(a.E / 8);
     const int64_t groups = ceil_div<int64_t>(a.n, 256 >> l);
-    if (whole && groups <= 1 << 23)
-        hipLaunchKernelGGL((lookup_kernel<TYPE, OUT>), dim3(groups), dim3(256), 0, s, a, l);
-    else
-        hipLaunchKernelGGL((lookup_any_kernel<TYPE, OUT>), dim3(std::min<int64_t>(1 << 20, ceil_div<int64_t>(a.n * a.E, 256))), dim3(256), 0, s, a);
-    return hipGetLastError();
+    if (whole && groups <= 1 << 23) return launch(lookup_kernel<TYPE, OUT>, dim3(groups), dim3(256), 0, s, a, l);
+    return launch(lookup_any_kernel<TYPE, OUT>, dim3(std::min<int64_t>(1 << 20, ceil_div<int64_t>(a.n * a.E, 256))), dim3(256), 0, s, a);
 }
 
 template <int TYPE>
@@ -515,15 +512,13 @@ template <int TYPE, int COLS>
 hipError_t sum_t(const LookupGradArgs &a, const SumArgs &p, hipStream_t s) {
     const int threads = std::min(256, ceil_div(ceil_div(a.E, COLS), 64) * 64);
     const int across = ceil_div(ceil_div(a.E, COLS), threads);
-    hipLaunchKernelGGL((sum_kernel<TYPE, COLS>), dim3(p.tiles, across), dim3(threads), 0, s, a, p);
-    hipLaunchKernelGGL((join_kernel<COLS>), dim3(p.tiles, ceil_div(a.E, 64 * COLS)), dim3(256), 0, s, a, p);
-    return hipGetLastError();
+    if (hipError_t e = launch(sum_kernel<TYPE, COLS>, dim3(p.tiles, across), dim3(threads), 0, s, a, p); e != hipSuccess) return e;
+    return launch(join_kernel<COLS>, dim3(p.tiles, ceil_div(a.E, 64 * COLS)), dim3(256), 0, s, a, p);
 }
 template <int TYPE, int COLS>
 hipError_t few_t(const LookupGradArgs &a, const ZeroPart &z, hipStream_t s) {
     const int groups = (int)a.n + zero_groups(z);
-    if (groups) hipLaunchKernelGGL((few_kernel<TYPE, COLS>), dim3(groups), dim3(256), 0, s, a, z);
-    return hipGetLastError();
+    return groups ? launch(few_kernel<TYPE, COLS>, dim3(groups), dim3(256), 0, s, a, z) : hipSuccess;
 }
 // four columns a thread where rows and places allow it
 bool four_columns(const LookupGradArgs &a) {
@@ -585,12 +580,11 @@ hipError_t launch_lookup_grad(const LookupGradArgs &a, hipStream_t s) {
         p.key_out = key[at ^ 1], p.place_out = place[at ^ 1];
         p.shift = i * p.bits;
         const int hist = i ? share(1) : 0;
-        hipLaunchKernelGGL(sort_hist_kernel, dim3(tiles + hist), dim3(256), 0, s, p);
+        if (hipError_t e = launch(sort_hist_kernel, dim3(tiles + hist), dim3(256), 0, s, p); e != hipSuccess) return e;
         const int scan = i ? share(1) : std::min(1024, tiles * 4);  // first pass: the marks
-        hipLaunchKernelGGL(sort_scan_kernel, dim3((1 << p.bits) + scan), dim3(256), 0, s, p);
+        if (hipError_t e = launch(sort_scan_kernel, dim3((1 << p.bits) + scan), dim3(256), 0, s, p); e != hipSuccess) return e;
         const int scatter = share(4);
-        hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles + scatter), dim3(256), 0, s, p);
-        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        if (hipError_t e = launch(sort_scatter_kernel, dim3(tiles + scatter), dim3(256), 0, s, p); e != hipSuccess) return e;
         at ^= 1;
     }
     q.key = key[at], q.place = place[at];

@@ -194,8 +194,10 @@ BERT_API int32_t bert_amd_shard_cuts(int32_t n_seqs, const int32_t *n_tokens, in
    again for every row); nothing is written between them.  Results do not
    depend on the launch: the same inputs give the same bits.  Outputs and the
    workspace must not overlap inputs or each other unless a call says so (columns
-   of one wider matrix do not overlap).  Each returns 0, or negative without having launched anything: -1 an invalid argument, -3 a HIP
-   error (message via bert_amd_last_error). */
+   of one wider matrix do not overlap).  Each returns 0; or -1, an invalid
+   argument, without having launched anything; or -3, a HIP error of this call's
+   own, after which a part of it may have run: what it writes (an optimizer's
+   weights and moments too) is then undefined (message via bert_amd_last_error). */
 
 /* element types of the operators' tensors (ggml's numbers, as in the model files) */
 enum bert_amd_type {

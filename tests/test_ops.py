@@ -952,3 +952,53 @@ def test_linear_f32_operands_are_taken_whole(M, K, N):
     y = bertops.linear(x.cuda(), w.cuda(), b.cuda())
     terms = x.to(F64).abs() @ w.to(F64).abs().t() + b.to(F64).abs()
     close(y, x.to(F64) @ w.to(F64).t() + b.to(F64), (K + 2) * U32 * terms, "y")
+
+
+# ---- errors of the device
+
+
+def every_operator():
+    """One small call of each operator, as functions without arguments."""
+    g = gen(40)
+    x, w, table = normal(g, 20, 64).float().cuda(), normal(g, 48, 64).float().cuda(), normal(g, 30, 48).float().cuda()
+    dy = normal(g, 20, 48).float().cuda()
+    ids, many = torch.arange(20, dtype=torch.int32, device="cuda"), torch.arange(6000, dtype=torch.int32, device="cuda") % 30
+    rows = table[many.long()]
+    opt = bertops.AdamW([table.clone(), w.clone()], bits=8)
+    return [lambda: bertops.linear(x, w), lambda: bertops.linear(x[:1], w), lambda: bertops.linear(x[:, :63], w[:, :63]),
+            lambda: bertops.linear_backward(dy, x, w, z=dy, act="gelu"), lambda: bertops.linear_backward(dy[:2], x[:2], w),
+            lambda: bertops.lookup(table, ids), lambda: bertops.lookup_grad(dy, ids, 30),
+            lambda: bertops.lookup_grad(rows, many, 30), lambda: opt.step([table, w]), opt.moments]
+
+
+@gpu
+def test_a_failed_call_leaves_no_error_behind():
+    """A device that is not there: this call fails, the next ones, the library's and torch's, do not."""
+    L, x = bertlib.lib(), torch.ones(4, 8, device="cuda")
+    y = torch.empty(4, 4, device="cuda")
+    for call in every_operator():
+        rc = L.bert_amd_linear(torch.cuda.device_count() + 5, 0, 0, 4, 4, 8, x.data_ptr(), 8, x.data_ptr(), 8, None, None, 0, y.data_ptr(), 4, None, 4, None, 0, None)
+        assert rc == -3 and bertlib.last_error()
+        call()
+        (x + 1).sum().item()
+
+
+@gpu
+def test_an_error_of_an_earlier_call_is_not_the_operators():
+    """An error that another HIP call of this thread left and nobody took: the operators run and say so."""
+    with open("/proc/self/maps") as f:
+        runtimes = [ctypes.CDLL(p) for p in sorted({line.split()[-1] for line in f if "libamdhip64" in line})]
+    calls = every_operator()
+    for call in calls:
+        call()  # memory from torch's cache from here on
+    torch.cuda.synchronize()
+    assert runtimes
+    for call in calls:
+        for r in runtimes:
+            assert r.hipSetDevice(1000) != 0
+        try:
+            call()
+        finally:
+            for r in runtimes:
+                r.hipGetLastError()
+    torch.cuda.synchronize()
