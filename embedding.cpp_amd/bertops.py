@@ -198,7 +198,8 @@ class AdamW:
     that gets its updated values rounded (None: none).  seed: what 8-bit states are rounded by, with the
     step's number added.  The moments are buffers of their own, laid out once: tensor i's begin at
     where[i], a multiple of 256; load saved ones with copy_.  Tensors, copies and states stay where they
-    are: step() refuses to run once one has moved.  A step captured in a graph repeats its own number,
+    are: step() refuses to run once one has moved.  A step that fails on the device may have moved some of the
+    weights and moments: step() refuses from then on, too.  A step captured in a graph repeats its own number,
     learning rate and rounding."""
 
     _ROW = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("ms", "u8"), ("vs", "u8"), ("copy", "u8"), ("n", "i8"),
@@ -228,7 +229,7 @@ class AdamW:
         decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(self.params)
         if len(decay) != len(self.params):
             raise ValueError("weight_decay: one value, or one for each tensor")
-        self.device, self.bits, self.seed, self.t = dev, bits, int(seed), 0
+        self.device, self.bits, self.seed, self.t, self._failed = dev, bits, int(seed), 0, False
         self.lr, self.betas, self.eps = lr, betas, eps
         sizes = [t.numel() for t in self.params]
         room = [-(-n // STATE_BLOCK) * STATE_BLOCK for n in sizes]
@@ -257,6 +258,8 @@ class AdamW:
     def step(self, grads: Sequence[torch.Tensor], grad_scale: Optional[torch.Tensor] = None) -> None:
         """One step; grads: one for each tensor, all of one float type.  grad_scale: one float32 on the device
         (a clipping factor) that multiplies them."""
+        if self._failed:
+            raise RuntimeError("an earlier step failed on the device: weights and moments are undefined")
         dt, dev = grads[0].dtype, self.device
         if dt not in TYPES or len(grads) != len(self._shapes):
             raise ValueError("grads: one float tensor for each parameter")
@@ -268,10 +271,12 @@ class AdamW:
         if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.device != dev or grad_scale.numel() != 1):
             raise ValueError(f"grad_scale has to be one float32 on {dev}")
         self._rows["g"] = [g.data_ptr() for g in grads]
-        _check(bertlib.lib().bert_amd_adamw(dev.index, len(self._rows), self._rows.ctypes.data, self.bits, TYPES[dt], self._copy_type,
-                                            self.lr, self.betas[0], self.betas[1], self.eps, self.t + 1,
-                                            (self.seed + self.t + 1) & 0xFFFFFFFF,
-                                            grad_scale.data_ptr() if grad_scale is not None else None, _stream(dev)))
+        rc = bertlib.lib().bert_amd_adamw(dev.index, len(self._rows), self._rows.ctypes.data, self.bits, TYPES[dt], self._copy_type,
+                                          self.lr, self.betas[0], self.betas[1], self.eps, self.t + 1,
+                                          (self.seed + self.t + 1) & 0xFFFFFFFF,
+                                          grad_scale.data_ptr() if grad_scale is not None else None, _stream(dev))
+        self._failed = rc == -3
+        _check(rc)
         self.t += 1
 
     def moments(self):

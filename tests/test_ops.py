@@ -1002,3 +1002,30 @@ def test_an_error_of_an_earlier_call_is_not_the_operators():
             for r in runtimes:
                 r.hipGetLastError()
     torch.cuda.synchronize()
+
+
+@gpu
+def test_adamw_refuses_after_a_failed_step(monkeypatch):
+    """A step that the device failed may have moved some tensors: no second one over them.  A refused one moved none."""
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = bertops.AdamW([p])
+    opt.lr = -1.0
+    with pytest.raises(ValueError):
+        opt.step([g])
+    opt.lr = 1e-3
+    opt.step([g])
+    real = bertlib.lib()
+
+    class Failing:
+        def __getattr__(self, name):
+            return (lambda *a: -3) if name == "bert_amd_adamw" else getattr(real, name)
+
+    monkeypatch.setattr(bertlib, "lib", lambda: Failing())
+    with pytest.raises(RuntimeError):
+        opt.step([g])
+    monkeypatch.undo()
+    before = p.clone()
+    with pytest.raises(RuntimeError, match="undefined"):
+        opt.step([g])
+    torch.cuda.synchronize()
+    assert opt.t == 1 and torch.equal(p, before)
