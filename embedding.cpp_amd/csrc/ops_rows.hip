@@ -155,12 +155,13 @@ struct ZeroPart {
 };
 constexpr int ZERO_ROWS = 16;
 
+template <int ROWS>
 __device__ __forceinline__ void zero_rows(const ZeroPart &z, int first, const uint8_t *used /* of row `first` on */) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    static_assert(ZERO_ROWS <= 64, "a lane looks at one row's mark");
-    const bool mine = lane < ZERO_ROWS && first + lane < z.end;
+    static_assert(ROWS <= 64, "a lane looks at one row's mark");
+    const bool mine = lane < ROWS && first + lane < z.end;
     const uint64_t unused = __ballot(mine && !used[mine ? lane : 0]);
-    for (int v = first + wave; v < min(z.end, first + ZERO_ROWS); v += blockDim.x >> 6) {
+    for (int v = first + wave; v < min(z.end, first + ROWS); v += blockDim.x >> 6) {
         if (!(unused >> (v - first) & 1)) continue;
         float *row = z.dtable + (int64_t)v * z.ldt;
         if (z.four)
@@ -170,9 +171,9 @@ __device__ __forceinline__ void zero_rows(const ZeroPart &z, int first, const ui
     }
 }
 __device__ __forceinline__ void zero_part(const ZeroPart &z, int g, int groups) {
-    for (int64_t v = z.first + (int64_t)g * ZERO_ROWS; v < z.end; v += (int64_t)groups * ZERO_ROWS) zero_rows(z, (int)v, z.used + v);
+    for (int64_t v = z.first + (int64_t)g * ZERO_ROWS; v < z.end; v += (int64_t)groups * ZERO_ROWS) zero_rows<ZERO_ROWS>(z, (int)v, z.used + v);
 }
-inline int zero_groups(const ZeroPart &z) { return std::min(1 << 20, ceil_div(std::max(0, z.end - z.first), ZERO_ROWS)); }
+inline int zero_groups(const ZeroPart &z, int rows = ZERO_ROWS) { return std::min(1 << 20, ceil_div(std::max(0, z.end - z.first), rows)); }
 
 struct SortPass {
     const int32_t *ids;                // first pass: the caller's ids, else null
@@ -411,53 +412,61 @@ __global__ __launch_bounds__(256) void join_kernel(LookupGradArgs a, SumArgs s) 
 }
 
 // Few places (at most FEW): no sort.  A workgroup for each place looks through
-// all ids; only a token's first place goes on, its four waves each sum the
-// token's places of a quarter of the ids, in order, and the quarters are added
-// in order.  Again the other workgroups write the zeros, and find out from the
-// ids which rows are in use.  2048 x 384 f32 places of a 30522 row table: 13.9
-// us, 50 MB at 3.6 TB/s, where the sort's launches alone would take 40; looking
-// through all ids grows with their square, 4 us at 4096 and 16 at 8192.
-constexpr int FEW = 4096;
+// all ids; its waves find the token's places among an eighth of the ids each,
+// sum those in order, and the eighths are added in order.  A token's r-th place
+// takes the columns' slices r, r + its places, ..: a rare token's first place
+// does it all, a frequent one's sums are spread over as many workgroups as there
+// are slices, so that none walks along a wide row place by place.  Again the other
+// workgroups write the zeros, and find out from the ids which rows are in use.
+// f32 of a 30522 row table, us, here and sorted: 2048 x 384 places of tokens as
+// text has them 15.4 and 48, all of one token 33 and 38; 4096 x 384 25 and 49, of
+// one token 61 and 40; 4096 x 1023 (a column a lane) 60 and 59, of one token 93
+// and 52.  The looking grows with the places' square.  Half as many waves are 2 to
+// 5 us faster on rare tokens and twice as slow on frequent ones; the first place
+// alone at work took 307 us for 4096 x 768 of one token and 2302 for 4096 x 1023.
+constexpr int FEW = 4096, FEW_WAVES = 8, FEW_ZEROS = 4 * FEW_WAVES;
 
 template <int TYPE, int COLS>
-__global__ __launch_bounds__(256) void few_kernel(LookupGradArgs a, ZeroPart z) {
+__global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(LookupGradArgs a, ZeroPart z) {
     typedef typename Elem<TYPE>::T T;
-    const int n = (int)a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if ((int)blockIdx.x >= n) {
-        __shared__ uint8_t used[256];
-        static_assert(ZERO_ROWS <= 256, "one thread clears one row's mark");
-        for (int64_t b = blockIdx.x - n; b * ZERO_ROWS < a.V; b += gridDim.x - n) {
-            const int first = (int)b * ZERO_ROWS;
+    const int n = (int)a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = blockIdx.x;
+    if (at >= n) {
+        __shared__ uint8_t used[FEW_ZEROS];
+        static_assert(FEW_ZEROS <= 64 * FEW_WAVES, "one thread clears one row's mark");
+        for (int64_t b = at - n; b * FEW_ZEROS < a.V; b += gridDim.x - n) {
+            const int first = (int)b * FEW_ZEROS;
             __syncthreads();
-            used[threadIdx.x] = 0;
+            if (threadIdx.x < FEW_ZEROS) used[threadIdx.x] = 0;
             __syncthreads();
-            for (int i = threadIdx.x; i < n; i += 256) {
+            for (int i = threadIdx.x; i < n; i += 64 * FEW_WAVES) {
                 const int id = a.ids[i];
-                if (id >= first && id < first + ZERO_ROWS && id != a.pad_id) used[id - first] = 1;
+                if (id >= first && id < first + FEW_ZEROS && id != a.pad_id) used[id - first] = 1;
             }
             __syncthreads();
-            zero_rows(z, first, used);
+            zero_rows<FEW_ZEROS>(z, first, used);
         }
         return;
     }
-    const int k = sort_key(a.ids[blockIdx.x], a.V, a.pad_id);
+    const int k = sort_key(a.ids[at], a.V, a.pad_id);
     if (k == a.V) return;
-    __shared__ uint16_t list[4][FEW / 4];
-    __shared__ int before[4];
-    __shared__ float sums[3][64][COLS + 1];
-    const int quarter = ceil_div(n, 256) * 64, from = wave * quarter;
+    __shared__ uint16_t list[FEW_WAVES][FEW / FEW_WAVES];
+    __shared__ int counts[FEW_WAVES], before[FEW_WAVES];
+    __shared__ float sums[FEW_WAVES - 1][64][COLS + 1];
+    const int share = ceil_div(n, 64 * FEW_WAVES) * 64, from = wave * share;
     int count = 0, earlier = 0;
-    for (int i = from; i < min(n, from + quarter); i += 64) {
+    for (int i = from; i < min(n, from + share); i += 64) {
         const bool same = i + lane < n && a.ids[i + lane] == k;
         const uint64_t mask = __ballot(same);
         if (same) list[wave][count + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(i + lane);
-        if (mask && i + __ffsll((unsigned long long)mask) - 1 < (int)blockIdx.x) earlier = 1;
+        earlier += __popcll(__ballot(same && i + lane < at));
         count += __popcll(mask);
     }
-    before[wave] = earlier;
+    counts[wave] = count, before[wave] = earlier;
     __syncthreads();
-    if (before[0] | before[1] | before[2] | before[3]) return;
-    for (int e0 = 0; e0 < a.E; e0 += 64 * COLS) {
+    int rank = 0, places = 0;  // of this place among its token's
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; w++) rank += before[w], places += counts[w];
+    for (int e0 = rank * 64 * COLS; e0 < a.E; e0 += places * 64 * COLS) {
         const int e = e0 + lane * COLS;
         float sum[COLS] = {};
         if (e < a.E)
@@ -477,7 +486,7 @@ __global__ __launch_bounds__(256) void few_kernel(LookupGradArgs a, ZeroPart z) 
         __syncthreads();
         if (!wave && e < a.E) {
 #pragma unroll
-            for (int w = 0; w < 3; w++)
+            for (int w = 0; w < FEW_WAVES - 1; w++)
 #pragma unroll
                 for (int c = 0; c < COLS; c++) sum[c] += sums[w][lane][c];
             store_row<COLS>(a, k, e, sum);
@@ -517,8 +526,8 @@ hipError_t sum_t(const LookupGradArgs &a, const SumArgs &p, hipStream_t s) {
 }
 template <int TYPE, int COLS>
 hipError_t few_t(const LookupGradArgs &a, const ZeroPart &z, hipStream_t s) {
-    const int groups = (int)a.n + zero_groups(z);
-    return groups ? launch(few_kernel<TYPE, COLS>, dim3(groups), dim3(256), 0, s, a, z) : hipSuccess;
+    const int groups = (int)a.n + zero_groups(z, FEW_ZEROS);
+    return groups ? launch(few_kernel<TYPE, COLS>, dim3(groups), dim3(64 * FEW_WAVES), 0, s, a, z) : hipSuccess;
 }
 // four columns a thread where rows and places allow it
 bool four_columns(const LookupGradArgs &a) {

@@ -1029,3 +1029,42 @@ def test_adamw_refuses_after_a_failed_step(monkeypatch):
         opt.step([g])
     torch.cuda.synchronize()
     assert opt.t == 1 and torch.equal(p, before)
+
+
+# ---- frequent tokens among few places
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 2, 63, 513, 2000, 4096])
+@pytest.mark.parametrize("E", [1, 65, 129, 260, 1023, 2052])
+def test_lookup_grad_frequent_tokens(n, E, dtype):
+    """Tokens with fewer and with more places than a row has slices of columns, up to every place the same one."""
+    g = gen(50)
+    dout = normal(g, n, E).to(DTYPES[dtype])
+    D = dout.cuda()
+    for V, ids in ((3, torch.zeros(n)), (70, torch.full((n,), 69)), (40, torch.rand(n, generator=g) ** 6 * 40), (9, torch.where(torch.arange(n) % 3 == 0, -1, 4))):
+        ids = ids.to(torch.int32)
+        out = torch.full((V, E), float("nan"), device="cuda")
+        got = bertops.lookup_grad(D, ids.cuda(), V, scale=0.5, out=out)
+        check_grad(got, dout, ids, V, 0.5, -1)
+        assert torch.equal(got, bertops.lookup_grad(D, ids.cuda(), V, scale=0.5))
+        base = normal(g, V, E).float()
+        check_grad(bertops.lookup_grad(D, ids.cuda(), V, out=base.cuda(), accumulate=True), dout, ids, V, 1.0, -1, base)
+
+
+@gpu
+def test_lookup_grad_of_one_token_is_spread():
+    """All places one token: with 4096 of them, which are not sorted, not ten times as long as with one more, which are."""
+    def time_of(n, E=1023):
+        dout, ids, out = torch.ones(n, E, device="cuda"), torch.full((n,), 7, dtype=torch.int32, device="cuda"), torch.empty(100, E, device="cuda")
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        for k in range(12):
+            if k == 2:
+                start.record()
+            bertops.lookup_grad(dout, ids, 100, out=out)
+        end.record()
+        end.synchronize()
+        return start.elapsed_time(end)
+
+    assert time_of(4096) < 10 * time_of(4097)
