@@ -746,16 +746,21 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const float *part, int
     out[n] = v;
 }
 
-// How dz_kernel goes over its matrix.  Up to 1024 rows: 8 columns wide, all
-// rows, and the sums are the bias's gradient at once (256 x 384 in f32: 32
-// columns wide it took 8.8 us on 12 CUs).  More: 8 or, past 128 columns, 256
-// columns wide, about 2048 workgroups (16384 x 4096 in bf16: 403 MB in 75 us).
+// How dz_kernel goes over its matrix.  Up to 1024 rows and 2^21 elements: 8
+// columns wide, all rows, and the sums are the bias's gradient at once.  Else 8 or,
+// past 128 columns, 256 columns wide, whole pieces of rows, about 2048 workgroups
+// (16384 x 4096 in bf16: 403 MB in 75 us), and the sums take a launch more.  The
+// bias's gradient alone, us, 8 and 256 columns wide: bf16 256 x 384 4.0 and 11.3,
+// 1024 x 1024 6.2 and 10.6, 512 x 4096 13.3 and 10.8, 1024 x 4096 23 and 11; f32
+// 3.8 and 13.9, 8.0 and 13.1, 14.1 and 13.2, 24 and 15.  With dx 512 x 4096 comes
+// out even (bf16 29.7 and 30.9), 1000 x 2500 takes 52 and 37: past that many
+// elements the few bytes of a row cost whole cache lines of several L2s.
 struct DzPlan {
     bool narrow;
     int64_t rows;
 };
 DzPlan dz_plan(int64_t M, int64_t N) {
-    if (M <= 1024) return {true, std::max<int64_t>(M, 1)};
+    if (M <= 1024 && M * N <= 1 << 21) return {true, std::max<int64_t>(M, 1)};
     const bool narrow = N <= 128;
     const int64_t across = ceil_div<int64_t>(N, narrow ? 8 : 256);
     int64_t rows = narrow ? 256 : 64;

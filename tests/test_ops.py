@@ -1068,3 +1068,43 @@ def test_lookup_grad_of_one_token_is_spread():
         return start.elapsed_time(end)
 
     assert time_of(4096) < 10 * time_of(4097)
+
+
+# ---- the two ways over a layer's dz
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N", [(1024, 2048), (1024, 2049), (1023, 2056), (517, 4104), (64, 33000), (16, 131080), (9, 240001)])
+def test_backward_dz_forms(M, N, dtype):
+    """Up to 1024 rows, with as many and with more columns than the narrow form takes."""
+    dt, K = DTYPES[dtype], 8
+    x, w, dy, _ = make_layer(M, K, N, dt, seed=60)
+    z = normal(gen(61), M, N).to(dt)
+    dx, dw, db = bertops.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z=z.cuda(), act="relu")  # its dz needs no rounding
+    dz = torch.where(z > 0, dy, torch.zeros_like(dy)).to(F64)
+    for got, a, b, n, what in ((dx, dz, w, N, "dx"), (dw, dz.t(), x, M, "dw")):
+        far = (n + 1) * U32 * (a.abs() @ b.to(F64).abs())
+        want = a @ b.to(F64)
+        close(got, want, far + u(dt) * (want.abs() + far) + tiny(dt), what)
+    close(db, dz.sum(0), (M + 1) * U32 * dz.abs().sum(0), "db")
+    (alone,) = (t for t in bertops.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z=z.cuda(), act="relu", need=(False, False, True)) if t is not None)
+    assert torch.equal(alone, db)
+
+
+@gpu
+def test_backward_of_wide_layers_takes_whole_lines():
+    """A wide layer's bias gradient over 1000 rows takes no more than twice the time of 1040."""
+    def time_of(M, N=65536):
+        x, w, dy = (torch.ones(*s, device="cuda").bfloat16() for s in ((M, 8), (N, 8), (M, N)))
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        for k in range(12):
+            if k == 2:
+                start.record()
+            bertops.linear_backward(dy, x, w, z=dy, act="gelu", need=(False, False, True))
+        end.record()
+        end.synchronize()
+        return start.elapsed_time(end)
+
+    time_of(1040)
+    assert time_of(1000) < 2 * time_of(1040)
