@@ -290,10 +290,34 @@ class AdamW:
         return m, v
 
 
+class _Kept:
+    """What a training forward keeps for its backward: one forward at a time, until the weights move."""
+
+    def __init__(self):
+        self._what, self._open = None, 0  # the newest forward's; forwards since the last backward
+
+    def put(self, *what) -> None:
+        self._what, self._open = what, self._open + 1
+
+    def get(self):
+        if self._what is None:
+            raise ValueError("backward() follows forward(), before step()")
+        if self._open > 1:
+            self.drop()
+            raise ValueError("two forwards before a backward, whose gradient is meant? Take both batches in one forward, "
+                             "and forwards without a backward with train=False")
+        self._open = 0
+        return self._what
+
+    def drop(self) -> None:
+        self._what, self._open = None, 0
+
+
 class Adapter:
     """A trained layer on embeddings: y = act(W e + b) + e, W and b starting at zero.
 
-    Trained by the caller's loss: y = forward(e), backward(dy), step()."""
+    Trained by the caller's loss: y = forward(e), backward(dy), step().  A backward is its newest forward's;
+    pairs and triplets of a loss go through one forward, side by side in a batch."""
 
     def __init__(self, n_embd: int, act: str = "tanh", device="cuda:0", **optimizer):
         _act(act)
@@ -301,20 +325,18 @@ class Adapter:
         self.act = act
         self.w, self.b = torch.zeros(n_embd, n_embd, device=device), torch.zeros(n_embd, device=device)
         self.opt = AdamW([self.w, self.b], **{"weight_decay": [0.01, 0.0], **optimizer})
-        self._kept = self._grads = None
+        self._kept, self._grads = _Kept(), None
 
     def forward(self, e: torch.Tensor, train: bool = True) -> torch.Tensor:
         if not train:
             return linear(e, self.w, self.b, residual=e, act=self.act)
         y, z = linear(e, self.w, self.b, residual=e, act=self.act, save_z=True)
-        self._kept = (e, z)
+        self._kept.put(e, z)
         return y
 
     def backward(self, dy: torch.Tensor, need_input: bool = False) -> Optional[torch.Tensor]:
         """Keeps the weights' gradients for step(); the embeddings' own where asked for."""
-        if self._kept is None:
-            raise ValueError("backward() follows forward()")
-        e, z = self._kept
+        e, z = self._kept.get()
         de, dw, db = linear_backward(dy, e, self.w, z=z, act=self.act, need=(need_input, True, True))
         self._grads = [dw, db]
         return de + dy if need_input else None
@@ -324,6 +346,7 @@ class Adapter:
             raise ValueError("step() follows backward()")
         self.opt.step(self._grads)
         self._grads = None
+        self._kept.drop()  # z is of the weights as they were
 
     def encode(self, model: "bertlib.BertModel", sentences, batch_size: int = 16) -> np.ndarray:
         """The model's embeddings of `sentences` through the adapter, L2-normalised again."""
@@ -335,31 +358,34 @@ class Adapter:
 
 
 class TokenTable:
-    """A trainable float32 copy of a model's word rows: static embeddings of tokens."""
+    """A trainable float32 copy of a model's word rows: static embeddings of tokens.
+
+    forward(ids), backward(dout), step(), as Adapter; backward() adds up until step()."""
 
     def __init__(self, model: "bertlib.BertModel", slot: int = 0, pad_id: int = 0, **optimizer):
         self.rows = word_rows(model, slot=slot)
         self.pad_id = pad_id
         self.opt = AdamW([self.rows], **optimizer)
-        self._ids = self._grad = None
+        self._kept, self._grad = _Kept(), None
 
-    def forward(self, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-        self._ids, self._scale = ids, scale
-        return lookup(self.rows, ids, scale=scale)
+    def forward(self, ids: torch.Tensor, scale: float = 1.0, train: bool = True) -> torch.Tensor:
+        out = lookup(self.rows, ids, scale=scale)
+        if train:
+            self._kept.put(ids, scale)
+        return out
 
     def backward(self, dout: torch.Tensor) -> None:
         """Adds to the table's gradient until step()."""
-        if self._ids is None:
-            raise ValueError("backward() follows forward()")
+        ids, scale = self._kept.get()
         first = self._grad is None
-        self._grad = lookup_grad(dout, self._ids, self.rows.shape[0], scale=self._scale, pad_id=self.pad_id, out=self._grad,
-                                 accumulate=not first)
+        self._grad = lookup_grad(dout, ids, self.rows.shape[0], scale=scale, pad_id=self.pad_id, out=self._grad, accumulate=not first)
 
     def step(self) -> None:
         if self._grad is None:
             raise ValueError("step() follows backward()")
         self.opt.step([self._grad])
         self._grad = None
+        self._kept.drop()
 
 
 def word_rows(model: "bertlib.BertModel", ids: Optional[torch.Tensor] = None, *, slot: int = 0, scale: float = 1.0,

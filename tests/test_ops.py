@@ -1108,3 +1108,69 @@ def test_backward_of_wide_layers_takes_whole_lines():
 
     time_of(1040)
     assert time_of(1000) < 2 * time_of(1040)
+
+
+# ---- what Adapter and TokenTable keep between their calls
+
+
+class FewRows:
+    """A model's word rows as bert_amd_word_table gives them, without a model."""
+
+    def __init__(self, rows):
+        self.rows = rows
+
+    def word_table(self, slot=0):
+        return self.rows.data_ptr(), 0, *self.rows.shape, self.rows.device.index
+
+
+def token_table(V=20, E=32, **kw):
+    return bertops.TokenTable(FewRows(normal(gen(70), V, E).float().cuda()), pad_id=-1, **kw)
+
+
+@gpu
+def test_trained_layers_refuse_mixed_and_stale_backwards():
+    """Two forwards before a backward, and a backward of weights that have moved since."""
+    a, t = bertops.Adapter(32, lr=1e-2), token_table()
+    e, f = (normal(gen(s), 6, 32).float().cuda() for s in (71, 72))
+    i, j = torch.arange(6, dtype=torch.int32, device="cuda"), torch.arange(6, 12, dtype=torch.int32, device="cuda")
+    for o, one, two, dy in ((a, e, f, e), (t, i, j, f)):
+        with pytest.raises(ValueError, match="follows"):
+            o.backward(dy)
+        o.forward(one)
+        o.forward(two)
+        with pytest.raises(ValueError, match="two forwards"):
+            o.backward(dy)
+        with pytest.raises(ValueError, match="follows"):  # neither is meant from here on
+            o.backward(dy)
+        with pytest.raises(ValueError):
+            o.step()
+        o.forward(one)
+        o.forward(two, train=False)
+        o.backward(dy)
+        o.step()
+        with pytest.raises(ValueError, match="follows"):
+            o.backward(dy)
+        o.forward(two)
+        o.backward(dy)
+        o.forward(one)
+        o.step()
+        with pytest.raises(ValueError, match="follows"):  # the weights that forward used are gone
+            o.backward(dy)
+        o.forward(one)
+        o.backward(dy)
+        o.step()
+    assert a.opt.t == 3 and t.opt.t == 3
+
+
+@gpu
+def test_pairs_through_one_forward():
+    """The two sides of a pair in one batch: the gradients of both against 64 bits."""
+    a = bertops.Adapter(16, act="gelu_erf", lr=1e-2)
+    a.w.copy_(normal(gen(73), 16, 16, std=0.2))
+    e, dy = (normal(gen(s), 10, 16).float() for s in (74, 75))
+    a.forward(e.cuda())
+    de = a.backward(dy.cuda(), need_input=True)
+    E, W, B = e.to(F64).requires_grad_(True), a.w.cpu().to(F64).requires_grad_(True), torch.zeros(16, dtype=F64, requires_grad=True)
+    (act64(E @ W.t() + B, "gelu_erf") + E).backward(dy.to(F64))
+    for got, want in ((a._grads[0], W.grad), (a._grads[1], B.grad), (de, E.grad)):
+        close(got, want, 200 * U32 * want.abs().max() * torch.ones_like(want), "pair")  # f32 sums of at most 16 terms, each within some 2^-24
