@@ -317,7 +317,7 @@ class Adapter:
     """A trained layer on embeddings: y = act(W e + b) + e, W and b starting at zero.
 
     Trained by the caller's loss: y = forward(e), backward(dy), step().  A backward is its newest forward's;
-    pairs and triplets of a loss go through one forward, side by side in a batch."""
+    pairs and triplets of a loss go through one forward, side by side in a batch.  Gradients add up over backwards until step()."""
 
     def __init__(self, n_embd: int, act: str = "tanh", device="cuda:0", **optimizer):
         _act(act)
@@ -335,10 +335,10 @@ class Adapter:
         return y
 
     def backward(self, dy: torch.Tensor, need_input: bool = False) -> Optional[torch.Tensor]:
-        """Keeps the weights' gradients for step(); the embeddings' own where asked for."""
+        """Adds to the weights' gradients until step(); gives the embeddings' own where asked for."""
         e, z = self._kept.get()
         de, dw, db = linear_backward(dy, e, self.w, z=z, act=self.act, need=(need_input, True, True))
-        self._grads = [dw, db]
+        self._grads = [dw, db] if self._grads is None else [kept.add_(new) for kept, new in zip(self._grads, (dw, db))]
         return de + dy if need_input else None
 
     def step(self) -> None:
@@ -360,7 +360,7 @@ class Adapter:
 class TokenTable:
     """A trainable float32 copy of a model's word rows: static embeddings of tokens.
 
-    forward(ids), backward(dout), step(), as Adapter; backward() adds up until step()."""
+    forward(ids), backward(dout), step(), as Adapter."""
 
     def __init__(self, model: "bertlib.BertModel", slot: int = 0, pad_id: int = 0, **optimizer):
         self.rows = word_rows(model, slot=slot)

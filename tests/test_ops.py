@@ -1174,3 +1174,30 @@ def test_pairs_through_one_forward():
     (act64(E @ W.t() + B, "gelu_erf") + E).backward(dy.to(F64))
     for got, want in ((a._grads[0], W.grad), (a._grads[1], B.grad), (de, E.grad)):
         close(got, want, 200 * U32 * want.abs().max() * torch.ones_like(want), "pair")  # f32 sums of at most 16 terms, each within some 2^-24
+
+
+@gpu
+def test_gradients_add_up_until_the_step():
+    """Two forwards and backwards before one step: the sum of both gradients moves the weights, as TokenTable's does."""
+    e, f = (normal(gen(s), 12, 24).float().cuda() for s in (76, 77))
+    both, lone = bertops.Adapter(24, lr=1e-2), [bertops.Adapter(24, lr=1e-2) for _ in range(2)]
+    for x, o in zip((e, f), lone):
+        both.backward(both.forward(x) - 1.0)
+        o.backward(o.forward(x) - 1.0)
+    assert all(torch.equal(s, p + q) for s, p, q in zip(both._grads, lone[0]._grads, lone[1]._grads))
+    both.step()
+    both.backward(both.forward(e) - 1.0)
+    assert not torch.equal(both._grads[0], lone[0]._grads[0])  # a new sum of the moved weights
+    table = token_table()
+    rows = table.rows.clone()
+    ids = [torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([3, 4, 3], [4, 4, 9])]
+    dout = normal(gen(78), 3, 32).float().cuda()
+    for i in ids:
+        table.forward(i)
+        table.backward(dout)
+    want = sum(bertops.lookup_grad(dout, i, 20) for i in ids)
+    assert torch.equal(table._grad, want)
+    table.step()
+    opt = bertops.AdamW([rows])
+    opt.step([want])
+    assert torch.equal(table.rows, rows)
