@@ -290,14 +290,29 @@ class AdamW:
         return m, v
 
 
+class _Own:
+    """Tensors made on one stream that calls on others may use and drop: their memory is not given out again
+    before those are done with it."""
+
+    def __init__(self, *tensors: torch.Tensor):
+        self._tensors, self._stream = tensors, _stream(tensors[0].device)
+
+    def use(self):
+        dev = self._tensors[0].device
+        if _stream(dev) != self._stream:
+            for t in self._tensors:
+                t.record_stream(torch.cuda.current_stream(dev))
+        return self._tensors
+
+
 class _Kept:
     """What a training forward keeps for its backward: one forward at a time, until the weights move."""
 
     def __init__(self):
         self._what, self._open = None, 0  # the newest forward's; forwards since the last backward
 
-    def put(self, *what) -> None:
-        self._what, self._open = what, self._open + 1
+    def put(self, *tensors: torch.Tensor) -> None:
+        self._what, self._open = _Own(*tensors), self._open + 1
 
     def get(self):
         if self._what is None:
@@ -307,7 +322,7 @@ class _Kept:
             raise ValueError("two forwards before a backward, whose gradient is meant? Take both batches in one forward, "
                              "and forwards without a backward with train=False")
         self._open = 0
-        return self._what
+        return self._what.use()
 
     def drop(self) -> None:
         self._what, self._open = None, 0
@@ -338,13 +353,17 @@ class Adapter:
         """Adds to the weights' gradients until step(); gives the embeddings' own where asked for."""
         e, z = self._kept.get()
         de, dw, db = linear_backward(dy, e, self.w, z=z, act=self.act, need=(need_input, True, True))
-        self._grads = [dw, db] if self._grads is None else [kept.add_(new) for kept, new in zip(self._grads, (dw, db))]
+        if self._grads is None:
+            self._grads = _Own(dw, db)
+        else:
+            for kept, new in zip(self._grads.use(), (dw, db)):
+                kept.add_(new)
         return de + dy if need_input else None
 
     def step(self) -> None:
         if self._grads is None:
             raise ValueError("step() follows backward()")
-        self.opt.step(self._grads)
+        self.opt.step(self._grads.use())
         self._grads = None
         self._kept.drop()  # z is of the weights as they were
 
@@ -366,24 +385,27 @@ class TokenTable:
         self.rows = word_rows(model, slot=slot)
         self.pad_id = pad_id
         self.opt = AdamW([self.rows], **optimizer)
-        self._kept, self._grad = _Kept(), None
+        self._kept, self._scale, self._grad = _Kept(), 1.0, None
 
     def forward(self, ids: torch.Tensor, scale: float = 1.0, train: bool = True) -> torch.Tensor:
         out = lookup(self.rows, ids, scale=scale)
         if train:
-            self._kept.put(ids, scale)
+            self._kept.put(ids)
+            self._scale = scale
         return out
 
     def backward(self, dout: torch.Tensor) -> None:
         """Adds to the table's gradient until step()."""
-        ids, scale = self._kept.get()
-        first = self._grad is None
-        self._grad = lookup_grad(dout, ids, self.rows.shape[0], scale=scale, pad_id=self.pad_id, out=self._grad, accumulate=not first)
+        (ids,) = self._kept.get()
+        (out,) = (None,) if self._grad is None else self._grad.use()
+        grad = lookup_grad(dout, ids, self.rows.shape[0], scale=self._scale, pad_id=self.pad_id, out=out, accumulate=out is not None)
+        if out is None:
+            self._grad = _Own(grad)
 
     def step(self) -> None:
         if self._grad is None:
             raise ValueError("step() follows backward()")
-        self.opt.step([self._grad])
+        self.opt.step(self._grad.use())
         self._grad = None
         self._kept.drop()
 

@@ -1172,7 +1172,7 @@ def test_pairs_through_one_forward():
     de = a.backward(dy.cuda(), need_input=True)
     E, W, B = e.to(F64).requires_grad_(True), a.w.cpu().to(F64).requires_grad_(True), torch.zeros(16, dtype=F64, requires_grad=True)
     (act64(E @ W.t() + B, "gelu_erf") + E).backward(dy.to(F64))
-    for got, want in ((a._grads[0], W.grad), (a._grads[1], B.grad), (de, E.grad)):
+    for got, want in (*zip(a._grads.use(), (W.grad, B.grad)), (de, E.grad)):
         close(got, want, 200 * U32 * want.abs().max() * torch.ones_like(want), "pair")  # f32 sums of at most 16 terms, each within some 2^-24
 
 
@@ -1184,10 +1184,10 @@ def test_gradients_add_up_until_the_step():
     for x, o in zip((e, f), lone):
         both.backward(both.forward(x) - 1.0)
         o.backward(o.forward(x) - 1.0)
-    assert all(torch.equal(s, p + q) for s, p, q in zip(both._grads, lone[0]._grads, lone[1]._grads))
+    assert all(torch.equal(s, p + q) for s, p, q in zip(*(o._grads.use() for o in (both, *lone))))
     both.step()
     both.backward(both.forward(e) - 1.0)
-    assert not torch.equal(both._grads[0], lone[0]._grads[0])  # a new sum of the moved weights
+    assert not torch.equal(both._grads.use()[0], lone[0]._grads.use()[0])  # a new sum of the moved weights
     table = token_table()
     rows = table.rows.clone()
     ids = [torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([3, 4, 3], [4, 4, 9])]
@@ -1196,8 +1196,54 @@ def test_gradients_add_up_until_the_step():
         table.forward(i)
         table.backward(dout)
     want = sum(bertops.lookup_grad(dout, i, 20) for i in ids)
-    assert torch.equal(table._grad, want)
+    assert torch.equal(table._grad.use()[0], want)
     table.step()
     opt = bertops.AdamW([rows])
     opt.step([want])
     assert torch.equal(table.rows, rows)
+
+
+@gpu
+def test_steps_on_another_stream():
+    """Forward, backward and step on a stream each: what a call drops is not given out while another stream reads it."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+    x = normal(gen(79), 64, 384).float().cuda()
+    ids = torch.arange(64, dtype=torch.int32, device="cuda") % 20
+    for made, inputs in ((lambda: bertops.Adapter(384, lr=1e-2), x), (lambda: token_table(E=384, lr=1e-2), ids)):
+        here, there = made(), made()
+        weights = lambda o: o.opt.params  # noqa: E731
+        here.forward(inputs)
+        here.backward(x)
+        here.backward(x)
+        here.step()
+        s0, s1, s2 = (torch.cuda.Stream() for _ in range(3))
+
+        def given_out(stream, like, taken):
+            with torch.cuda.stream(stream):
+                new = [span(torch.empty_like(t)) for t in like]
+            return any(a < d and c < b for a, b in new for c, d in taken)
+
+        s0.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s0):
+            there.forward(inputs.clone())
+        s1.wait_stream(s0)
+        with torch.cuda.stream(s1):
+            torch.cuda._sleep(50_000_000)  # the backward is not done when what it reads is dropped
+            there.backward(x)
+            there.backward(x)
+        kept = [span(t) for t in there._kept._what._tensors]
+        there._kept.drop()
+        assert not given_out(s0, [inputs, x], kept)
+        grads = there._grads if hasattr(there, "_grads") else there._grad
+        sums = [span(t) for t in grads._tensors]
+        del grads
+        s2.wait_stream(s1)
+        with torch.cuda.stream(s2):
+            torch.cuda._sleep(50_000_000)
+            there.step()
+        s1.synchronize()
+        assert not given_out(s1, weights(there), sums)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(weights(here), weights(there)))
