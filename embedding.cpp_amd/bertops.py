@@ -30,6 +30,9 @@ def _check(rc: int) -> None:
         raise (RuntimeError if rc == -3 else ValueError)(bertlib.last_error())
 
 
+# a tensor that the library has written: what autograd saved of it is not its value any more
+_written = torch.autograd.graph.increment_version
+
 # the current stream's handle without the Stream object around it (2 us of a 10 us call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -109,6 +112,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     keep, ws, nws = _room(L.bert_amd_linear_workspace(typ, M, N, K, _aligned(x.element_size(), (px, ldx), (pw, ldw))), dev)
     _check(L.bert_amd_linear(dev.index, typ, a, M, N, K, px, ldx, pw, ldw, b, r, ldr, y.data_ptr(), ldy,
                              z.data_ptr() if save_z else None, N, ws, nws, _stream(dev)))
+    if out is not None:
+        _written(out)
     return (y, z) if save_z else y
 
 
@@ -188,6 +193,7 @@ def lookup_grad(dout: torch.Tensor, ids: torch.Tensor, n_rows: int, *, scale: fl
     keep, ws, nws = _room(L.bert_amd_lookup_grad_workspace(ids.numel(), n_rows, width), dev)
     _check(L.bert_amd_lookup_grad(dev.index, TYPES[dout.dtype], ids.numel(), n_rows, width, dout.data_ptr(), ldd, _ids(ids, dev),
                                   scale, pad_id, int(accumulate), out.data_ptr(), ldt, ws, nws, _stream(dev)))
+    _written(out)
     return out
 
 
@@ -276,6 +282,8 @@ class AdamW:
                                           (self.seed + self.t + 1) & 0xFFFFFFFF,
                                           grad_scale.data_ptr() if grad_scale is not None else None, _stream(dev))
         self._failed = rc == -3
+        if rc != -1:
+            _written([*self.params, *(self.copies or ())])
         _check(rc)
         self.t += 1
 

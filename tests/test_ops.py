@@ -1247,3 +1247,35 @@ def test_steps_on_another_stream():
         assert not given_out(s1, weights(there), sums)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(weights(here), weights(there)))
+
+
+# ---- beside torch's autograd
+
+
+@gpu
+def test_written_tensors_count_as_changed():
+    """A graph that saved a weight, a copy or an output notices that an operator has written it since."""
+    def stale(t, change):
+        w = torch.ones_like(t, requires_grad=True)
+        y = (w * t).sum()  # saves t
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+    p = torch.nn.Parameter(torch.ones(8, 8, device="cuda"))
+    copy = p.detach().bfloat16()
+    opt = bertops.AdamW([p], copies=[copy])
+    for t in (p, copy):
+        stale(t, lambda: opt.step([torch.ones(8, 8, device="cuda")]))
+    x, out = torch.ones(8, 8, device="cuda"), torch.ones(8, 8, device="cuda")
+    stale(out, lambda: bertops.linear(x, x, out=out))
+    ids = torch.zeros(8, dtype=torch.int32, device="cuda")
+    stale(out, lambda: bertops.lookup_grad(x, ids, 8, out=out))
+    opt.lr = -1.0
+    w = torch.ones(8, 8, device="cuda", requires_grad=True)
+    y = (w * p).sum()
+    with pytest.raises(ValueError):
+        opt.step([x])
+    y.backward()  # a refused step has written nothing
+    with torch.inference_mode():
+        bertops.linear(x, x, out=torch.ones(8, 8, device="cuda"))
