@@ -3,7 +3,8 @@
 `linear` / `linear_backward` are a dense layer with its epilogue, `lookup` / `lookup_grad` the rows of a
 token table, `AdamW` the step that trains both.  Tensors stay on their device; every call is enqueued on
 torch's current stream of that device and returns at once.  Arguments are checked here and in the
-library: a bad one raises before anything is launched.
+library: a bad one raises before anything is launched.  Results have no autograd nodes: `linear` and
+`lookup` warn where torch would have made one, outside of torch.no_grad() and of an autograd.Function.
 
 `Adapter` is a trained layer on a BertModel's embeddings and `TokenTable` a trainable copy of its word
 rows; both are what a user builds from the operators.
@@ -11,6 +12,7 @@ rows; both are what a user builds from the operators.
 from __future__ import annotations
 
 import ctypes
+import warnings
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -72,6 +74,16 @@ def _first(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: two dimensions are needed")
 
 
+def _no_node(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Says so where the results would need a gradient that they do not get."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                warnings.warn(f"{name}() of a tensor that requires a gradient: its results have none.  Call it under torch.no_grad(), "
+                              "or in a torch.autograd.Function", stacklevel=3)
+                return
+
+
 def _act(act: str) -> int:
     if act not in ACTS:
         raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTS)}")
@@ -101,6 +113,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     save_z: also returns the pre-activation, (y, z), which linear_backward takes.  out: where y goes (may
     be `residual`)."""
     _first("x", x)
+    _no_node("linear", x, w, bias, residual)
     (M, K), N, dt, dev, a = x.shape, w.shape[0], x.dtype, x.device, _act(act)
     ldx, ldw = _matrix("x", x, dt, dev, M, K), _matrix("w", w, dt, dev, N, K)
     b = None if bias is None else _vector("bias", bias, dev, N)
@@ -153,6 +166,7 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, table_
     a model file.  out_dtype: float32 for those, the table's own type otherwise, unless given."""
     if not table.is_cuda or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError("the table has to be a GPU tensor [rows, width]")
+    _no_node("lookup", table)
     blocks = table_type in BLOCK_BYTES
     if blocks:
         if table.dtype != torch.uint8 or table.shape[1] % BLOCK_BYTES[table_type]:

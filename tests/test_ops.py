@@ -1279,3 +1279,46 @@ def test_written_tensors_count_as_changed():
     y.backward()  # a refused step has written nothing
     with torch.inference_mode():
         bertops.linear(x, x, out=torch.ones(8, 8, device="cuda"))
+
+
+@gpu
+def test_lost_gradients_are_said():
+    """linear and lookup of tensors that require a gradient warn, but not where a wrapper takes care of it."""
+    import warnings
+
+    x, w, b = (torch.ones(*s, device="cuda") for s in ((4, 8), (6, 8), (6,)))
+    r, ids = torch.ones(4, 6, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+
+    class Layer(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w, b):
+            y, z = bertops.linear(x, w, b, act="tanh", save_z=True)
+            ctx.save_for_backward(x, w, z)
+            return y
+
+        @staticmethod
+        def backward(ctx, dy):
+            x, w, z = ctx.saved_tensors
+            return bertops.linear_backward(dy.contiguous(), x, w, z=z, act="tanh")  # a sum hands a broadcast one back
+
+    for t in (x, w, b, r):
+        t.requires_grad_(True)
+        with pytest.warns(UserWarning, match="requires a gradient"):
+            y = bertops.linear(x, w, b, residual=r)
+        assert not y.requires_grad
+        t.requires_grad_(False)
+    w.requires_grad_(True)
+    with pytest.warns(UserWarning, match="requires a gradient"):
+        bertops.lookup(w, ids)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with torch.no_grad():
+            bertops.linear(x, w, b)
+            bertops.lookup(w, ids)
+        bertops.linear(x, w.detach(), b)
+        y = Layer.apply(x, w, b)
+        y.sum().backward()
+    want = torch.tanh(x @ w.detach().t() + b)
+    slope = (1 - want.to(F64) ** 2).cpu()
+    # eight ones and a bias of one: z is 9 exactly, and 1 - tanh(9)^2 is off by some 2^-24 of 1
+    close(w.grad, slope.t() @ x.cpu().to(F64), 4 * SLACK * U32 * torch.ones(6, 8, dtype=F64), "dw")
