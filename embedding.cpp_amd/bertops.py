@@ -96,6 +96,13 @@ def _vector(name: str, t: torch.Tensor, device, n: int) -> int:
     return t.data_ptr()
 
 
+def _int32(name: str, *values: int) -> None:
+    """The library takes these in 32 bits, and ctypes would cut them off without a word."""
+    for v in values:
+        if not -(1 << 31) <= v < 1 << 31:
+            raise ValueError(f"{name} {v} is over 32 bits")
+
+
 def _aligned(size: int, *matrices) -> int:
     """Whether all (address, row stride) allow 16-byte pieces."""
     bits = 0
@@ -115,6 +122,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     _first("x", x)
     _no_node("linear", x, w, bias, residual)
     (M, K), N, dt, dev, a = x.shape, w.shape[0], x.dtype, x.device, _act(act)
+    _int32("a width of", N, K)
     ldx, ldw = _matrix("x", x, dt, dev, M, K), _matrix("w", w, dt, dev, N, K)
     b = None if bias is None else _vector("bias", bias, dev, N)
     r, ldr = (None, 0) if residual is None else (residual.data_ptr(), _matrix("residual", residual, dt, dev, M, N))
@@ -135,6 +143,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *, z: Op
     """(dx, dw, dbias) of linear() from dy [M, N]; None where `need` says so.  The residual's gradient is dy."""
     _first("x", x)
     (M, K), N, dt, dev, a = x.shape, w.shape[0], x.dtype, x.device, _act(act)
+    _int32("a width of", N, K)
     ldx, ldw, lddy = _matrix("x", x, dt, dev, M, K), _matrix("w", w, dt, dev, N, K), _matrix("dy", dy, dt, dev, M, N)
     if a and z is None:
         raise ValueError(f"the gradient of {act!r} needs z: linear(..., save_z=True)")
@@ -176,6 +185,7 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, table_
         if table.dtype not in TYPES or (table_type is not None and TABLE_TYPES.get(table_type) != TYPES[table.dtype]):
             raise ValueError(f"a {table.dtype} table is not of type {table_type!r}")
         width, typ = table.shape[1], TYPES[table.dtype]
+    _int32("a table of", table.shape[0], width)
     out_dtype = out_dtype or (torch.float32 if blocks else table.dtype)
     if out_dtype not in TYPES:
         raise ValueError(f"out_dtype {out_dtype} is not supported")
@@ -194,6 +204,8 @@ def lookup_grad(dout: torch.Tensor, ids: torch.Tensor, n_rows: int, *, scale: fl
     dev, width = dout.device, dout.shape[-1]
     if tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"dout has shape {tuple(dout.shape)} for ids {tuple(ids.shape)}")
+    _int32("a table of", n_rows, width)
+    _int32("pad_id", pad_id)
     if dout.dim() != 2:
         dout = dout.reshape(-1, width)
     _first("dout", dout)

@@ -1322,3 +1322,30 @@ def test_lost_gradients_are_said():
     slope = (1 - want.to(F64) ** 2).cpu()
     # eight ones and a bias of one: z is 9 exactly, and 1 - tanh(9)^2 is off by some 2^-24 of 1
     close(w.grad, slope.t() @ x.cpu().to(F64), 4 * SLACK * U32 * torch.ones(6, 8, dtype=F64), "dw")
+
+
+# ---- sizes past 32 bits
+
+
+def test_sizes_in_32_bits():
+    for ok in (0, -1, 2**31 - 1, -(2**31)):
+        bertops._int32("n", ok)
+    for bad in (2**31, 2**32 + 5, -(2**31) - 1):
+        with pytest.raises(ValueError, match="32 bits"):
+            bertops._int32("n", 3, bad)
+
+
+@gpu
+def test_sizes_past_32_bits_are_refused():
+    """Widths, rows and padding tokens whose low 32 bits would name others."""
+    long = torch.empty(1, 2**32 + 8, dtype=torch.float16, device="cuda")
+    ids, dout = torch.arange(6, dtype=torch.int32, device="cuda"), torch.ones(6, 1, device="cuda")
+    one = torch.ones(1, 1, dtype=torch.float16, device="cuda")
+    tall = long.view(-1, 1)
+    for call in (lambda: bertops.linear(long, long), lambda: bertops.linear_backward(one, long, long),
+                 lambda: bertops.linear(one, tall), lambda: bertops.lookup(tall, ids), lambda: bertops.lookup(long, ids),
+                 lambda: bertops.lookup_grad(dout, ids, 2**32 + 8), lambda: bertops.lookup_grad(dout, ids, 6, pad_id=2**32 + 5)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+    assert bertops.lookup_grad(dout, ids, 6, pad_id=5)[:, 0].tolist() == [1.0] * 5 + [0.0]
+    assert bertops.lookup_grad(dout, ids, 6, pad_id=-(2**31))[:, 0].tolist() == [1.0] * 6
