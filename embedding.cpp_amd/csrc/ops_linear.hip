@@ -299,11 +299,16 @@ __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // 16 bytes a lane from the descriptor's base + off to LDS bytes lds .. lds + 1023.
-// The compiler sees neither the load nor its M0: a write of M0 has to be one
-// wait state ahead of a load that reads it.
+// The compiler sees neither the load nor what M0 means to it: a write of M0 has to
+// be one wait state ahead of a load that reads it, and M0 is named as overwritten
+// (clang warns that it keeps no values there itself), so that no write and use of it
+// by other instructions end up on both sides of this.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // A buffer descriptor of 2^31 bytes from `base` on.  Scalar registers that the
 // vector unit has written have to be five wait states old when a load reads
 // them, and here the compiler does not know of the load.

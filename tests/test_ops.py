@@ -1349,3 +1349,18 @@ def test_sizes_past_32_bits_are_refused():
             call()
     assert bertops.lookup_grad(dout, ids, 6, pad_id=5)[:, 0].tolist() == [1.0] * 5 + [0.0]
     assert bertops.lookup_grad(dout, ids, 6, pad_id=-(2**31))[:, 0].tolist() == [1.0] * 6
+
+
+def test_hand_written_m0_is_named_as_overwritten():
+    """Every asm statement of the kernels that writes M0 says so to the compiler."""
+    import glob
+    import re
+
+    found = 0
+    for path in glob.glob(os.path.join(os.path.dirname(bertops.__file__), "csrc", "*.h*")):
+        with open(path) as f:
+            for statement in re.findall(r"\basm\b[^;]*;", f.read()):
+                if re.search(r"s_mov_b32\s+m0", statement):
+                    found += 1
+                    assert statement.rsplit(":", 1)[1].count('"m0"') == 1, (path, statement)
+    assert found
