@@ -132,10 +132,16 @@ __device__ __forceinline__ float act_slope_f(float z, int act) {
 __device__ __forceinline__ float sigmoid_16(float v) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
 }
+// z sigmoid(v).  v_rcp_f32 gives 0 for what is under 2^-126, where z times it is still
+// one of bf16's values: both factors carry 2^14 that cancels, which takes the
+// product down to 2^-133, bf16's smallest.
+__device__ __forceinline__ float z_sigmoid_16(float z, float v) {
+    return z * 0x1p-14f * __builtin_amdgcn_rcpf(0x1p-14f + __builtin_amdgcn_exp2f(__builtin_fmaf(v, -1.4426950408889634f, -14.f)));
+}
 template <int ACT, bool WIDE>
 __device__ __forceinline__ float act_t(float z) {
-    if constexpr (!WIDE && ACT == BERT_AMD_ACT_GELU) return z * sigmoid_16(2.f * GELU_C * (z + GELU_K * z * z * z));
-    else if constexpr (!WIDE && ACT == BERT_AMD_ACT_SILU) return z * sigmoid_16(z);
+    if constexpr (!WIDE && ACT == BERT_AMD_ACT_GELU) return z_sigmoid_16(z, 2.f * GELU_C * (z + GELU_K * z * z * z));
+    else if constexpr (!WIDE && ACT == BERT_AMD_ACT_SILU) return z_sigmoid_16(z, z);
     else if constexpr (!WIDE && ACT == BERT_AMD_ACT_TANH) {
         const float q = z * z, far = 1.f - 2.f * sigmoid_16(-2.f * z);
         const float near = z * (1.f + q * (-1.f / 3 + q * (2.f / 15 - q * (17.f / 315))));  // next to zero, where `far` cancels

@@ -1364,3 +1364,28 @@ def test_hand_written_m0_is_named_as_overwritten():
                     found += 1
                     assert statement.rsplit(":", 1)[1].count('"m0"') == 1, (path, statement)
     assert found
+
+
+# ---- the activations of 16-bit layers
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("act", bertops.ACTS)
+@pytest.mark.parametrize("K,N", [(1, 1), (8, 64)])
+def test_activations_far_out_in_16_bits(act, dtype, K, N):
+    """Every activation over its whole range, down to the type's smallest values: in tiles, inside and at an edge, and few rows."""
+    dt = DTYPES[dtype]
+    z = torch.cat([torch.linspace(-110, 40, 4076, dtype=F64), torch.tensor([-6e4, -300, 0.0, 1e-4, -1e-4, 300, 6e4, 3e4], dtype=F64), torch.linspace(-12, -4, 12, dtype=F64)]).to(dt)
+    x, w = torch.zeros(len(z), K, dtype=dt), torch.zeros(N, K, dtype=dt)
+    x[:, 0], w[:, 0] = z, 1.0
+    d = z.to(F64)
+    want = act64(d, act)
+    steep = 1 + (2 * d.abs() ** 3).clamp(max=2400) if act == "gelu" else 1 + d.abs().clamp(max=200) ** (2 if act == "gelu_erf" else 1)
+    off = SLACK * U32 * steep * want.abs()
+    # off by half a step, and as much again where f32's own smallest values round next to the type's
+    tol = off + u(dt) * (want.abs() + off) + 2 * tiny(dt)
+    for rows in (slice(None), slice(4080, 4088), slice(0, 8), slice(1500, 1508)):
+        y = bertops.linear(x[rows].cuda(), w.cuda(), act=act)
+        assert N == 1 or torch.equal(y, y[:, :1].expand_as(y))
+        close(y[:, 0], want[rows], tol[rows], f"{act} {rows}")
