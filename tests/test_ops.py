@@ -1389,3 +1389,53 @@ def test_activations_far_out_in_16_bits(act, dtype, K, N):
         y = bertops.linear(x[rows].cuda(), w.cuda(), act=act)
         assert N == 1 or torch.equal(y, y[:, :1].expand_as(y))
         close(y[:, 0], want[rows], tol[rows], f"{act} {rows}")
+
+
+# ---- 8-bit states: no drift
+
+
+SIZES_IN_A_BLOCK = np.logspace(-3, 0, 256).astype(np.float32)  # many magnitudes beside the peak, none under the lowest octave
+DRIFT_STEPS, DRIFT_BLOCKS = 40, 4096
+# A code is at most 2^-3 (m) or 2^-4 (r = sqrt v) of its value from the next one, and rounding between two at random
+# varies by at most half of that.  m forgets at 0.9 a step: its standard deviation is at most 2^-4 / sqrt(1 - 0.81), the
+# blocks' mean's by sqrt(blocks) less.  v grows evenly, so that step s of T is left in r with weight s / T:
+# 2^-5 sqrt(T / 3); and r^2 is on average larger than the square of r's mean by the variance, in all at most
+# 2^-10 T / 2 of v, half of it in r.  Five deviations.
+M_LIMIT = 5 * 2.0**-4 / (1 - 0.81) ** 0.5 / DRIFT_BLOCKS**0.5
+R_LIMIT = 5 * 2.0**-5 * (DRIFT_STEPS / 3) ** 0.5 / DRIFT_BLOCKS**0.5 + 2.0**-10 * DRIFT_STEPS / 4
+
+
+def drift(m, v):
+    """How far the blocks' means of m and v are from what constant gradients give, at worst, as parts of it."""
+    g = SIZES_IN_A_BLOCK.astype(np.float64)
+    want_m, want_r = g * (1 - 0.9**DRIFT_STEPS), g * (1 - 0.999**DRIFT_STEPS) ** 0.5
+    m, v = (np.asarray(x, np.float64).reshape(-1, 256).mean(0) for x in (m, v))
+    return abs(m / want_m - 1).max(), abs(np.sqrt(v) / want_r - 1).max()
+
+
+def test_drift_limits_tell_other_roundings():
+    """Rounding to the nearest code, up or down, the same in every block, is over both limits."""
+    f, g = np.float32, SIZES_IN_A_BLOCK
+    for bits in (0x80000000, 0xFFFFFFFF, 0):
+        h = np.full(256, bits, np.uint32)
+        m, v = np.zeros(256, f), np.zeros(256, f)
+        for _ in range(DRIFT_STEPS):
+            m, v = m * f(0.9) + g * f(0.1), v * f(0.999) + (g * f(1 - 0.999)) * g
+            c, s = encode(m, 3, h)
+            m = code_values(3)[c] * s[0]
+            c, s = encode(np.sqrt(v), 4, h)
+            v = (code_values(4)[np.maximum(c, 1)] * s[0]) ** 2
+        far_m, far_r = drift(m, v)
+        assert far_m > 2 * M_LIMIT and far_r > 1.4 * R_LIMIT, (hex(bits), far_m, far_r)
+
+
+@gpu
+@pytest.mark.parametrize("seed", [1, 2**31])
+def test_adamw_8_bit_states_have_no_drift(seed):
+    """The same 256 magnitudes in every block: each place's stored moments average to the exact ones over the blocks."""
+    g = torch.from_numpy(np.tile(SIZES_IN_A_BLOCK, DRIFT_BLOCKS)).cuda()
+    opt = bertops.AdamW([torch.zeros_like(g)], bits=8, seed=seed)
+    for _ in range(DRIFT_STEPS):
+        opt.step([g])
+    far_m, far_r = drift(*(x.cpu().numpy() for x in opt.moments()))
+    assert far_m < M_LIMIT and far_r < R_LIMIT, (far_m, far_r)
