@@ -1439,3 +1439,83 @@ def test_adamw_8_bit_states_have_no_drift(seed):
         opt.step([g])
     far_m, far_r = drift(*(x.cpu().numpy() for x in opt.moments()))
     assert far_m < M_LIMIT and far_r < R_LIMIT, (far_m, far_r)
+
+
+# ---- outputs with rows further apart than their width, through the C entry points
+
+
+def wider(rows, cols, pad, dtype):
+    return strided(torch.zeros(rows, cols, dtype=dtype, device="cuda"), pad)
+
+
+def gap_is_untouched(t):
+    return bool(torch.isnan(t._base[:, t.shape[1]:]).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pad", [1, 3, 8])
+@pytest.mark.parametrize("M,K,N", [(1, 36, 20), (5, 264, 130), (8, 1000, 777), (20, 2000, 24), (70, 96, 130), (300, 384, 384), (1100, 130, 264)])
+def test_strided_outputs(M, K, N, pad, dtype):
+    """y, z, dx and dw into wider rows: the same bits as into contiguous ones, and nothing between the rows."""
+    L, dt = bertlib.lib(), DTYPES[dtype]
+    x, w, dy, b = (t.cuda() for t in make_layer(M, K, N, dt, seed=80))
+    typ, stream = bertops.TYPES[dt], torch.cuda.current_stream().cuda_stream
+    room = torch.empty(max(L.bert_amd_linear_workspace(typ, M, N, K, 0), L.bert_amd_linear_backward_workspace(typ, 2, M, N, K, 0), 16), dtype=torch.uint8, device="cuda")
+    ws = (room.data_ptr(), room.numel())
+    for act in ("none", "gelu", "tanh"):
+        a = bertops.ACTS[act]
+        want_y, want_z = bertops.linear(x, w, b, residual=dy, act=act, save_z=True)
+        y, z = wider(M, N, pad, dt), wider(M, N, pad, dt)
+        assert L.bert_amd_linear(0, typ, a, M, N, K, x.data_ptr(), K, w.data_ptr(), K, b.data_ptr(), dy.data_ptr(), N, y.data_ptr(), N + pad, z.data_ptr(), N + pad, *ws, stream) == 0
+        want = bertops.linear_backward(dy, x, w, z=want_z, act=act)
+        dx, dw, db = wider(M, K, pad, dt), wider(N, K, pad, dt), torch.empty(N, device="cuda")
+        assert L.bert_amd_linear_backward(0, typ, a, M, N, K, dy.data_ptr(), N, z.data_ptr(), N + pad, x.data_ptr(), K, w.data_ptr(), K, dx.data_ptr(), K + pad, dw.data_ptr(), K + pad, db.data_ptr(), *ws, stream) == 0
+        for got, expected in ((y, want_y), (z, want_z), (dx, want[0]), (dw, want[1])):
+            assert torch.equal(got, expected) and gap_is_untouched(got), act
+        assert torch.equal(db, want[2])
+
+
+FIRST_GRADIENTS = """
+import sys
+sys.path[:0] = sys.argv[1:]
+import torch, bertops
+g = torch.Generator(device="cuda").manual_seed(90)
+def normal(*s, t=torch.float32): return torch.randn(*s, generator=g, device="cuda").to(t)
+layers = [(normal(M, K, t=t), normal(N, K, t=t), normal(M, N, t=t)) for M, K, N, t in
+          ((1, 384, 384, torch.float32), (7, 130, 77, torch.bfloat16), (300, 384, 384, torch.float32), (200, 64, 96, torch.float16), (1000, 72, 2500, torch.bfloat16))]
+ids = torch.randint(-1, 50, (900,), generator=g, device="cuda").int()
+dout = normal(900, 1023)
+into = normal(50, 1023)
+def calls():
+    out = []
+    for x, w, dy in layers:
+        out += bertops.linear(x, w, act="gelu_erf", save_z=True)
+        out += bertops.linear_backward(dy, x, w, z=dy, act="silu")
+    out += [bertops.lookup_grad(dout, ids, 50), bertops.lookup_grad(dout, ids, 50, out=into.clone(), accumulate=True)]
+    out += [bertops.lookup(into, ids, scale=3.0, out_dtype=torch.float16)]
+    return out
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls()
+for k in range(4):
+    graph.replay()
+    want = calls()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want)), k
+    for x, w, dy in layers:
+        x.mul_(-0.75)
+        dy.add_(0.25)
+    ids.add_(1)
+    into.mul_(0.5)
+    torch.cuda.synchronize()
+print("four replays")
+"""
+
+
+@gpu
+def test_first_gradients_are_captured():
+    """As test_first_calls_are_captured, for the gradients of few rows, of small layers in a pair and of wide ones, and few places."""
+    done = subprocess.run([sys.executable, "-c", FIRST_GRADIENTS, os.path.dirname(bertops.__file__)], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "four replays" in done.stdout, done.stderr[-2000:]
