@@ -223,3 +223,16 @@ def test_shard_cuts_balance_and_cover(n_rep):
             assert all(cut[r + 1] > cut[r] for r in range(n_rep)), cut
     with pytest.raises(ValueError):
         bertlib.shard_cuts([1, 2], 0)
+
+
+def test_build_compiles_what_is_built_already(monkeypatch, repo):
+    """build() runs every compile again: an object newer than its source says nothing of the compiler's options."""
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("graft_entry", os.path.join(repo, "__graft_entry__.py"))
+    entry = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(entry)
+    ran = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: ran.append(cmd) or subprocess.CompletedProcess(cmd, 0))
+    entry.build()
+    assert len(ran) >= 2 and all(cmd[0] == "make" and "-B" in cmd for cmd in ran[:2])
