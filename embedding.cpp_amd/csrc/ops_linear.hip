@@ -6,8 +6,8 @@
 // error of half a step in each term, where the result is rounded by half a
 // step once more (bf16 16384 x 1024 x 4096 with gelu: dx and dw are 2.34e-3 off in
 // the mean square, of which the result's own rounding is 1.66e-3 and f32 sums
-// 1.4e-4); db sums the unrounded dz.  Without that rounding dz would have to be
-// taken as two 16-bit halves: twice the products' time.
+// 1.4e-4); db sums the unrounded dz.  Small layers go without that rounding, dz in
+// two 16-bit halves (dz_passes): up to twice the products' time.
 #include "ops_common.h"
 
 #include <algorithm>
@@ -40,6 +40,7 @@ struct Operand {
     int64_t ld = 0;
     bool vec = false;  // p and ld allow 16-byte loads
     bool padded = false;  // zeros follow a row up to a multiple of 16 bytes
+    int64_t rest = 0;     // dz in two halves: bytes from the first to the second
 };
 struct Epilogue {
     int act = 0;
@@ -331,6 +332,8 @@ struct Tile {
     static constexpr int CHUNKS = R / CH;                           // of a k row, if TRANS
     const char *base;     // of the stage to load next
     int64_t step;         // bytes from a stage to the next
+    int64_t jump = 0;     // and, once `until` stages are loaded, to the first one of a second pass over k
+    int until = 0;
     uint32_t off[LOADS];  // from base
     int at[LOADS];        // the chunk's k within the stage
 
@@ -362,10 +365,14 @@ struct Tile {
             }
         }
     }
+    // a second pass over the same `stages`, `rest` bytes further on
+    __device__ __forceinline__ void again(int stages, int64_t rest) { until = stages, jump = rest - stages * step; }
     // the descriptor of the next stage to load
+    template <bool TWO>
     __device__ __forceinline__ u32x4 next_stage() {
         const u32x4 d = descriptor(base);
         base += step;
+        if (TWO && --until == 0) base += jump;
         return d;
     }
     // loads FROM .. TO - 1 of a stage to `lds`; `left`: k from the stage's start to the end
@@ -453,8 +460,8 @@ struct Product {
     bool vec = false;                      // the epilogue's rows are aligned
 };
 
-// `block` of p.tiles, part `split` of k
-template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
+// `block` of p.tiles, part `split` of k; TWO: A is the sum of two matrices, A.rest apart, k is gone over twice
+template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN, bool TWO>
 __device__ __forceinline__ void stage_product(const Product &p, char *smem, int block, int split) {
     typedef typename Elem<TYPE>::T T;
     const Operand A = p.A, B = p.B;
@@ -490,14 +497,19 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
             for (int i = 0; i < 8; i++) biases[h][i] = e.bias[min(n0 + wn + 64 * h + 8 * (lane & 7) + i, N - 1)];
     f32x16 acc[TM][TN] = {};
     constexpr int SK = stage_k<TYPE>(), KS = 4;
+    const int64_t span = ceil_div(kb - ka, (int64_t)SK) * SK, end = TWO ? ka + 2 * span : kb;
+    if constexpr (TWO) ta.again((int)(span / SK), A.rest), tb.again((int)(span / SK), 0);
     u32x4 a[2][TM], b[2][TN];
     const auto read_a = [&](int set, int i, int from, int ks) { a[set][i] = TileA::read(smem + from * STAGE, wm + 32 * i, ks); };
     const auto read_b = [&](int set, int i, int from, int ks) { b[set][i] = TileB::read(smem + from * STAGE + TileA::BYTES, wn + 32 * i, ks); };
-    const auto left_at = [&](int64_t k0) { return (int)max((int64_t)0, min((int64_t)SK, kb - k0)); };
+    const auto left_at = [&](int64_t k0) {
+        if (TWO && k0 >= ka + span) k0 -= span;
+        return (int)max((int64_t)0, min((int64_t)SK, kb - k0));
+    };
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        ta.template load<0, TileA::LOADS>(ta.next_stage(), lds + i * STAGE, left_at(ka + i * SK));
-        tb.template load<0, TileB::LOADS>(tb.next_stage(), lds + i * STAGE + TileA::BYTES, left_at(ka + i * SK));
+        ta.template load<0, TileA::LOADS>(ta.template next_stage<TWO>(), lds + i * STAGE, left_at(ka + i * SK));
+        tb.template load<0, TileB::LOADS>(tb.template next_stage<TWO>(), lds + i * STAGE + TileA::BYTES, left_at(ka + i * SK));
     }
     wait_loads<TileA::LOADS + TileB::LOADS>();
     barrier();
@@ -507,7 +519,7 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
     for (int i = 0; i < TM; i++) read_a(0, i, 0, 0);
     int buf = 0;
     u32x4 stage = {};
-    for (int64_t k0 = ka; k0 < kb; k0 += SK, buf ^= 1) {
+    for (int64_t k0 = ka; k0 < end; k0 += SK, buf ^= 1) {
         // The loads of the stage after the next go out between the products of
         // this stage's last quarter (its second matrix, once the barrier has freed
         // the buffer) and the next stage's first (its first matrix): a burst of them would hold up
@@ -520,9 +532,9 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
                 wait_reads();
                 wait_loads<0>();
                 barrier();
-                stage = tb.next_stage();
+                stage = tb.template next_stage<TWO>();
             }
-            if (ks == 0 && k0 > ka) stage = ta.next_stage();
+            if (ks == 0 && k0 > ka) stage = ta.template next_stage<TWO>();
             for_const<TM>([&](auto ic) {
                 constexpr int i = ic.value;
                 if (ks == KS - 1) tb.template load<i * TileB::LOADS / TM, (i + 1) * TileB::LOADS / TM>(stage, lds + buf * STAGE + TileA::BYTES, left_at(k0 + 2 * SK));
@@ -615,22 +627,22 @@ __device__ __forceinline__ void stage_product(const Product &p, char *smem, int 
     }
 }
 
-template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
+template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN, bool TWO>
 __global__ __launch_bounds__(WM *WN * 64, 2) void stage_gemm_kernel(Product p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    stage_product<TYPE, TA, TBT, BM, BN, WM, WN>(p, smem, blockIdx.x, blockIdx.z);
+    stage_product<TYPE, TA, TBT, BM, BN, WM, WN, TWO>(p, smem, blockIdx.x, blockIdx.z);
 }
 
 // Both products of a small layer's gradients at once, in tiles of 64 x BN: each
 // alone leaves most of the chip idle, and a launch less counts there.
-template <int TYPE, int BN, int WN>
+template <int TYPE, int BN, int WN, bool TWO>
 __global__ __launch_bounds__(128 * WN, 2) void pair_gemm_kernel(Product dx, Product dw) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int first = dx.tiles * dx.parts, b = blockIdx.x;
     if (b < first)
-        stage_product<TYPE, false, true, 64, BN, 2, WN>(dx, smem, b % dx.tiles, b / dx.tiles);
+        stage_product<TYPE, false, true, 64, BN, 2, WN, TWO>(dx, smem, b % dx.tiles, b / dx.tiles);
     else
-        stage_product<TYPE, true, true, 64, BN, 2, WN>(dw, smem, (b - first) % dw.tiles, (b - first) / dw.tiles);
+        stage_product<TYPE, true, true, 64, BN, 2, WN, TWO>(dw, smem, (b - first) % dw.tiles, (b - first) / dw.tiles);
 }
 
 // The parts of one or two products (blockIdx.y) added in order, COLS columns a
@@ -668,12 +680,20 @@ __global__ __launch_bounds__(256) void split_join_kernel(Product a, Product b) {
 }
 
 // dz = dy act'(z) in the layer's type, rows `lddz` apart with zeros past their
-// end, and the unrounded dz's column sums over `rows` rows at a time: CT
+// end (`rest`: and there what that rounding left, a finite dz past the type's largest
+// value with it), and the unrounded dz's column sums over `rows` rows at a time: CT
 // threads of 8 columns each, 256 / CT rows side by side, their sums joined in
 // LDS in a fixed order.
+template <typename T>
+__device__ __forceinline__ void halves(float v, float &high, float &low) {
+    constexpr float MOST = std::is_same<T, _Float16>::value ? 65504.f : 0x1.fep127f;
+    high = (float)(T)v;
+    if (fabsf(high) > MOST && fabsf(v) <= 0x1.fffffep127f) high = v > 0.f ? MOST : -MOST;
+    low = fabsf(high) <= MOST ? v - high : 0.f;
+}
 template <typename T, int CT>
 __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, const T *z, int64_t ldz, int act, int64_t M, int64_t N,
-                                                 int64_t rows, T *dz, int64_t lddz, float *part, bool vec) {
+                                                 int64_t rows, T *dz, T *rest, int64_t lddz, float *part, bool vec) {
     constexpr int RT = 256 / CT;
     __shared__ float sums[RT][CT][9];
     const int c = threadIdx.x % CT, r = threadIdx.x / CT;
@@ -696,15 +716,26 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
         }
         if (act) slope8<T>(v, s, act);
         if (dz) {
-            if (n + 8 <= lddz) {
+            const auto keep = [&](T *to, const float *from) {
+                if (n + 8 <= lddz) {
+                    put8(to + m * lddz + n, from);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (n + i >= N) v[i] = 0.f;
-                put8(dz + m * lddz + n, v);
+                    for (int i = 0; i < 8; i++)
+                        if (n + i < lddz) to[m * lddz + n + i] = (T)from[i];
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (n + i >= N) v[i] = 0.f;
+            if (!rest) {
+                keep(dz, v);
             } else {
+                float high[8], low[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (n + i < lddz) dz[m * lddz + n + i] = n + i < N ? (T)v[i] : (T)0.f;
+                for (int i = 0; i < 8; i++) halves<T>(v[i], high[i], low[i]);
+                keep(dz, high);
+                keep(rest, low);
             }
         }
 #pragma unroll
@@ -792,7 +823,7 @@ struct Plan {
 // in 256 wide, 40 in 128, 59 in 64; bf16 1536 x 384 over k = 65536 123 in 21
 // parts of 256 wide tiles, 549 unsplit in 64 wide.  The choice was on average
 // 1 % off the best measured, at most 9 %.
-Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
+Plan plan_for(int type, int64_t M, int64_t N, int64_t K, int passes = 1) {
     struct Form {
         int rows, cols;
         double alone, more, around;
@@ -814,7 +845,7 @@ Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
             if (n < 1 || (n > 1 && (n > 64 || K < n * sk * 2 || tiles * n > 1600))) continue;
             const int64_t per = std::max<int64_t>(64, ceil_div(ceil_div(K, n), (int64_t)64) * 64), parts = ceil_div(K, per);
             const int64_t each = ceil_div(tiles * parts, (int64_t)256), left = each % f.holds;
-            const double stages = (double)ceil_div(per, (int64_t)sk);
+            const double stages = (double)passes * ceil_div(per, (int64_t)sk);
             const auto round = [&](int64_t wgs) { return stages * (f.alone + (wgs - 1) * f.more) + f.around; };
             const double t = each / f.holds * round(f.holds) + (left ? round(left) : 0) + (parts > 1 ? 3.7 + 1.6e-6 * parts * M * N : 0);
             if (t < least) least = t, best = {f.rows, f.cols, (int)parts, per};
@@ -824,16 +855,28 @@ Plan plan_for(int type, int64_t M, int64_t N, int64_t K) {
     return best;
 }
 // bytes of a product's split sums
-int64_t split_bytes(int type, int64_t M, int64_t N, int64_t K) {
-    const Plan p = plan_for(type, M, N, K);
+int64_t split_bytes(int type, int64_t M, int64_t N, int64_t K, int passes = 1) {
+    const Plan p = plan_for(type, M, N, K, passes);
     return p.splits > 1 ? round256(p.splits * M * N * 4) : 0;
 }
 
 // whether a layer's two gradient products share a launch: both in the same
 // small tiles (256 x 384 x 384 in f32 29 -> 22 us for all three gradients)
-bool gradients_in_pair(int type, int64_t M, int64_t N, int64_t K) {
-    const Plan dx = plan_for(type, M, K, N), dw = plan_for(type, N, K, M);
+bool gradients_in_pair(int type, int64_t M, int64_t N, int64_t K, int passes) {
+    const Plan dx = plan_for(type, M, K, N, passes), dw = plan_for(type, N, K, M, passes);
     return M > 0 && dx.rows == 64 && dw.rows == 64 && dx.cols == dw.cols;
+}
+
+// Passes over dz in the gradients' products: two, of its two halves, where dx or dw
+// has few elements.  With dz rounded both are 1.41 times as far off as their own
+// rounding in the mean square, give or take 1.2 over the root of their size (f16
+// 1065 x 20 x 11: up to 1.66); in two halves 1.00.  us for all three gradients, rounded
+// and in halves: bf16 9 x 64 x 64 7.8 and 8.7, 64 x 64 x 64 7.2 and 8.0, 1065 x 20 x 11
+// 16.7 and 17.5, but 256 x 384 x 384 10.4 and 14.6, 1024 x 1024 x 1024 25 and 38,
+// 16384 x 1024 x 4096 354 and 610.
+constexpr int64_t FEW_RESULTS = 4096;
+int dz_passes(int type, int act, int64_t M, int64_t N, int64_t K) {
+    return type != BERT_AMD_F32 && act != BERT_AMD_ACT_NONE && std::min(M, N) * K <= FEW_RESULTS ? 2 : 1;
 }
 
 // Up to 8 rows, and no more than 8192 columns of dz: with more the tiles' workgroups
@@ -890,10 +933,10 @@ constexpr int stage_lds(int BM, int BN, int WM, int WN) {
     return std::max(2 * (BM + BN) * 128, std::min(BM / WM, 64) * WM * WN * OUT_LD * 4);
 }
 
-template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN>
+template <int TYPE, bool TA, bool TBT, int BM, int BN, int WM, int WN, bool TWO>
 hipError_t launch_stage(const Product &p, hipStream_t s) {
     constexpr int lds = stage_lds(BM, BN, WM, WN);
-    const auto k = stage_gemm_kernel<TYPE, TA, TBT, BM, BN, WM, WN>;
+    const auto k = stage_gemm_kernel<TYPE, TA, TBT, BM, BN, WM, WN, TWO>;
     if (lds > 65536) {  // beyond a launch's default: asked for once on each device
         static std::atomic<uint64_t> asked{0};
         int dev = 0;
@@ -919,15 +962,15 @@ hipError_t join(const Product &a, const Product &b, hipStream_t s) {
 }
 
 // C = A B^T of two matrices in whole chunks
-template <int TYPE, bool TA, bool TBT>
+template <int TYPE, bool TA, bool TBT, bool TWO = false>
 hipError_t gemm(const Operand &A, const Operand &B, int64_t M, int64_t N, int64_t K, void *ws, const Epilogue &e, hipStream_t s) {
-    const Plan plan = plan_for(TYPE, M, N, K);
+    const Plan plan = plan_for(TYPE, M, N, K, TWO ? 2 : 1);
     const Product p = product<TYPE>(A, B, M, N, K, plan, ws, e);
     hipError_t r = hipSuccess;
-    if (plan.cols == 64) r = launch_stage<TYPE, TA, TBT, 64, 64, 2, 1>(p, s);
-    else if (plan.rows == 128) r = launch_stage<TYPE, TA, TBT, 128, 128, 2, 2>(p, s);
-    else if constexpr (TYPE == BERT_AMD_F32) r = launch_stage<TYPE, TA, TBT, 64, 128, 2, 2>(p, s);
-    else r = launch_stage<TYPE, TA, TBT, 256, 256, 2, 4>(p, s);
+    if (plan.cols == 64) r = launch_stage<TYPE, TA, TBT, 64, 64, 2, 1, TWO>(p, s);
+    else if (plan.rows == 128) r = launch_stage<TYPE, TA, TBT, 128, 128, 2, 2, TWO>(p, s);
+    else if constexpr (TYPE == BERT_AMD_F32) r = launch_stage<TYPE, TA, TBT, 64, 128, 2, 2, TWO>(p, s);
+    else r = launch_stage<TYPE, TA, TBT, 256, 256, 2, 4, TWO>(p, s);
     return r != hipSuccess ? r : join<typename Elem<TYPE>::T>(p, Product(), s);
 }
 
@@ -979,6 +1022,46 @@ hipError_t few_rows_grad(const LinearGradArgs &a, hipStream_t s) {
     return join<T>(dx, Product(), s);
 }
 
+// dx = dz W and dw = dz^T x
+template <int TYPE, bool TWO>
+hipError_t grad_products(const LinearGradArgs &a, const Operand &dz, char *ws, hipStream_t s) {
+    typedef typename Elem<TYPE>::T T;
+    constexpr int PASSES = TWO ? 2 : 1;
+    Epilogue ex, ew;
+    ex.y = a.dx, ex.ldy = a.lddx;
+    ew.y = a.dw, ew.ldy = a.lddw;
+    if (a.dx && a.dw && gradients_in_pair(TYPE, a.M, a.N, a.K, PASSES)) {
+        Operand wx[] = {operand(a.w, a.ldw, TYPE), operand(a.x, a.ldx, TYPE)};
+        const int64_t rows[] = {a.N, a.M};
+        if (hipError_t r = pack<T>(TYPE, wx, rows, 2, a.K, ws, s); r != hipSuccess) return r;
+        const Plan plan = plan_for(TYPE, a.M, a.K, a.N, PASSES);
+        const Product dx = product<TYPE>(dz, wx[0], a.M, a.K, a.N, plan, ws, ex);
+        ws += split_bytes(TYPE, a.M, a.K, a.N, PASSES);
+        const Product dw = product<TYPE>(dz, wx[1], a.N, a.K, a.M, plan_for(TYPE, a.N, a.K, a.M, PASSES), ws, ew);
+        const dim3 grid(dx.tiles * dx.parts + dw.tiles * dw.parts);
+        hipError_t r = hipErrorInvalidValue;
+        if (plan.cols == 64)
+            r = launch(pair_gemm_kernel<TYPE, 64, 1, TWO>, grid, dim3(128), stage_lds(64, 64, 2, 1), s, dx, dw);
+        else if constexpr (TYPE == BERT_AMD_F32)
+            r = launch(pair_gemm_kernel<TYPE, 128, 2, TWO>, grid, dim3(256), stage_lds(64, 128, 2, 2), s, dx, dw);
+        return r != hipSuccess ? r : join<T>(dx, dw, s);
+    }
+    if (a.dx && a.M) {
+        char *rest = ws;
+        Operand w = operand(a.w, a.ldw, TYPE);
+        const int64_t rows = a.N;
+        if (hipError_t r = pack<T>(TYPE, &w, &rows, 1, a.K, rest, s); r != hipSuccess) return r;
+        if (hipError_t r = gemm<TYPE, false, true, TWO>(dz, w, a.M, a.K, a.N, rest, ex, s); r != hipSuccess) return r;
+    }
+    if (a.dw) {
+        char *rest = ws;
+        Operand x = operand(a.x, a.ldx, TYPE);
+        if (hipError_t r = pack<T>(TYPE, &x, &a.M, 1, a.K, rest, s); r != hipSuccess) return r;
+        if (hipError_t r = gemm<TYPE, true, true, TWO>(dz, x, a.N, a.K, a.M, rest, ew, s); r != hipSuccess) return r;
+    }
+    return hipSuccess;
+}
+
 template <int TYPE>
 hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
     typedef typename Elem<TYPE>::T T;
@@ -987,10 +1070,14 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
     Operand dz = operand(a.dy, a.lddy, TYPE);
     T *kept = nullptr;
     const int64_t lddz = padded(TYPE, a.N);
+    const int passes = dz_passes(TYPE, a.act, a.M, a.N, a.K);
+    T *rest = nullptr;
     if ((a.dx || a.dw) && (a.act || !whole_rows(dz, TYPE, a.N))) {
+        const int64_t bytes = packed_bytes(TYPE, a.M, a.N);
         kept = (T *)ws;
-        ws += packed_bytes(TYPE, a.M, a.N);
-        dz = {kept, lddz, true, true};
+        if (passes == 2) rest = (T *)(ws + bytes);
+        ws += passes * bytes;
+        dz = {kept, lddz, true, true, bytes};
     }
     if ((kept || a.db) && a.M) {
         const DzPlan plan = dz_plan(a.M, a.N);
@@ -1000,7 +1087,7 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
         const auto kernel = plan.narrow ? dz_kernel<T, 1> : dz_kernel<T, 32>;
         const dim3 grid(ceil_div(a.N, plan.narrow ? 8 : 256), blocks);
         if (hipError_t r = launch(kernel, grid, dim3(256), 0, s, (const T *)a.dy, a.lddy, (const T *)a.z, a.ldz, a.act, a.M, a.N, rows, kept,
-                                  lddz, part, vec);
+                                  rest, lddz, part, vec);
             r != hipSuccess)
             return r;
         if (a.db && blocks > 1) {
@@ -1010,39 +1097,9 @@ hipError_t linear_grad_t(const LinearGradArgs &a, hipStream_t s) {
     } else if (a.db) {
         if (hipError_t r = launch(column_sum_kernel, dim3(ceil_div(a.N, 16)), dim3(1024), 0, s, nullptr, 0, a.N, a.db); r != hipSuccess) return r;
     }
-    Epilogue ex, ew;
-    ex.y = a.dx, ex.ldy = a.lddx;
-    ew.y = a.dw, ew.ldy = a.lddw;
-    if (a.dx && a.dw && gradients_in_pair(TYPE, a.M, a.N, a.K)) {
-        Operand wx[] = {operand(a.w, a.ldw, TYPE), operand(a.x, a.ldx, TYPE)};
-        const int64_t rows[] = {a.N, a.M};
-        if (hipError_t r = pack<T>(TYPE, wx, rows, 2, a.K, ws, s); r != hipSuccess) return r;
-        const Plan plan = plan_for(TYPE, a.M, a.K, a.N);
-        const Product dx = product<TYPE>(dz, wx[0], a.M, a.K, a.N, plan, ws, ex);
-        ws += split_bytes(TYPE, a.M, a.K, a.N);
-        const Product dw = product<TYPE>(dz, wx[1], a.N, a.K, a.M, plan_for(TYPE, a.N, a.K, a.M), ws, ew);
-        const dim3 grid(dx.tiles * dx.parts + dw.tiles * dw.parts);
-        hipError_t r = hipErrorInvalidValue;
-        if (plan.cols == 64)
-            r = launch(pair_gemm_kernel<TYPE, 64, 1>, grid, dim3(128), stage_lds(64, 64, 2, 1), s, dx, dw);
-        else if constexpr (TYPE == BERT_AMD_F32)
-            r = launch(pair_gemm_kernel<TYPE, 128, 2>, grid, dim3(256), stage_lds(64, 128, 2, 2), s, dx, dw);
-        return r != hipSuccess ? r : join<T>(dx, dw, s);
-    }
-    if (a.dx && a.M) {
-        char *rest = ws;
-        Operand w = operand(a.w, a.ldw, TYPE);
-        const int64_t rows = a.N;
-        if (hipError_t r = pack<T>(TYPE, &w, &rows, 1, a.K, rest, s); r != hipSuccess) return r;
-        if (hipError_t r = gemm<TYPE, false, true>(dz, w, a.M, a.K, a.N, rest, ex, s); r != hipSuccess) return r;
-    }
-    if (a.dw) {
-        char *rest = ws;
-        Operand x = operand(a.x, a.ldx, TYPE);
-        if (hipError_t r = pack<T>(TYPE, &x, &a.M, 1, a.K, rest, s); r != hipSuccess) return r;
-        if (hipError_t r = gemm<TYPE, true, true>(dz, x, a.N, a.K, a.M, rest, ew, s); r != hipSuccess) return r;
-    }
-    return hipSuccess;
+    if constexpr (TYPE != BERT_AMD_F32)
+        if (passes == 2) return grad_products<TYPE, true>(a, dz, ws, s);
+    return grad_products<TYPE, false>(a, dz, ws, s);
 }
 
 }  // namespace
@@ -1064,10 +1121,11 @@ hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
 int64_t linear_grad_ws_bytes(int type, int act, int64_t M, int N, int K, bool aligned) {
     if (few_grads(M, N)) return round256(few_grad_parts(N, K) * M * K * 4);
     const bool whole_n = aligned && padded(type, N) == N, whole_k = aligned && padded(type, K) == K;
-    const int64_t for_dx = (whole_k ? 0 : packed_bytes(type, N, K)) + split_bytes(type, M, K, N);
-    const int64_t for_dw = (whole_k ? 0 : packed_bytes(type, M, K)) + split_bytes(type, N, K, M);
-    return (act || !whole_n ? packed_bytes(type, M, N) : 0) + round256(ceil_div<int64_t>(M, dz_plan(M, N).rows) * N * 4) +
-           (gradients_in_pair(type, M, N, K) ? for_dx + for_dw : std::max(for_dx, for_dw));
+    const int passes = dz_passes(type, act, M, N, K);
+    const int64_t for_dx = (whole_k ? 0 : packed_bytes(type, N, K)) + split_bytes(type, M, K, N, passes);
+    const int64_t for_dw = (whole_k ? 0 : packed_bytes(type, M, K)) + split_bytes(type, N, K, M, passes);
+    return (act || !whole_n ? passes * packed_bytes(type, M, N) : 0) + round256(ceil_div<int64_t>(M, dz_plan(M, N).rows) * N * 4) +
+           (gradients_in_pair(type, M, N, K, passes) ? for_dx + for_dw : std::max(for_dx, for_dw));
 }
 
 hipError_t launch_linear_grad(const LinearGradArgs &a, hipStream_t s) {

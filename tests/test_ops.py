@@ -924,10 +924,10 @@ def rounded_between(v, off, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M,K,N,pad", [(1, 40, 9000, 0), (5, 72, 8200, 3), (8, 8, 9001, 0), (9, 96, 130, 0), (12, 1000, 48, 1), (40, 384, 384, 0), (63, 130, 257, 8), (64, 512, 64, 0), (700, 256, 512, 0)])
+@pytest.mark.parametrize("M,K,N,pad", [(1, 40, 9000, 0), (5, 72, 8200, 3), (8, 8, 9001, 0), (9, 96, 130, 0), (12, 1000, 48, 1), (40, 384, 384, 0), (63, 130, 257, 8), (64, 512, 64, 0), (700, 256, 512, 0), (9, 64, 64, 0), (64, 64, 64, 0), (1065, 20, 11, 5), (9, 455, 300, 0), (130, 31, 132, 0), (131, 33, 124, 1), (20000, 8, 12, 0), (3000, 1, 4096, 0), (4000, 3, 1366, 0)])
 def test_linear_backward_rounds_dz_once(M, K, N, pad, dtype):
-    """Past 8 rows or 8192 columns: dz rounded to the layer's type (f32: not at all), and from there on nothing is
-    lost but sums in f32 and each result's own rounding.  f32 operands are taken whole."""
+    """Past 8 rows or 8192 columns: dz rounded to the layer's type (f32 and where dx or dw has few elements: not at
+    all), and from there on nothing is lost but sums in f32 and each result's own rounding.  f32 operands are taken whole."""
     dt = DTYPES[dtype]
     x, w, dy, _ = make_layer(M, K, N, dt, seed=30)
     z = normal(gen(31), M, N).to(dt)
@@ -937,7 +937,11 @@ def test_linear_backward_rounds_dz_once(M, K, N, pad, dtype):
         at = z.to(F64).clone().requires_grad_(True)
         (dz,) = torch.autograd.grad(act64(at, act), at, dy.to(F64))
         off = SLACK * U32 * (1 + z.to(F64).abs()) * dy.to(F64).abs() * (act != "none")
-        kept, apart = rounded_between(dz, off, dt) if dt != torch.float32 else (dz, off)
+        kept, apart = rounded_between(dz, off, dt)
+        if dt == torch.float32:
+            kept, apart = dz, off
+        elif act != "none" and min(M, N) * K <= 4096:  # two halves: the second is what the first left, rounded
+            kept, apart = dz, off + 2 * u(dt) ** 2 * dz.abs() + tiny(dt)
         for got, a, o, b, n, what in ((dx, kept, apart, w, N, "dx"), (dw, kept.t(), apart.t(), x, M, "dw")):
             want, far = a @ b.to(F64), (o + (n + 1) * U32 * (a.abs() + o)) @ b.to(F64).abs()
             close(got, want, far + u(dt) * (want.abs() + far) + tiny(dt), f"{what} {act}")
@@ -1519,3 +1523,23 @@ def test_first_gradients_are_captured():
     """As test_first_calls_are_captured, for the gradients of few rows, of small layers in a pair and of wide ones, and few places."""
     done = subprocess.run([sys.executable, "-c", FIRST_GRADIENTS, os.path.dirname(bertops.__file__)], capture_output=True, text=True, timeout=100)
     assert done.returncode == 0 and "four replays" in done.stdout, done.stderr[-2000:]
+
+
+@gpu
+def test_f16_dz_past_its_largest_value():
+    """dy next to f16's largest value times a slope over 1, in a layer small enough for halves: gradients are finite."""
+    M, K, N = 40, 16, 24
+    x, w, _, _ = make_layer(M, K, N, torch.float16, seed=95)
+    dy, z = torch.full((M, N), 65504.0).half(), torch.full((M, N), 1.5).half()  # GELU's slope there is 1.13
+    w, x = w / 64, x / 1024
+    dx, dw, db = bertops.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z=z.cuda(), act="gelu")
+    at = z.to(F64).clone().requires_grad_(True)
+    (dz,) = torch.autograd.grad(act64(at, "gelu"), at, dy.to(F64))
+    assert (dz > 65520).all()
+    far = dz * SLACK * U32 + 2 * u(torch.float16) ** 2 * dz
+    for got, a, b, o in ((dx, dz, w, far), (dw, dz.t(), x, far.t())):
+        want, o = a @ b.to(F64), (o + 50 * U32 * a) @ b.to(F64).abs()
+        close(got, want, o + u(torch.float16) * (want.abs() + o) + tiny(torch.float16), "gradient")
+    dy[0, 0] = float("inf")
+    dx, dw, db = bertops.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z=z.cuda(), act="gelu")
+    assert not torch.isfinite(dx[0]).any() and torch.isfinite(dx[1:]).all() and not torch.isnan(db).any()
