@@ -867,16 +867,16 @@ bool gradients_in_pair(int type, int64_t M, int64_t N, int64_t K, int passes) {
     return M > 0 && dx.rows == 64 && dw.rows == 64 && dx.cols == dw.cols;
 }
 
-// Passes over dz in the gradients' products: two, of its two halves, where dx or dw
-// has few elements.  With dz rounded both are 1.41 times as far off as their own
-// rounding in the mean square, give or take 1.2 over the root of their size (f16
-// 1065 x 20 x 11: up to 1.66); in two halves 1.00.  us for all three gradients, rounded
-// and in halves: bf16 9 x 64 x 64 7.8 and 8.7, 64 x 64 x 64 7.2 and 8.0, 1065 x 20 x 11
-// 16.7 and 17.5, but 256 x 384 x 384 10.4 and 14.6, 1024 x 1024 x 1024 25 and 38,
-// 16384 x 1024 x 4096 354 and 610.
-constexpr int64_t FEW_RESULTS = 4096;
+// Passes over dz in the gradients' products: two, of its two halves, where dz, dx or
+// dw has few elements.  With dz rounded dx and dw are 1.41 times as far off as their own
+// rounding in the mean square, give or take about 1.2 over the root of the least of
+// the three sizes (f16 1065 x 20 x 11: up to 1.66, bf16 11 x 605 x 11 1.52); in two
+// halves 1.00.  us for all three gradients, rounded and in halves: bf16 9 x 64 x 64 7.8
+// and 8.7, 64 x 4096 x 64 7.5 and 8.5, 1065 x 20 x 11 16.7 and 17.5, but 256 x 384 x
+// 384 10.4 and 14.6, 1024 x 1024 x 1024 25 and 38, 16384 x 1024 x 4096 354 and 610.
+constexpr int64_t FEW_ELEMENTS = 4096;
 int dz_passes(int type, int act, int64_t M, int64_t N, int64_t K) {
-    return type != BERT_AMD_F32 && act != BERT_AMD_ACT_NONE && std::min(M, N) * K <= FEW_RESULTS ? 2 : 1;
+    return type != BERT_AMD_F32 && act != BERT_AMD_ACT_NONE && std::min({M * N, M * K, N * K}) <= FEW_ELEMENTS ? 2 : 1;
 }
 
 // Up to 8 rows, and no more than 8192 columns of dz: with more the tiles' workgroups

@@ -242,8 +242,8 @@ BERT_API int32_t bert_amd_linear(int32_t device, int32_t type, int32_t act, int6
    over the rows, f32 [N].  z is not read (and may be NULL) for act NONE; it may
    be any [M][N] values.  Any of dx, dw, dbias may be NULL: not computed.  F16
    and BF16 round dz to the type before the two products (F16: to an infinity past
-   65504), but not for M <= 8 with N <= 8192, nor where dx or dw is a matrix of at
-   most 4096 elements.  M = 0 gives zero dw and dbias.  `aligned` as above, of dy, x and w. */
+   65504), but not for M <= 8 with N <= 8192, nor where dz, dx or dw has at most
+   4096 elements.  M = 0 gives zero dw and dbias.  `aligned` as above, of dy, x and w. */
 BERT_API int64_t bert_amd_linear_backward_workspace(int32_t type, int32_t act, int64_t M, int32_t N, int32_t K,
                                                     int32_t aligned);
 BERT_API int32_t bert_amd_linear_backward(int32_t device, int32_t type, int32_t act, int64_t M, int32_t N, int32_t K,

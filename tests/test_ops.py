@@ -924,10 +924,10 @@ def rounded_between(v, off, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M,K,N,pad", [(1, 40, 9000, 0), (5, 72, 8200, 3), (8, 8, 9001, 0), (9, 96, 130, 0), (12, 1000, 48, 1), (40, 384, 384, 0), (63, 130, 257, 8), (64, 512, 64, 0), (700, 256, 512, 0), (9, 64, 64, 0), (64, 64, 64, 0), (1065, 20, 11, 5), (9, 455, 300, 0), (130, 31, 132, 0), (131, 33, 124, 1), (20000, 8, 12, 0), (3000, 1, 4096, 0), (4000, 3, 1366, 0)])
+@pytest.mark.parametrize("M,K,N,pad", [(1, 40, 9000, 0), (5, 72, 8200, 3), (8, 8, 9001, 0), (9, 96, 130, 0), (12, 1000, 48, 1), (40, 384, 384, 0), (63, 130, 257, 8), (64, 512, 64, 0), (700, 256, 512, 0), (9, 64, 64, 0), (64, 64, 64, 0), (1065, 20, 11, 5), (9, 455, 300, 0), (130, 31, 132, 0), (131, 33, 124, 1), (20000, 8, 12, 0), (3000, 1, 4096, 0), (4000, 3, 1366, 0), (11, 605, 11, 0), (64, 2056, 64, 0), (64, 300, 65, 0)])
 def test_linear_backward_rounds_dz_once(M, K, N, pad, dtype):
-    """Past 8 rows or 8192 columns: dz rounded to the layer's type (f32 and where dx or dw has few elements: not at
-    all), and from there on nothing is lost but sums in f32 and each result's own rounding.  f32 operands are taken whole."""
+    """Past 8 rows or 8192 columns: dz rounded to the layer's type (f32 and where dz, dx or dw has few elements: not
+    at all), and from there on nothing is lost but sums in f32 and each result's own rounding.  f32 operands are taken whole."""
     dt = DTYPES[dtype]
     x, w, dy, _ = make_layer(M, K, N, dt, seed=30)
     z = normal(gen(31), M, N).to(dt)
@@ -940,7 +940,7 @@ def test_linear_backward_rounds_dz_once(M, K, N, pad, dtype):
         kept, apart = rounded_between(dz, off, dt)
         if dt == torch.float32:
             kept, apart = dz, off
-        elif act != "none" and min(M, N) * K <= 4096:  # two halves: the second is what the first left, rounded
+        elif act != "none" and min(M * N, M * K, N * K) <= 4096:  # two halves: the second is what the first left, rounded
             kept, apart = dz, off + 2 * u(dt) ** 2 * dz.abs() + tiny(dt)
         for got, a, o, b, n, what in ((dx, kept, apart, w, N, "dx"), (dw, kept.t(), apart.t(), x, M, "dw")):
             want, far = a @ b.to(F64), (o + (n + 1) * U32 * (a.abs() + o)) @ b.to(F64).abs()
