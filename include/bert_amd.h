@@ -258,7 +258,8 @@ BERT_API int32_t bert_amd_linear_backward(int32_t device, int32_t type, int32_t 
      table    : [n_rows][width] of table_type, F32, F16, BF16 or a GGUF's Q4_0 or
                 Q4_1 rows (width a multiple of 32; a block's values as ggml's
                 get_rows gives them), ld_table_bytes between rows
-     out      : [n][width] */
+     out      : [n][width]
+   n <= 2^30, width < 2^22. */
 BERT_API int32_t bert_amd_lookup(int32_t device, int32_t table_type, int32_t out_type, int64_t n, int32_t n_rows,
                                  int32_t width, const void *table, int64_t ld_table_bytes, const int32_t *ids,
                                  float scale, void *out, int64_t ldo, void *hip_stream);

@@ -1543,3 +1543,21 @@ def test_f16_dz_past_its_largest_value():
     dy[0, 0] = float("inf")
     dx, dw, db = bertops.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z=z.cuda(), act="gelu")
     assert not torch.isfinite(dx[0]).any() and torch.isfinite(dx[1:]).all() and not torch.isnan(db).any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(4096, 20000, 1), (1024, 20000, 4), (16, 30000, 256)])
+def test_few_dz_of_wide_inputs(M, K, N, dtype):
+    """dz of few elements in two halves where dx or dw is large: the large tiles go over k twice, too."""
+    dt = DTYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(96)
+    x, w, dy, z = (torch.randn(*s, generator=g, device="cuda").to(dt) for s in ((M, K), (N, K), (M, N), (M, N)))
+    dx, dw, db = bertops.linear_backward(dy, x, w, z=z, act="silu")
+    zz = z.to(F64)
+    s = torch.sigmoid(zz)
+    dz = dy.to(F64) * (s + zz * s * (1 - s))
+    off = SLACK * U32 * (1 + zz.abs()) * dy.to(F64).abs() + 2 * u(dt) ** 2 * dz.abs() + tiny(dt)
+    for got, a, o, b, n in ((dx, dz, off, w.to(F64), N), (dw, dz.t().contiguous(), off.t().contiguous(), x.to(F64), M)):
+        want, far = a @ b, (o + (n + 1) * U32 * (a.abs() + o)) @ b.abs()
+        assert ((got.to(F64) - want).abs() <= far + u(dt) * (want.abs() + far) + tiny(dt)).all()
