@@ -74,14 +74,11 @@ def _first(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: two dimensions are needed")
 
 
-def _no_node(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Says so where the results would need a gradient that they do not get."""
+def _no_node(name: str) -> None:
+    """Says that the results of tensors that require a gradient have none, where torch would have given them one."""
     if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                warnings.warn(f"{name}() of a tensor that requires a gradient: its results have none.  Call it under torch.no_grad(), "
-                              "or in a torch.autograd.Function", stacklevel=3)
-                return
+        warnings.warn(f"{name}() of a tensor that requires a gradient: its results have none.  Call it under torch.no_grad(), "
+                      "or in a torch.autograd.Function", stacklevel=3)
 
 
 def _act(act: str) -> int:
@@ -96,11 +93,10 @@ def _vector(name: str, t: torch.Tensor, device, n: int) -> int:
     return t.data_ptr()
 
 
-def _int32(name: str, *values: int) -> None:
+def _int32(name: str, a: int, b: int = 0) -> None:
     """The library takes these in 32 bits, and ctypes would cut them off without a word."""
-    for v in values:
-        if not -(1 << 31) <= v < 1 << 31:
-            raise ValueError(f"{name} {v} is over 32 bits")
+    if not -(1 << 31) <= a < 1 << 31 or not -(1 << 31) <= b < 1 << 31:
+        raise ValueError(f"{name} {a if b == 0 else (a, b)} is over 32 bits")
 
 
 def _aligned(size: int, *matrices) -> int:
@@ -120,7 +116,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     save_z: also returns the pre-activation, (y, z), which linear_backward takes.  out: where y goes (may
     be `residual`)."""
     _first("x", x)
-    _no_node("linear", x, w, bias, residual)
+    if x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad):
+        _no_node("linear")
     (M, K), N, dt, dev, a = x.shape, w.shape[0], x.dtype, x.device, _act(act)
     _int32("a width of", N, K)
     ldx, ldw = _matrix("x", x, dt, dev, M, K), _matrix("w", w, dt, dev, N, K)
@@ -175,7 +172,8 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, table_
     a model file.  out_dtype: float32 for those, the table's own type otherwise, unless given."""
     if not table.is_cuda or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError("the table has to be a GPU tensor [rows, width]")
-    _no_node("lookup", table)
+    if table.requires_grad:
+        _no_node("lookup")
     blocks = table_type in BLOCK_BYTES
     if blocks:
         if table.dtype != torch.uint8 or table.shape[1] % BLOCK_BYTES[table_type]:

@@ -412,47 +412,48 @@ __global__ __launch_bounds__(256) void join_kernel(LookupGradArgs a, SumArgs s) 
 }
 
 // Few places (at most FEW): no sort.  A workgroup for each place looks through
-// all ids; its waves find the token's places among an eighth of the ids each,
-// sum those in order, and the eighths are added in order.  A token's r-th place
+// all ids; its waves find the token's places among at most 512 ids each, sum
+// those in order, and the waves' sums are added in order.  A token's r-th place
 // takes the columns' slices r, r + its places, ..: a rare token's first place
 // does it all, a frequent one's sums are spread over as many workgroups as there
 // are slices, so that none walks along a wide row place by place.  Again the other
 // workgroups write the zeros, and find out from the ids which rows are in use.
 // f32 of a 30522 row table, us, here and sorted: 2048 x 384 places of tokens as
-// text has them 15.4 and 48, all of one token 33 and 38; 4096 x 384 25 and 49, of
+// text has them 14.1 and 48, all of one token 58 and 38; 4096 x 384 25 and 49, of
 // one token 61 and 40; 4096 x 1023 (a column a lane) 60 and 59, of one token 93
-// and 52.  The looking grows with the places' square.  Half as many waves are 2 to
-// 5 us faster on rare tokens and twice as slow on frequent ones; the first place
-// alone at work took 307 us for 4096 x 768 of one token and 2302 for 4096 x 1023.
-constexpr int FEW = 4096, FEW_WAVES = 8, FEW_ZEROS = 4 * FEW_WAVES;
+// and 52.  The looking grows with the places' square.  Eight waves for 2048 places
+// too take 15.7 and 33, four for 4096 x 384 22 and 111; the first place alone at work
+// took 307 us for 4096 x 768 of one token and 2302 for 4096 x 1023.
+constexpr int FEW = 4096, FEW_EACH = 512;
 
-template <int TYPE, int COLS>
-__global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(LookupGradArgs a, ZeroPart z) {
+template <int TYPE, int COLS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void few_kernel(LookupGradArgs a, ZeroPart z) {
     typedef typename Elem<TYPE>::T T;
+    constexpr int ZEROS = 4 * WAVES;
     const int n = (int)a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = blockIdx.x;
     if (at >= n) {
-        __shared__ uint8_t used[FEW_ZEROS];
-        static_assert(FEW_ZEROS <= 64 * FEW_WAVES, "one thread clears one row's mark");
-        for (int64_t b = at - n; b * FEW_ZEROS < a.V; b += gridDim.x - n) {
-            const int first = (int)b * FEW_ZEROS;
+        __shared__ uint8_t used[ZEROS];
+        static_assert(ZEROS <= 64 * WAVES, "one thread clears one row's mark");
+        for (int64_t b = at - n; b * ZEROS < a.V; b += gridDim.x - n) {
+            const int first = (int)b * ZEROS;
             __syncthreads();
-            if (threadIdx.x < FEW_ZEROS) used[threadIdx.x] = 0;
+            if (threadIdx.x < ZEROS) used[threadIdx.x] = 0;
             __syncthreads();
-            for (int i = threadIdx.x; i < n; i += 64 * FEW_WAVES) {
+            for (int i = threadIdx.x; i < n; i += 64 * WAVES) {
                 const int id = a.ids[i];
-                if (id >= first && id < first + FEW_ZEROS && id != a.pad_id) used[id - first] = 1;
+                if (id >= first && id < first + ZEROS && id != a.pad_id) used[id - first] = 1;
             }
             __syncthreads();
-            zero_rows<FEW_ZEROS>(z, first, used);
+            zero_rows<ZEROS>(z, first, used);
         }
         return;
     }
     const int k = sort_key(a.ids[at], a.V, a.pad_id);
     if (k == a.V) return;
-    __shared__ uint16_t list[FEW_WAVES][FEW / FEW_WAVES];
-    __shared__ int counts[FEW_WAVES], before[FEW_WAVES];
-    __shared__ float sums[FEW_WAVES - 1][64][COLS + 1];
-    const int share = ceil_div(n, 64 * FEW_WAVES) * 64, from = wave * share;
+    __shared__ uint16_t list[WAVES][FEW_EACH];
+    __shared__ int counts[WAVES], before[WAVES];
+    __shared__ float sums[WAVES - 1][64][COLS + 1];
+    const int share = ceil_div(n, 64 * WAVES) * 64, from = wave * share;
     int count = 0, earlier = 0;
     for (int i = from; i < min(n, from + share); i += 64) {
         const bool same = i + lane < n && a.ids[i + lane] == k;
@@ -465,7 +466,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(LookupGradArgs a, Z
     __syncthreads();
     int rank = 0, places = 0;  // of this place among its token's
 #pragma unroll
-    for (int w = 0; w < FEW_WAVES; w++) rank += before[w], places += counts[w];
+    for (int w = 0; w < WAVES; w++) rank += before[w], places += counts[w];
     for (int e0 = rank * 64 * COLS; e0 < a.E; e0 += places * 64 * COLS) {
         const int e = e0 + lane * COLS;
         float sum[COLS] = {};
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(LookupGradArgs a, Z
         __syncthreads();
         if (!wave && e < a.E) {
 #pragma unroll
-            for (int w = 0; w < FEW_WAVES - 1; w++)
+            for (int w = 0; w < WAVES - 1; w++)
 #pragma unroll
                 for (int c = 0; c < COLS; c++) sum[c] += sums[w][lane][c];
             store_row<COLS>(a, k, e, sum);
@@ -524,10 +525,15 @@ hipError_t sum_t(const LookupGradArgs &a, const SumArgs &p, hipStream_t s) {
     if (hipError_t e = launch(sum_kernel<TYPE, COLS>, dim3(p.tiles, across), dim3(threads), 0, s, a, p); e != hipSuccess) return e;
     return launch(join_kernel<COLS>, dim3(p.tiles, ceil_div(a.E, 64 * COLS)), dim3(256), 0, s, a, p);
 }
+template <int TYPE, int COLS, int WAVES>
+hipError_t few_w(const LookupGradArgs &a, const ZeroPart &z, hipStream_t s) {
+    const int groups = (int)a.n + zero_groups(z, 4 * WAVES);
+    return groups ? launch(few_kernel<TYPE, COLS, WAVES>, dim3(groups), dim3(64 * WAVES), 0, s, a, z) : hipSuccess;
+}
 template <int TYPE, int COLS>
 hipError_t few_t(const LookupGradArgs &a, const ZeroPart &z, hipStream_t s) {
-    const int groups = (int)a.n + zero_groups(z, FEW_ZEROS);
-    return groups ? launch(few_kernel<TYPE, COLS>, dim3(groups), dim3(64 * FEW_WAVES), 0, s, a, z) : hipSuccess;
+    static_assert(8 * FEW_EACH == FEW, "eight waves take all places");
+    return a.n <= 4 * FEW_EACH ? few_w<TYPE, COLS, 4>(a, z, s) : few_w<TYPE, COLS, 8>(a, z, s);
 }
 // four columns a thread where rows and places allow it
 bool four_columns(const LookupGradArgs &a) {
