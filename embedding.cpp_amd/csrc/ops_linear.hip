@@ -285,8 +285,9 @@ __global__ __launch_bounds__(256) void pack_kernel(Packing a, Packing b) {
 //
 // Measured (us): bf16 8192 x 8192 x 8192 861 (1.28 PFLOP/s; all-zero operands
 // run a fifth faster: the chip's power bounds it with the LDS reads, 96 of 128
-// bytes a clock at the full rate); 32768 x 1024 x 4096 270, of which 33 are the
-// way out's LDS passes and 15 its stores; four waves of 128 x 128 each instead
+// bytes a clock at the full rate); 32768 x 1024 x 4096 270, 198 of them
+// the main loop's and 72 around it, with the matrix units idle: eight rounds of first
+// loads and the way out, 33 its LDS passes and 15 its stores; four waves of 128 x 128 each instead
 // of eight of 128 x 64 took 5 % longer.  f32 65536 x 1536 x 384 590 (131
 // TFLOP/s, the matrix units busy 9 parts in 10).  With one workgroup on a CU a
 // wave's LDS reads bound a 128 x 128 stage (0.7 us, its products take 0.25);
