@@ -57,3 +57,23 @@ def test_int8_qkv_gemm_priced_by_resolved_choice():
     assert bench.dtype_label("q4_1", off) == "fp16"
     # the pc kernel reports i8_qkv = 1 with qkva_ntw = 0
     assert bench.kernel_parts("gemm_qkv", 8, 128, HP, dict(PC, i8_qkv=1), "q4_0")[0][1] == bench.PEAK_INT8_TOPS
+
+
+def test_pmc_traffic_deals_shared_kernels_in_dispatch_order(tmp_path):
+    """o-proj and FFN-down on the same kernel but for the last layer's: their dispatches alternate over both kernels."""
+    import json
+    import subprocess
+
+    one, last = ("void bertamd::i8_ln384_kernel<2, %s, true>(bertamd::GemmArgs, int)" % b for b in ("true", "false"))
+    for counter, o, down in (("FETCH_SIZE", 10.0, 20.0), ("WRITE_SIZE", 3.0, 5.0)):
+        d = tmp_path / counter
+        d.mkdir()
+        lines = ["Dispatch_Id,Kernel_Name,Counter_Name,Counter_Value"]
+        for i in range(36):  # three steps of six layers
+            lines.append('%d,"%s",%s,%f' % (2 * i + 7, last if i % 12 == 11 else one, counter, down if i % 2 else o))
+        (d / "x_counter_collection.csv").write_text("\n".join(lines) + "\n")
+    out = tmp_path / "t.json"
+    subprocess.run([sys.executable, os.path.join(os.path.dirname(bench.__file__), "tools", "pmc_traffic.py"), str(tmp_path / "FETCH_SIZE"), str(tmp_path / "WRITE_SIZE"), "w", str(out)], check=True)
+    got = json.loads(out.read_text())
+    assert got["fetch_bytes"] == {"gemm_o_ln": 20480, "gemm_down_ln": 40960}
+    assert got["write_bytes"] == {"gemm_o_ln": 3072, "gemm_down_ln": 5120}

@@ -63,10 +63,11 @@ def main():
         fv, wv = [], []
         group = share.get(tuple(hits[name]), [name])
         slot, n_share = group.index(name), len(group)
-        for k in hits[name]:
-            for src, dst in ((fetch, fv), (write, wv)):
-                ds = sorted(src.get(k, {}).items(), key=lambda kv: int(kv[0]) if str(kv[0]).isdigit() else 0)
-                dst += [v for i, (_, v) in enumerate(ds) if i % n_share == slot]
+        for src, dst in ((fetch, fv), (write, wv)):
+            # of all the kernels it resolves to in one order: the last layer's FFN-down is another one
+            ds = sorted((kv for k in hits[name] for kv in src.get(k, {}).items()),
+                        key=lambda kv: int(kv[0]) if str(kv[0]).isdigit() else 0)
+            dst += [v for i, (_, v) in enumerate(ds) if i % n_share == slot]
         if fv and wv:
             fb = 2.0 * sum(fv) / len(fv) * 1024.0
             wb = sum(wv) / len(wv) * 1024.0
