@@ -1071,7 +1071,7 @@ def test_lookup_grad_of_one_token_is_spread():
         end.synchronize()
         return start.elapsed_time(end)
 
-    assert time_of(4096) < 10 * time_of(4097)
+    assert min(time_of(4096) for _ in range(3)) < 10 * min(time_of(4097) for _ in range(3))
 
 
 # ---- the two ways over a layer's dz
@@ -1110,8 +1110,7 @@ def test_backward_of_wide_layers_takes_whole_lines():
         end.synchronize()
         return start.elapsed_time(end)
 
-    time_of(1040)
-    assert time_of(1000) < 2 * time_of(1040)
+    assert min(time_of(1000) for _ in range(4)) < 2 * min(time_of(1040) for _ in range(4))
 
 
 # ---- what Adapter and TokenTable keep between their calls
