@@ -226,7 +226,7 @@ int32_t bert_amd_lookup(int32_t device, int32_t table_type, int32_t out_type, in
     if (n == 0) return 0;
     const int e = is_float(table_type) ? size_of(table_type) : 2;
     const int64_t row = blocks ? (int64_t)ggml_row_bytes(table_type, width) : (int64_t)width * e;
-    if (!table || off(table, e) || ld_table_bytes < row || ld_table_bytes % e || ld_table_bytes > (int64_t)1 << 40)
+    if (!table || off(table, e) || (ld_table_bytes != 0 && ld_table_bytes < row) || ld_table_bytes % e || ld_table_bytes > (int64_t)1 << 40)
         return refuse("bert_amd_lookup: table is null, misaligned or has too short rows");
     if (!ids || off(ids, 4)) return refuse("bert_amd_lookup: ids are null or misaligned");
     if (const char *bad = bad_matrix({"out", out, ldo, width, false, size_of(out_type)}))

@@ -1560,3 +1560,23 @@ def test_few_dz_of_wide_inputs(M, K, N, dtype):
     for got, a, o, b, n in ((dx, dz, off, w.to(F64), N), (dw, dz.t().contiguous(), off.t().contiguous(), x.to(F64), M)):
         want, far = a @ b, (o + (n + 1) * U32 * (a.abs() + o)) @ b.abs()
         assert ((got.to(F64) - want).abs() <= far + u(dt) * (want.abs() + far) + tiny(dt)).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "q4_0"])
+def test_lookup_in_one_row(kind):
+    """A table whose rows are the same one again, as every input's may be: 0 elements apart."""
+    table, values = make_table(kind, 1, 96)
+    ids = torch.tensor([0, 4, 5, -1], dtype=torch.int32)
+    got = bertops.lookup(table.cuda().expand(5, -1), ids.cuda(), scale=2.0, table_type=kind, out_dtype=torch.float32).cpu()
+    assert torch.equal(got, (values * 2.0).float().expand(4, 96) * torch.tensor([1.0, 1.0, 0.0, 0.0])[:, None])
+
+
+def test_rows_of_a_table_that_are_one():
+    """0 bytes between rows pass the library's checks; without a GPU only the device call refuses them."""
+    L, P = bertlib.lib(), 1 << 20
+    args = dict(device=0, type=2, out=0, n=4, V=10, E=64, table=P, ld=0, ids=P, scale=1.0, o=P + 4096, ldo=64, s=None)
+    if not torch.cuda.is_available():
+        assert L.bert_amd_lookup(*args.values()) == -3
+    assert L.bert_amd_lookup(*{**args, "ld": -36}.values()) == -1
+    assert L.bert_amd_lookup(*{**args, "o": P + 16}.values()) == -1
