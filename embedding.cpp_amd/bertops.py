@@ -337,14 +337,19 @@ class _Own:
         return self._tensors
 
 
+def _version(t: torch.Tensor) -> int:
+    return 0 if t.is_inference() else t._version
+
+
 class _Kept:
     """What a training forward keeps for its backward: one forward at a time, until the weights move."""
 
     def __init__(self):
         self._what, self._open = None, 0  # the newest forward's; forwards since the last backward
+        self._versions = []
 
     def put(self, *tensors: torch.Tensor) -> None:
-        self._what, self._open = _Own(*tensors), self._open + 1
+        self._what, self._open, self._versions = _Own(*tensors), self._open + 1, [_version(t) for t in tensors]
 
     def get(self):
         if self._what is None:
@@ -354,7 +359,10 @@ class _Kept:
             raise ValueError("two forwards before a backward, whose gradient is meant? Take both batches in one forward, "
                              "and forwards without a backward with train=False")
         self._open = 0
-        return self._what.use()
+        tensors = self._what.use()
+        if [_version(t) for t in tensors] != self._versions:
+            raise ValueError("an input of forward() has been changed in place since: its backward needs it as it was")
+        return tensors
 
     def drop(self) -> None:
         self._what, self._open = None, 0

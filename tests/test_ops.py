@@ -1580,3 +1580,23 @@ def test_rows_of_a_table_that_are_one():
         assert L.bert_amd_lookup(*args.values()) == -3
     assert L.bert_amd_lookup(*{**args, "ld": -36}.values()) == -1
     assert L.bert_amd_lookup(*{**args, "o": P + 16}.values()) == -1
+
+
+@gpu
+def test_trained_layers_refuse_changed_inputs():
+    """Embeddings or ids overwritten between forward and backward; fresh ones, and inference tensors, pass."""
+    a, t = bertops.Adapter(32), token_table()
+    e, dy = (normal(gen(s), 6, 32).float().cuda() for s in (97, 98))
+    ids = torch.arange(6, dtype=torch.int32, device="cuda")
+    for o, x in ((a, e), (t, ids)):
+        o.forward(x)
+        x.add_(1)
+        with pytest.raises(ValueError, match="changed in place"):
+            o.backward(dy)
+        o.forward(x)
+        o.backward(dy)
+        o.step()
+        with torch.inference_mode():
+            o.forward(x.clone())
+            o.backward(dy)
+            o.step()
