@@ -65,7 +65,7 @@ def test_pmc_traffic_deals_shared_kernels_in_dispatch_order(tmp_path):
     import subprocess
 
     one, last = ("void bertamd::i8_ln384_kernel<2, %s, true>(bertamd::GemmArgs, int)" % b for b in ("true", "false"))
-    for counter, o, down in (("FETCH_SIZE", 10.0, 20.0), ("WRITE_SIZE", 3.0, 5.0)):
+    for counter, o, down in (("FETCH_SIZE", 10.0, 20.0), ("WRITE_SIZE", 4.0, 5.0)):
         d = tmp_path / counter
         d.mkdir()
         lines = ["Dispatch_Id,Kernel_Name,Counter_Name,Counter_Value"]
@@ -76,4 +76,4 @@ def test_pmc_traffic_deals_shared_kernels_in_dispatch_order(tmp_path):
     subprocess.run([sys.executable, os.path.join(os.path.dirname(bench.__file__), "tools", "pmc_traffic.py"), str(tmp_path / "FETCH_SIZE"), str(tmp_path / "WRITE_SIZE"), "w", str(out)], check=True)
     got = json.loads(out.read_text())
     assert got["fetch_bytes"] == {"gemm_o_ln": 20480, "gemm_down_ln": 40960}
-    assert got["write_bytes"] == {"gemm_o_ln": 3072, "gemm_down_ln": 5120}
+    assert got["write_bytes"] == {"gemm_o_ln": 4096, "gemm_down_ln": 5120}
